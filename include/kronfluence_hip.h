@@ -439,6 +439,59 @@ int kf_mul_bcast(float* out, const void* X, int x_dtype, const float* M, int64_t
 /* Elementwise helper: dst[i] = (out_dtype) src[i] -- export of fp32 accumulators in the factor dtype. */
 int kf_cast(void* dst, int dst_dtype, const void* src, int src_dtype, int64_t numel, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Model passes (ABI 15) -- the untracked parts of a transformer that every stage runs forward and
+ * backward between the tracked layers.  All of them: fp32 statistics, sums and accumulators, one
+ * rounding of each output; no atomics (a result does not depend on the order of workgroups).
+ * ------------------------------------------------------------------------------------------- */
+
+/* A [batch][token][head][width] operand, the width contiguous: strides in elements, the pointer 16-byte aligned, every stride a
+ * multiple of 16 bytes (slices of a fused projection are taken as they are).  Packed batches ignore batch_stride. */
+typedef struct kf_heads_view {
+    const void* p;
+    int64_t batch_stride, token_stride, head_stride;
+} kf_heads_view;
+
+/*
+ * out = softmax(scale q k' + mask) v over whole prompts; KF_BF16 or KF_F32 (every tensor in the same type).
+ *
+ * Padded batch (offsets == NULL): `sequences` rows of `length` tokens, rows = sequences * length; lengths (device int32
+ * [sequences], nullable) gives the real tokens of each row, the first ones.  Packed batch: sequence s is token rows
+ * offsets[s] .. offsets[s + 1] (device int32 [sequences + 1]) of `rows` in all; lengths == NULL, `length` ignored.  Values are
+ * clamped to the rows that exist.  causal: token i sees tokens 0 .. i of its sequence, otherwise every real token of it.
+ * Query head h reads key / value head h / (heads / kv_heads).
+ *
+ * Rows that hold no real token (padding; packed rows behind the last sequence) get out = 0 and, in the backward pass, gradients of
+ * 0; what the inputs hold there is never used.  lse (fp32 [heads][rows], nullable in the forward call): log2 of the sum of
+ * 2^(scale log2(e) q.k), +inf for rows without a token; the backward call needs it.
+ * width <= 128, a multiple of 8 (bf16) or 4 (fp32); scale > 0.
+ */
+int kf_attention_forward(const kf_heads_view* out, float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v,
+                         int dtype, int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width,
+                         const int32_t* lengths, const int32_t* offsets, int causal, float scale, void* stream);
+int64_t kf_attention_backward_workspace_bytes(int64_t rows, int64_t heads);
+int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, const kf_heads_view* dv, const kf_heads_view* grad,
+                          const kf_heads_view* out, const float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v,
+                          int dtype, int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width,
+                          const int32_t* lengths, const int32_t* offsets, int causal, float scale, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+
+/*
+ * y = (x - mu) r w + b over the last axis: layer norm (centred != 0) or RMS norm (centred == 0: mu = 0), r = 1 / sqrt(mean (x - mu)^2
+ * + eps).  x: [rows][width], rows row_stride elements apart; y: contiguous, in a type of its own (KF_F32, KF_BF16, KF_F16 each, at
+ * any element alignment).  weight, bias: [width] in w_dtype, nullable.  stats (fp32 [rows][2]: mu, r; nullable) is what the
+ * backward call reads.
+ *
+ * Backward: dx [rows][width] contiguous in x's type, dweight and dbias [width] in w_dtype; each nullable (not computed).  grad:
+ * contiguous.  The workspace (needed for dweight / dbias) holds one partial row of sums per workgroup.
+ */
+int kf_norm_forward(void* y, int y_dtype, float* stats, const void* x, int x_dtype, int64_t rows, int64_t width, int64_t row_stride,
+                    const void* weight, const void* bias, int w_dtype, int centred, float eps, void* stream);
+int64_t kf_norm_backward_workspace_bytes(int64_t rows, int64_t width);
+int kf_norm_backward(void* dx, void* dweight, void* dbias, const void* grad, int grad_dtype, const void* x, int x_dtype, const float* stats,
+                     int64_t rows, int64_t width, int64_t row_stride, const void* weight, int w_dtype, int centred, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,7 +15,7 @@ from typing import Optional
 import torch  # noqa: F401  (must precede the dlopen below)
 
 LIB_NAME = "libkronfluence_hip.so"
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 KF_F32, KF_BF16, KF_F16, KF_F64, KF_I64, KF_I32, KF_U8 = range(7)
 
@@ -39,7 +39,13 @@ class kf_view(ctypes.Structure):
     ]
 
 
+class kf_heads_view(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
 _i, _i64, _p, _f, _d = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float, ctypes.c_double
+
+_h = ctypes.POINTER(kf_heads_view)
 
 # name -> (restype, argtypes); mirrors include/kronfluence_hip.h declaration by declaration.
 SIGNATURES = {
@@ -85,6 +91,12 @@ SIGNATURES = {
     "kf_lowrank_rows_dot": (_i, [_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _f, _p]),
     "kf_mul_bcast": (_i, [_p, _p, _i, _p, _i64, _i64, _f, _p]),
     "kf_cast": (_i, [_p, _i, _p, _i, _i64, _p]),
+    "kf_attention_forward": (_i, [_h, _p, _h, _h, _h, _i] + [_i64] * 6 + [_p, _p, _i, _f, _p]),
+    "kf_attention_backward_workspace_bytes": (_i64, [_i64, _i64]),
+    "kf_attention_backward": (_i, [_h] * 5 + [_p] + [_h] * 3 + [_i] + [_i64] * 6 + [_p, _p, _i, _f, _p, _i64, _p]),
+    "kf_norm_forward": (_i, [_p, _i, _p, _p, _i, _i64, _i64, _i64, _p, _p, _i, _i, _f, _p]),
+    "kf_norm_backward_workspace_bytes": (_i64, [_i64, _i64]),
+    "kf_norm_backward": (_i, [_p, _p, _p, _p, _i, _p, _i, _p, _i64, _i64, _i64, _p, _i, _i, _p, _i64, _p]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

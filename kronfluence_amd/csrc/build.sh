@@ -10,7 +10,8 @@ flags=(--offload-arch=gfx950 -O3 -std=c++17 -fPIC -munsafe-fp-atomics -Wall -Wno
        -Xclang -target-feature -Xclang -packed-fp32-ops)
 mkdir -p "${here}/obj"
 pids=()
-for src in kf_kernels kf_eigh kf_score_v2; do
+units=(kf_kernels kf_eigh kf_score_v2 kf_attention kf_norm)
+for src in "${units[@]}"; do
   stale=0
   [[ -f "${here}/obj/${src}.o" ]] || stale=1
   for dep in "${here}/${src}.hip" "${here}"/*.h "${here}/../../include/kronfluence_hip.h"; do
@@ -22,5 +23,7 @@ for src in kf_kernels kf_eigh kf_score_v2; do
   fi
 done
 for p in "${pids[@]:-}"; do [[ -n "${p}" ]] && wait "${p}"; done
-"${HIPCC}" --offload-arch=gfx950 -shared -fPIC "${here}/obj/kf_kernels.o" "${here}/obj/kf_eigh.o" "${here}/obj/kf_score_v2.o" -o "${out}"
+objects=("${units[@]/#/${here}/obj/}")
+objects=("${objects[@]/%/.o}")
+"${HIPCC}" --offload-arch=gfx950 -shared -fPIC "${objects[@]}" -o "${out}"
 echo "built ${out}"

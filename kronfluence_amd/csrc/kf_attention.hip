@@ -1,0 +1,720 @@
+// kf_attention.hip -- attention over whole prompts, forward and backward (see include/kronfluence_hip.h, "Model passes").
+//
+// Mathematics (per sequence and head; c = scale * log2 e):
+//     s_ij = q_i . k_j          p_ij = 2^(c s_ij - L_i)      L_i = log2 sum_j 2^(c s_ij)      o_i = sum_j p_ij v_j
+//     D_i = do_i . o_i          ds_ij = p_ij (do_i . v_j - D_i)
+//     dq_i = scale sum_j ds_ij k_j     dk_j = scale sum_i ds_ij q_i     dv_j = sum_i p_ij do_i
+// j runs over the visible keys of i.  The heads of a group share k and v; their dk, dv are summed in registers (no atomics: the
+// result does not depend on the order in which workgroups run).
+//
+// One pass over the keys with a running maximum and sum: the scores never leave the registers.  Every product is a 32 x 32 matrix
+// instruction tile with the LANE as the row that owns softmax statistics:
+//     forward, dQ:  S^T = K Q^T  (lane = query, registers = keys)   ->  O^T += V^T P^T,   dQ^T += K^T dS^T
+//     dK / dV:      S   = Q K^T  (lane = key,  registers = queries) ->  dV^T += dO^T P,   dK^T += Q^T dS
+// The accumulator layout (register r of lane half h holds row 8 (r / 4) + 4 h + r % 4) IS the operand layout of the second product
+// once the contraction index is permuted the same way in its other operand, so P and dS go from accumulator to operand by
+// conversion alone, with no cross-lane traffic; the other operand is read from LDS column-wise (ds_read_b64_tr_b16 for 2-byte
+// types, plain 4-byte reads for fp32).  fp32 runs on v_mfma_f32_32x32x2_f32 with the same structure: exact fp32 products.
+//
+// Roundings to fewer bits than 32: P and dS are rounded to bf16 as operands of their second product when the inputs are bf16 (one
+// rounding of half a step, 2^-9 relative, per term of a sum whose inputs carry the same rounding), and the outputs once at the end.
+// Maxima, sums, L, D and all accumulators are fp32.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "../../include/kronfluence_hip.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int THREADS = 256;      // 4 waves
+constexpr int ROWS = 128;         // rows (queries; keys in the dK / dV kernel) of a workgroup: 32 per wave
+constexpr float LOG2E = 1.44269504088896340736f;
+
+struct Tensor {   // [batch][token][head][width], the width contiguous; strides in elements
+    const void* p;
+    int64_t batch, token, head;
+};
+
+struct Args {
+    Tensor q, k, v, o, g;          // g: the gradient of o
+    Tensor dq, dk, dv;
+    float* lse;                    // [heads][rows]: L
+    float* delta;                  // [heads][rows]: D
+    const int32_t* lengths;        // per sequence (padded batch), or null
+    const int32_t* offsets;        // [sequences + 1] (packed batch), or null
+    int64_t rows;                  // token rows in all: batch * length, or the packed total
+    int sequences, length;         // length: token rows per sequence (padded batch)
+    int heads, group, width, causal;
+    int slots;                     // tile slots of all sequences
+    float scale;
+};
+
+// ---- element types ---------------------------------------------------------------------------------------------------------
+template <class T>
+struct Type;
+
+template <>
+struct Type<__bf16> {
+    typedef bf16x8 Frag;                       // 16 bytes: the lane's part of a 16-deep contraction slab
+    static constexpr int SLAB_REGS = 8;        // accumulator registers that make one operand of the second product
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ Frag from_acc(const f32x16& s, int slab) {
+        Frag f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = static_cast<__bf16>(s[8 * slab + i]);
+        return f;
+    }
+    static __device__ __forceinline__ void store4(void* p, float a, float b, float c, float d) {
+        bf16x4 v = {static_cast<__bf16>(a), static_cast<__bf16>(b), static_cast<__bf16>(c), static_cast<__bf16>(d)};
+        *reinterpret_cast<bf16x4*>(p) = v;
+    }
+    static __device__ __forceinline__ float dot(Frag a, Frag b, float acc) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc = fmaf(static_cast<float>(a[i]), static_cast<float>(b[i]), acc);
+        return acc;
+    }
+};
+
+template <>
+struct Type<float> {
+    typedef f32x4 Frag;                        // an 8-deep slab: four instructions of depth 2, one component each
+    static constexpr int SLAB_REGS = 4;
+    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ Frag from_acc(const f32x16& s, int slab) {
+        Frag f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = s[4 * slab + i];
+        return f;
+    }
+    static __device__ __forceinline__ void store4(void* p, float a, float b, float c, float d) {
+        f32x4 v = {a, b, c, d};
+        *reinterpret_cast<f32x4*>(p) = v;
+    }
+    static __device__ __forceinline__ float dot(Frag a, Frag b, float acc) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc = fmaf(a[i], b[i], acc);
+        return acc;
+    }
+};
+
+// ---- an operand tile in LDS: [row][16-byte chunk], the chunk XORed with a function of the row --------------------------------
+// Two kinds of reads meet the same image.  Row fragments: 32 consecutive rows, one 16-byte chunk each -- any 16 consecutive rows
+// must fall into the 16 different 16-byte slots of the 256-byte bank space.  Transposed reads of 2-byte types: 4 consecutive rows,
+// 64 consecutive bytes each -- the four must fall into its four quarters.
+template <class T, int DP>
+struct Image {
+    static constexpr int CHUNKS = DP * static_cast<int>(sizeof(T)) / 16;
+    static constexpr int ROW_BYTES = CHUNKS * 16;
+    static constexpr int SLABS = CHUNKS / 2;
+    static __device__ __forceinline__ int swizzle(int row, int chunk) {
+        if constexpr (sizeof(T) == 2) {
+            const int low = (row >> 2) & 3;
+            if constexpr (CHUNKS == 16) return chunk ^ (((row & 3) << 2) | low);
+            else if constexpr (CHUNKS == 8) return chunk ^ ((((row >> 1) & 1) << 2) | low);
+            else return chunk ^ low;
+        } else {
+            if constexpr (CHUNKS % 16 == 0) return chunk ^ (row & 15);
+            else return chunk ^ ((row >> 1) & 7);
+        }
+    }
+    static __device__ __forceinline__ int at(int row, int chunk) { return row * ROW_BYTES + swizzle(row, chunk) * 16; }
+
+    // the lane's fragment of rows row0 .. row0 + 31, contraction slab `slab`
+    static __device__ __forceinline__ typename Type<T>::Frag row_fragment(const char* tile, int row0, int slab, int lane) {
+        return *reinterpret_cast<const typename Type<T>::Frag*>(tile + at(row0 + (lane & 31), 2 * slab + (lane >> 5)));
+    }
+    // the lane's fragment of the TRANSPOSED tile: columns d0 .. d0 + 31 as rows, contraction over the tile rows that registers
+    // [SLAB_REGS * slab, SLAB_REGS * (slab + 1)) of an accumulator over rows row0 .. row0 + 31 stand for
+    static __device__ __forceinline__ typename Type<T>::Frag column_fragment(const char* tile, int row0, int slab, int d0, int lane) {
+        if constexpr (sizeof(T) == 2) {
+            const int g = lane >> 4, s = lane & 15;
+            const int row = row0 + 16 * slab + 4 * (g >> 1) + (s >> 2), d = d0 + 16 * (g & 1) + 4 * (s & 3);
+            union { s16x4 h[2]; bf16x8 v; } u;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                u.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s16x4*)(tile + at(row + 8 * i, d >> 3) + (d & 7) * 2));
+            return u.v;
+        } else {
+            f32x4 v;
+            const int row = row0 + 8 * slab + 4 * (lane >> 5), d = d0 + (lane & 31);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const float*>(tile + at(row + i, d >> 2) + (d & 3) * 4);
+            return v;
+        }
+    }
+};
+
+// Global rows [row0, row0 + N) of a tile into registers (every thread a few 16-byte chunks), and from there to LDS.  A row behind
+// the sequence's last reads the last one instead: what stands behind it may be anything, and its weight is 0.  Columns behind the
+// head width are 0.
+template <class T, int DP, int N>
+struct Stage {
+    typedef Image<T, DP> Img;
+    static constexpr int PER = N * Img::CHUNKS / THREADS;
+    static_assert(PER * THREADS == N * Img::CHUNKS, "whole chunks per thread");
+    u32x4 r[PER];
+    __device__ __forceinline__ void load(const T* base, int64_t token, int row0, int length, int width, int tid) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int n = tid + i * THREADS, row = n / Img::CHUNKS, chunk = n % Img::CHUNKS;
+            const int from = min(row0 + row, length - 1);
+            u32x4 v = {0, 0, 0, 0};
+            if (chunk * (16 / static_cast<int>(sizeof(T))) < width)
+                v = *reinterpret_cast<const u32x4*>(base + from * token + chunk * (16 / static_cast<int>(sizeof(T))));
+            r[i] = v;
+        }
+    }
+    __device__ __forceinline__ void store(char* tile, int tid) const {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int n = tid + i * THREADS;
+            *reinterpret_cast<u32x4*>(tile + Img::at(n / Img::CHUNKS, n % Img::CHUNKS)) = r[i];
+        }
+    }
+};
+
+// ---- which rows a workgroup works on --------------------------------------------------------------------------------------
+struct Place {
+    int64_t sequence, start;   // batch index; first token row (packed)
+    int64_t stat;              // row of lse / delta of the sequence's token 0
+    int length, written;       // visible tokens; token rows whose outputs this sequence owns (>= length: the rest is set to 0)
+    int row0;                  // first row of the workgroup's tile
+};
+
+// Tile slots.  Padded batch: ceil(length / ROWS) per sequence.  Packed batch: sequence s takes slots [c_s / ROWS + s,
+// c_{s+1} / ROWS + s + 1) with c the offsets -- at least ceil(len / ROWS) of them, found by a binary search without a table or a
+// host copy of the offsets; the rows behind the last sequence are one more sequence of no visible tokens.  Offsets outside
+// [0, rows] are clamped, so that no content of the offsets can send an access out of bounds.
+__device__ __forceinline__ bool locate(const Args& a, int slot, bool last_first, Place& w) {
+    if (a.offsets == nullptr) {
+        const int tiles = (a.length + ROWS - 1) / ROWS, s = slot / tiles, t = slot - s * tiles;
+        w.sequence = s; w.start = 0; w.stat = static_cast<int64_t>(s) * a.length;
+        w.written = a.length;
+        w.length = a.lengths ? min(max(a.lengths[s], 0), a.length) : a.length;
+        w.row0 = (last_first ? tiles - 1 - t : t) * ROWS;
+        return true;
+    }
+    const int total = static_cast<int>(a.rows);
+    auto offset = [&](int s) { return s > a.sequences ? total : min(max(a.offsets[s], 0), total); };
+    auto first_slot = [&](int s) { return offset(s) / ROWS + s; };
+    int lo = 0, hi = a.sequences;   // first_slot(lo) <= slot; the last such
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first_slot(mid) <= slot) lo = mid; else hi = mid - 1;
+    }
+    const int begin = offset(lo), rows = max(offset(lo + 1) - begin, 0);
+    int t = slot - first_slot(lo);
+    const int tiles = (rows + ROWS - 1) / ROWS;
+    if (t < 0 || t >= tiles) return false;
+    if (last_first) t = tiles - 1 - t;
+    w.sequence = 0; w.start = begin; w.stat = begin;
+    w.written = rows;
+    w.length = lo == a.sequences ? 0 : rows;
+    w.row0 = t * ROWS;
+    return true;
+}
+
+// Workgroup -> (slot, head).  Consecutive workgroup ids go to the eight XCDs in turn and each has an L2 of its own: an XCD gets a
+// contiguous run of work items, ordered so that the items that read the same k and v (the query heads of a group, the tiles of a
+// sequence) are neighbours.
+__device__ __forceinline__ int64_t work_item(int64_t id, int64_t count) {
+    constexpr int XCDS = 8;
+    const int64_t per = count / XCDS, rest = count % XCDS, x = id % XCDS, n = id / XCDS;
+    return x * per + min(x, rest) + n;
+}
+
+template <class T>
+__device__ __forceinline__ const T* rows_of(const Tensor& t, const Place& w, int head) {
+    return reinterpret_cast<const T*>(t.p) + w.sequence * t.batch + w.start * t.token + head * t.head;
+}
+template <class T>
+__device__ __forceinline__ T* rows_out(const Tensor& t, const Place& w, int head) { return const_cast<T*>(rows_of<T>(t, w, head)); }
+
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+
+// The fragments of 32 rows straight from memory (lane & 31 = row): the operand a wave keeps for the whole kernel.
+template <class T, int DP>
+struct Held {
+    typename Type<T>::Frag f[Image<T, DP>::SLABS];
+    __device__ __forceinline__ void load(const T* base, int64_t token, int row, int length, int width, int lane) {
+        constexpr int PER = 16 / static_cast<int>(sizeof(T));
+        const T* p = base + min(row, length - 1) * token;
+#pragma unroll
+        for (int s = 0; s < Image<T, DP>::SLABS; ++s) {
+            const int c = 2 * s + (lane >> 5);
+            typename Type<T>::Frag v = {};
+            if (c * PER < width) v = *reinterpret_cast<const typename Type<T>::Frag*>(p + c * PER);
+            f[s] = v;
+        }
+    }
+};
+
+// acc^T (lane = row, registers = columns d) -> memory, times `factor`
+template <class T, int DP>
+__device__ __forceinline__ void store_rows(const f32x16 (&acc)[DP / 32], T* base, int64_t token, int row, int written, int width, float factor,
+                                           int lane) {
+    if (row >= written) return;
+    T* p = base + row * token;
+#pragma unroll
+    for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = 32 * t + 8 * i + 4 * (lane >> 5);
+            if (d < width)
+                Type<T>::store4(p + d, acc[t][4 * i] * factor, acc[t][4 * i + 1] * factor, acc[t][4 * i + 2] * factor, acc[t][4 * i + 3] * factor);
+        }
+}
+
+template <class T, int DP>
+__device__ __forceinline__ void zero_rows(T* base, int64_t token, int row0, int written, int width, int tid) {
+    constexpr int PER = 16 / static_cast<int>(sizeof(T));
+    const int chunks = width / PER;
+    for (int n = tid; n < ROWS * chunks; n += THREADS) {
+        const int row = row0 + n / chunks;
+        if (row < written) *reinterpret_cast<u32x4*>(base + row * token + (n % chunks) * PER) = u32x4{0, 0, 0, 0};
+    }
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------------
+template <class T, int DP, int BK>
+__global__ __launch_bounds__(THREADS, 1) void attention_forward_kernel(const Args a) {
+    typedef Image<T, DP> Img;
+    typedef typename Type<T>::Frag Frag;
+    constexpr int TILE = BK * Img::ROW_BYTES, SECOND = 16 / Type<T>::SLAB_REGS;
+    extern __shared__ __align__(16) char lds[];   // [2][k tile, v tile]
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t item = work_item(blockIdx.x, gridDim.x);
+    const int member = static_cast<int>(item % a.group);
+    const int slot = static_cast<int>(item / a.group % a.slots);
+    const int kv_head = static_cast<int>(item / a.group / a.slots), head = kv_head * a.group + member;
+    Place w;
+    if (!locate(a, slot, a.causal, w)) return;
+    T* o = rows_out<T>(a.o, w, head);
+    float* lse = a.lse ? a.lse + head * a.rows + w.stat : nullptr;
+    if (w.row0 >= w.length) {
+        zero_rows<T, DP>(o, a.o.token, w.row0, w.written, a.width, tid);
+        if (lse && tid < ROWS && w.row0 + tid < w.written) lse[w.row0 + tid] = INFINITY;
+        return;
+    }
+    const T* k = rows_of<T>(a.k, w, kv_head);
+    const T* v = rows_of<T>(a.v, w, kv_head);
+    const int first = w.row0 + 32 * wave, query = first + (lane & 31), half = lane >> 5;
+
+    Held<T, DP> q;
+    q.load(rows_of<T>(a.q, w, head), a.q.token, query, w.length, a.width, lane);
+    f32x16 acc[DP / 32] = {};
+    const float c = a.scale * LOG2E;
+    float top = -INFINITY, sum = 0.0f;   // running maximum of c s; this half's part of the running sum
+
+    const int end = a.causal ? min(w.length, w.row0 + ROWS) : w.length, tiles = (end + BK - 1) / BK;
+    Stage<T, DP, BK> sk, sv;
+    sk.load(k, a.k.token, 0, w.length, a.width, tid);
+    sv.load(v, a.v.token, 0, w.length, a.width, tid);
+    sk.store(lds, tid);
+    sv.store(lds + TILE, tid);
+    for (int t = 0; t < tiles; ++t) {
+        const char* kt = lds + (t & 1) * 2 * TILE;
+        const char* vt = kt + TILE;
+        const int k0 = t * BK;
+        __syncthreads();   // tile t is written; everybody is done with tile t - 1, whose place t + 1 takes below
+        if (t + 1 < tiles) {
+            sk.load(k, a.k.token, k0 + BK, w.length, a.width, tid);
+            sv.load(v, a.v.token, k0 + BK, w.length, a.width, tid);
+        }
+        if (!(a.causal && k0 > first + 31)) {   // (wave-uniform)
+            f32x16 s[BK / 32];
+#pragma unroll
+            for (int b = 0; b < BK / 32; ++b) {
+                s[b] = f32x16{};
+#pragma unroll
+                for (int i = 0; i < Img::SLABS; ++i) s[b] = Type<T>::mma(Img::row_fragment(kt, 32 * b, i, lane), q.f[i], s[b]);
+            }
+            if (k0 + BK > w.length || (a.causal && k0 + BK - 1 > first)) {
+                const int visible = a.causal ? min(w.length, query + 1) : w.length;
+#pragma unroll
+                for (int b = 0; b < BK / 32; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (k0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 >= visible) s[b][r] = -INFINITY;
+            }
+            float m = s[0][0];
+#pragma unroll
+            for (int b = 0; b < BK / 32; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) m = fmaxf(m, s[b][r]);
+            m = fmaxf(m, other_half(m)) * c;
+            const float now = fmaxf(top, m), base = now == -INFINITY ? 0.0f : now;
+            if (__any(now != top)) {
+                const float shrink = __builtin_amdgcn_exp2f(top - base);
+                sum *= shrink;
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) acc[d] *= shrink;
+            }
+            top = now;
+#pragma unroll
+            for (int b = 0; b < BK / 32; ++b) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], c, -base));
+                    sum += s[b][r];
+                }
+#pragma unroll
+                for (int i = 0; i < SECOND; ++i) {
+                    const Frag p = Type<T>::from_acc(s[b], i);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mma(Img::column_fragment(vt, 32 * b, i, 32 * d, lane), p, acc[d]);
+                }
+            }
+        }
+        if (t + 1 < tiles) {
+            sk.store(lds + ((t + 1) & 1) * 2 * TILE, tid);
+            sv.store(lds + ((t + 1) & 1) * 2 * TILE + TILE, tid);
+        }
+    }
+    sum += other_half(sum);
+    const bool real = query < w.length;
+    store_rows<T, DP>(acc, o, a.o.token, query, w.written, a.width, real ? 1.0f / sum : 0.0f, lane);
+    if (lse && half == 0 && query < w.written) lse[query] = real ? top + __builtin_amdgcn_logf(sum) : INFINITY;
+}
+
+// ---- backward: dq (and D for the second kernel) ---------------------------------------------------------------------------
+template <class T, int DP, int BK>
+__global__ __launch_bounds__(THREADS, 1) void attention_dq_kernel(const Args a) {
+    typedef Image<T, DP> Img;
+    typedef typename Type<T>::Frag Frag;
+    constexpr int TILE = BK * Img::ROW_BYTES, SECOND = 16 / Type<T>::SLAB_REGS;
+    extern __shared__ __align__(16) char lds[];   // [2][k tile, v tile]
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t item = work_item(blockIdx.x, gridDim.x);
+    const int member = static_cast<int>(item % a.group);
+    const int slot = static_cast<int>(item / a.group % a.slots);
+    const int kv_head = static_cast<int>(item / a.group / a.slots), head = kv_head * a.group + member;
+    Place w;
+    if (!locate(a, slot, a.causal, w)) return;
+    T* dq = rows_out<T>(a.dq, w, head);
+    if (w.row0 >= w.length) {
+        zero_rows<T, DP>(dq, a.dq.token, w.row0, w.written, a.width, tid);
+        return;   // (D of rows that hold no token is never read)
+    }
+    const T* k = rows_of<T>(a.k, w, kv_head);
+    const T* v = rows_of<T>(a.v, w, kv_head);
+    const int first = w.row0 + 32 * wave, query = first + (lane & 31), half = lane >> 5;
+    const bool real = query < w.length;
+
+    Held<T, DP> q, g;
+    q.load(rows_of<T>(a.q, w, head), a.q.token, query, w.length, a.width, lane);
+    g.load(rows_of<T>(a.g, w, head), a.g.token, query, w.length, a.width, lane);
+    float delta = 0.0f;
+    {
+        Held<T, DP> o;
+        o.load(rows_of<T>(a.o, w, head), a.o.token, query, w.length, a.width, lane);
+#pragma unroll
+        for (int s = 0; s < Img::SLABS; ++s) delta = Type<T>::dot(o.f[s], g.f[s], delta);
+        delta += other_half(delta);
+    }
+    const int64_t stat = head * a.rows + w.stat;
+    const float lse = real ? a.lse[stat + query] : INFINITY;
+    if (half == 0 && real) a.delta[stat + query] = delta;
+
+    f32x16 acc[DP / 32] = {};
+    const float c = a.scale * LOG2E;
+    const int end = a.causal ? min(w.length, w.row0 + ROWS) : w.length, tiles = (end + BK - 1) / BK;
+    Stage<T, DP, BK> sk, sv;
+    sk.load(k, a.k.token, 0, w.length, a.width, tid);
+    sv.load(v, a.v.token, 0, w.length, a.width, tid);
+    sk.store(lds, tid);
+    sv.store(lds + TILE, tid);
+    for (int t = 0; t < tiles; ++t) {
+        const char* kt = lds + (t & 1) * 2 * TILE;
+        const char* vt = kt + TILE;
+        const int k0 = t * BK;
+        __syncthreads();
+        if (t + 1 < tiles) {
+            sk.load(k, a.k.token, k0 + BK, w.length, a.width, tid);
+            sv.load(v, a.v.token, k0 + BK, w.length, a.width, tid);
+        }
+        if (!(a.causal && k0 > first + 31)) {
+            const bool masked = k0 + BK > w.length || (a.causal && k0 + BK - 1 > first);
+            const int visible = a.causal ? min(w.length, query + 1) : w.length;
+#pragma unroll
+            for (int b = 0; b < BK / 32; ++b) {
+                f32x16 s = {}, dp = {};
+#pragma unroll
+                for (int i = 0; i < Img::SLABS; ++i) s = Type<T>::mma(Img::row_fragment(kt, 32 * b, i, lane), q.f[i], s);
+#pragma unroll
+                for (int i = 0; i < Img::SLABS; ++i) dp = Type<T>::mma(Img::row_fragment(vt, 32 * b, i, lane), g.f[i], dp);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
+                if (masked) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (k0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 >= visible) s[r] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < SECOND; ++i) {
+                    const Frag ds = Type<T>::from_acc(s, i);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mma(Img::column_fragment(kt, 32 * b, i, 32 * d, lane), ds, acc[d]);
+                }
+            }
+        }
+        if (t + 1 < tiles) {
+            sk.store(lds + ((t + 1) & 1) * 2 * TILE, tid);
+            sv.store(lds + ((t + 1) & 1) * 2 * TILE + TILE, tid);
+        }
+    }
+    // a row that sees one key has p = 1 whatever its score: ds is exactly 0, not the difference of two roundings
+    const bool lone = a.causal ? query == 0 : w.length == 1;
+    if (!real || lone) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[d] = f32x16{};
+    }
+    store_rows<T, DP>(acc, dq, a.dq.token, query, w.written, a.width, a.scale, lane);
+}
+
+// ---- backward: dk and dv --------------------------------------------------------------------------------------------------
+template <class T, int DP, int BQ>
+__global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(const Args a) {
+    typedef Image<T, DP> Img;
+    typedef typename Type<T>::Frag Frag;
+    constexpr int TILE = BQ * Img::ROW_BYTES, STAGE = 2 * TILE + 2 * BQ * 4, SECOND = 16 / Type<T>::SLAB_REGS;
+    extern __shared__ __align__(16) char lds[];   // [2][q tile, g tile, L of its rows, D of its rows]
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t item = work_item(blockIdx.x, gridDim.x);
+    const int slot = static_cast<int>(item % a.slots), kv_head = static_cast<int>(item / a.slots);
+    Place w;
+    if (!locate(a, slot, false, w)) return;
+    T* dk = rows_out<T>(a.dk, w, kv_head);
+    T* dv = rows_out<T>(a.dv, w, kv_head);
+    if (w.row0 >= w.length) {
+        zero_rows<T, DP>(dk, a.dk.token, w.row0, w.written, a.width, tid);
+        zero_rows<T, DP>(dv, a.dv.token, w.row0, w.written, a.width, tid);
+        return;
+    }
+    const int first = w.row0 + 32 * wave, key = first + (lane & 31), half = lane >> 5;
+    Held<T, DP> k, v;
+    k.load(rows_of<T>(a.k, w, kv_head), a.k.token, key, w.length, a.width, lane);
+    v.load(rows_of<T>(a.v, w, kv_head), a.v.token, key, w.length, a.width, lane);
+    f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
+    const float c = a.scale * LOG2E;
+
+    // the query tiles of the group's heads, one after the other: step n is tile begin + n % tiles of head n / tiles
+    const int begin = a.causal ? w.row0 / BQ : 0, tiles = (w.length + BQ - 1) / BQ - begin, steps = tiles * a.group;
+    Stage<T, DP, BQ> sq, sg;
+    float stat = 0.0f;   // threads 0 .. BQ-1: L, the next BQ: D, of the staged tile's rows
+    auto load = [&](int n) {
+        const int head = kv_head * a.group + n / tiles, q0 = (begin + n % tiles) * BQ;
+        sq.load(rows_of<T>(a.q, w, head), a.q.token, q0, w.length, a.width, tid);
+        sg.load(rows_of<T>(a.g, w, head), a.g.token, q0, w.length, a.width, tid);
+        if (tid < 2 * BQ) {
+            const int row = q0 + tid % BQ;
+            const float* from = (tid < BQ ? a.lse : a.delta) + head * a.rows + w.stat;
+            stat = row < w.length ? from[row] : tid < BQ ? INFINITY : 0.0f;   // L = inf: p = 0 for rows that hold no token
+        }
+    };
+    auto store = [&](int n) {
+        char* at = lds + (n & 1) * STAGE;
+        sq.store(at, tid);
+        sg.store(at + TILE, tid);
+        if (tid < 2 * BQ) reinterpret_cast<float*>(at + 2 * TILE)[tid] = stat;
+    };
+    load(0);
+    store(0);
+    for (int n = 0; n < steps; ++n) {
+        const char* qt = lds + (n & 1) * STAGE;
+        const char* gt = qt + TILE;
+        const float* lse = reinterpret_cast<const float*>(qt + 2 * TILE);
+        const float* delta = lse + BQ;
+        const int q0 = (begin + n % tiles) * BQ;
+        __syncthreads();
+        if (n + 1 < steps) load(n + 1);
+        if (!(a.causal && q0 + BQ <= first)) {
+            const bool masked = (a.causal && q0 < first + 31) || w.length == 1;
+#pragma unroll
+            for (int b = 0; b < BQ / 32; ++b) {
+                f32x16 s = {}, dp = {};
+#pragma unroll
+                for (int i = 0; i < Img::SLABS; ++i) s = Type<T>::mma(Img::row_fragment(qt, 32 * b, i, lane), k.f[i], s);
+#pragma unroll
+                for (int i = 0; i < Img::SLABS; ++i) dp = Type<T>::mma(Img::row_fragment(gt, 32 * b, i, lane), v.f[i], dp);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + 32 * b + 8 * i + 4 * half);
+                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(delta + 32 * b + 8 * i + 4 * half);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int r = 4 * i + j;
+                        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -l4[j]));
+                        dp[r] = s[r] * (dp[r] - d4[j]);
+                    }
+                }
+                if (masked) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int query = q0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4;
+                        if (a.causal && query < key) { s[r] = 0.0f; dp[r] = 0.0f; }
+                        if (a.causal ? query == 0 : w.length == 1) dp[r] = 0.0f;   // one visible key: ds is exactly 0
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < SECOND; ++i) {
+                    const Frag p = Type<T>::from_acc(s, i), ds = Type<T>::from_acc(dp, i);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) av[d] = Type<T>::mma(Img::column_fragment(gt, 32 * b, i, 32 * d, lane), p, av[d]);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) ak[d] = Type<T>::mma(Img::column_fragment(qt, 32 * b, i, 32 * d, lane), ds, ak[d]);
+                }
+            }
+        }
+        if (n + 1 < steps) store(n + 1);
+    }
+    if (key >= w.length) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) { ak[d] = f32x16{}; av[d] = f32x16{}; }
+    }
+    store_rows<T, DP>(ak, dk, a.dk.token, key, w.written, a.width, a.scale, lane);
+    store_rows<T, DP>(av, dv, a.dv.token, key, w.written, a.width, 1.0f, lane);
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------
+template <class T>
+constexpr int tile_rows() { return sizeof(T) == 2 ? 64 : 32; }
+template <class T, int DP>
+constexpr int key_lds() { return 2 * 2 * tile_rows<T>() * Image<T, DP>::ROW_BYTES; }
+template <class T, int DP>
+constexpr int query_lds() { return 2 * (2 * tile_rows<T>() * Image<T, DP>::ROW_BYTES + 2 * tile_rows<T>() * 4); }
+
+template <class T, int DP>
+bool configure() {
+    constexpr int B = tile_rows<T>();
+    auto set = [](const void* f, int bytes) { return hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess; };
+    return set(reinterpret_cast<const void*>(attention_forward_kernel<T, DP, B>), key_lds<T, DP>()) &&
+           set(reinterpret_cast<const void*>(attention_dq_kernel<T, DP, B>), key_lds<T, DP>()) &&
+           set(reinterpret_cast<const void*>(attention_dkv_kernel<T, DP, B>), query_lds<T, DP>());
+}
+
+// One-time kernel attribute set-up, thread-safe.
+int configure_kernels() {
+    static std::once_flag flag;
+    static int status = KF_OK;
+    std::call_once(flag, [] {
+        if (!(configure<__bf16, 32>() && configure<__bf16, 64>() && configure<__bf16, 96>() && configure<__bf16, 128>() && configure<float, 32>() &&
+              configure<float, 64>() && configure<float, 96>() && configure<float, 128>()))
+            status = KF_ERR_LAUNCH_FAILED;
+    });
+    return status;
+}
+
+template <class T, int DP>
+int launch_width(Args& a, bool backward, hipStream_t stream) {
+    constexpr int B = tile_rows<T>();
+    const unsigned items = static_cast<unsigned>(static_cast<int64_t>(a.slots) * a.heads);
+    if (!backward) {
+        attention_forward_kernel<T, DP, B><<<items, THREADS, key_lds<T, DP>(), stream>>>(a);
+    } else {
+        attention_dq_kernel<T, DP, B><<<items, THREADS, key_lds<T, DP>(), stream>>>(a);
+        attention_dkv_kernel<T, DP, B><<<items / a.group, THREADS, query_lds<T, DP>(), stream>>>(a);
+    }
+    return hipGetLastError() == hipSuccess ? KF_OK : KF_ERR_LAUNCH_FAILED;
+}
+
+template <class T>
+int launch_type(Args& a, bool backward, hipStream_t stream) {
+    if (a.width <= 32) return launch_width<T, 32>(a, backward, stream);
+    if (a.width <= 64) return launch_width<T, 64>(a, backward, stream);
+    if (a.width <= 96) return launch_width<T, 96>(a, backward, stream);
+    return launch_width<T, 128>(a, backward, stream);
+}
+
+Tensor tensor_of(const kf_heads_view* v) { return Tensor{v->p, v->batch_stride, v->token_stride, v->head_stride}; }
+
+bool aligned(const kf_heads_view* v, int64_t per) {
+    return v != nullptr && v->p != nullptr && reinterpret_cast<uintptr_t>(v->p) % 16 == 0 && v->batch_stride % per == 0 && v->token_stride % per == 0 &&
+           v->head_stride % per == 0;
+}
+
+int fill(Args& a, int dtype, int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width, const int32_t* lengths,
+         const int32_t* offsets, int causal, float scale) {
+    if (dtype != KF_BF16 && dtype != KF_F32) return KF_ERR_UNSUPPORTED_DTYPE;
+    const int64_t per = dtype == KF_BF16 ? 8 : 4, limit = 0x7fffffff;
+    if (sequences <= 0 || rows <= 0 || rows > limit - ROWS || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || width <= 0 || width > 128 ||
+        width % per != 0 || !(scale > 0.0f) || !isfinite(scale))
+        return KF_ERR_INVALID_ARGUMENT;
+    if (offsets ? lengths != nullptr : (length <= 0 || sequences > limit / length || rows != sequences * length)) return KF_ERR_INVALID_ARGUMENT;
+    const int64_t slots = offsets ? rows / ROWS + sequences + 1 : sequences * ((length + ROWS - 1) / ROWS);
+    if (sequences >= limit || slots > limit / heads) return KF_ERR_INVALID_ARGUMENT;
+    a.lengths = lengths;
+    a.offsets = offsets;
+    a.rows = rows;
+    a.sequences = static_cast<int>(sequences);
+    a.length = static_cast<int>(length);
+    a.heads = static_cast<int>(heads);
+    a.group = static_cast<int>(heads / kv_heads);
+    a.width = static_cast<int>(width);
+    a.causal = causal != 0;
+    a.slots = static_cast<int>(slots);
+    a.scale = scale;
+    return KF_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int kf_attention_forward(const kf_heads_view* out, float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v, int dtype,
+                         int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width, const int32_t* lengths,
+                         const int32_t* offsets, int causal, float scale, void* stream) {
+    Args a = {};
+    if (int s = fill(a, dtype, sequences, length, rows, heads, kv_heads, width, lengths, offsets, causal, scale)) return s;
+    const int64_t per = dtype == KF_BF16 ? 8 : 4;
+    if (!aligned(out, per) || !aligned(q, per) || !aligned(k, per) || !aligned(v, per)) return KF_ERR_INVALID_ARGUMENT;
+    if (int s = configure_kernels()) return s;
+    a.q = tensor_of(q); a.k = tensor_of(k); a.v = tensor_of(v); a.o = tensor_of(out);
+    a.lse = lse;
+    const hipStream_t on = reinterpret_cast<hipStream_t>(stream);
+    return dtype == KF_BF16 ? launch_type<__bf16>(a, false, on) : launch_type<float>(a, false, on);
+}
+
+int64_t kf_attention_backward_workspace_bytes(int64_t rows, int64_t heads) { return rows > 0 && heads > 0 ? rows * heads * 4 : 0; }
+
+int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, const kf_heads_view* dv, const kf_heads_view* grad, const kf_heads_view* out,
+                          const float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v, int dtype, int64_t sequences,
+                          int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width, const int32_t* lengths, const int32_t* offsets,
+                          int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+    Args a = {};
+    if (int s = fill(a, dtype, sequences, length, rows, heads, kv_heads, width, lengths, offsets, causal, scale)) return s;
+    const int64_t per = dtype == KF_BF16 ? 8 : 4;
+    const kf_heads_view* all[] = {dq, dk, dv, grad, out, q, k, v};
+    for (const kf_heads_view* t : all)
+        if (!aligned(t, per)) return KF_ERR_INVALID_ARGUMENT;
+    if (lse == nullptr) return KF_ERR_INVALID_ARGUMENT;
+    if (workspace == nullptr || workspace_bytes < kf_attention_backward_workspace_bytes(rows, heads)) return KF_ERR_WORKSPACE_TOO_SMALL;
+    if (int s = configure_kernels()) return s;
+    a.q = tensor_of(q); a.k = tensor_of(k); a.v = tensor_of(v); a.o = tensor_of(out); a.g = tensor_of(grad);
+    a.dq = tensor_of(dq); a.dk = tensor_of(dk); a.dv = tensor_of(dv);
+    a.lse = const_cast<float*>(lse);
+    a.delta = reinterpret_cast<float*>(workspace);
+    const hipStream_t on = reinterpret_cast<hipStream_t>(stream);
+    return dtype == KF_BF16 ? launch_type<__bf16>(a, true, on) : launch_type<float>(a, true, on);
+}
+
+}  // extern "C"
