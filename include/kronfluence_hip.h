@@ -446,7 +446,8 @@ int kf_cast(void* dst, int dst_dtype, const void* src, int src_dtype, int64_t nu
  * ------------------------------------------------------------------------------------------- */
 
 /* A [batch][token][head][width] operand, the width contiguous: strides in elements, the pointer 16-byte aligned, every stride a
- * multiple of 16 bytes (slices of a fused projection are taken as they are).  Packed batches ignore batch_stride. */
+ * multiple of 16 bytes, tokens at least the width and at most 8 MB apart (slices of a fused projection are taken as they are).
+ * Packed batches ignore batch_stride. */
 typedef struct kf_heads_view {
     const void* p;
     int64_t batch_stride, token_stride, head_stride;

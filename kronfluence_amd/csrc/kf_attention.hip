@@ -160,25 +160,38 @@ struct Image {
     }
 };
 
-// Global rows [row0, row0 + N) of a tile into registers (every thread a few 16-byte chunks), and from there to LDS.  A row behind
-// the sequence's last reads the last one instead: what stands behind it may be anything, and its weight is 0.  Columns behind the
-// head width are 0.
+// Rows of one head of one sequence as a buffer: a load behind the last row, or of a column behind the head width, returns 0 without
+// touching memory -- what stands there may be anything, and its weight is 0.  The descriptor is rebuilt per tile (scalar
+// arithmetic), so that the 32-bit offsets span one tile only.
+constexpr uint32_t NO_COLUMN = 0x80000000u;         // an offset no descriptor reaches
+constexpr int64_t MAX_RECORDS = 0x7fffffff;
+struct Rows {
+    const char* base;
+    int64_t token;     // bytes between rows
+    int length, width; // rows; bytes of a row
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t from(int row0) const {
+        const int64_t bytes = (length - row0 - 1) * token + width;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + row0 * token), 0, row0 < length ? static_cast<int>(min(bytes, MAX_RECORDS)) : 0,
+                                                 0x00020000);
+    }
+};
+
+// N rows of a tile into registers (every thread a few 16-byte chunks), and from there to LDS.
 template <class T, int DP, int N>
 struct Stage {
     typedef Image<T, DP> Img;
     static constexpr int PER = N * Img::CHUNKS / THREADS;
     static_assert(PER * THREADS == N * Img::CHUNKS, "whole chunks per thread");
     u32x4 r[PER];
-    __device__ __forceinline__ void load(const T* base, int64_t token, int row0, int length, int width, int tid) {
+    // byte offset of the thread's chunk i inside a tile whose rows are `token` bytes apart
+    static __device__ __forceinline__ uint32_t offset(int i, int64_t token, int width, int tid) {
+        const int n = tid + i * THREADS, chunk = n % Img::CHUNKS;
+        return chunk * 16 < width ? static_cast<uint32_t>(n / Img::CHUNKS * static_cast<int>(token) + chunk * 16) : NO_COLUMN;
+    }
+    __device__ __forceinline__ void load(const Rows& rows, int row0, int tid) {
+        const __amdgpu_buffer_rsrc_t from = rows.from(row0);
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int n = tid + i * THREADS, row = n / Img::CHUNKS, chunk = n % Img::CHUNKS;
-            const int from = min(row0 + row, length - 1);
-            u32x4 v = {0, 0, 0, 0};
-            if (chunk * (16 / static_cast<int>(sizeof(T))) < width)
-                v = *reinterpret_cast<const u32x4*>(base + from * token + chunk * (16 / static_cast<int>(sizeof(T))));
-            r[i] = v;
-        }
+        for (int i = 0; i < PER; ++i) r[i] = __builtin_amdgcn_raw_buffer_load_b128(from, offset(i, rows.token, rows.width, tid), 0, 0);
     }
     __device__ __forceinline__ void store(char* tile, int tid) const {
 #pragma unroll
@@ -244,6 +257,11 @@ __device__ __forceinline__ const T* rows_of(const Tensor& t, const Place& w, int
     return reinterpret_cast<const T*>(t.p) + w.sequence * t.batch + w.start * t.token + head * t.head;
 }
 template <class T>
+__device__ __forceinline__ Rows input_rows(const Args& a, const Tensor& t, const Place& w, int head) {
+    return Rows{reinterpret_cast<const char*>(rows_of<T>(t, w, head)), t.token * static_cast<int64_t>(sizeof(T)), w.length,
+                a.width * static_cast<int>(sizeof(T))};
+}
+template <class T>
 __device__ __forceinline__ T* rows_out(const Tensor& t, const Place& w, int head) { return const_cast<T*>(rows_of<T>(t, w, head)); }
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
@@ -252,15 +270,15 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32);
 template <class T, int DP>
 struct Held {
     typename Type<T>::Frag f[Image<T, DP>::SLABS];
-    __device__ __forceinline__ void load(const T* base, int64_t token, int row, int length, int width, int lane) {
-        constexpr int PER = 16 / static_cast<int>(sizeof(T));
-        const T* p = base + min(row, length - 1) * token;
+    __device__ __forceinline__ void load(const Rows& rows, int row0, int lane) {
+        const __amdgpu_buffer_rsrc_t from = rows.from(row0);
 #pragma unroll
         for (int s = 0; s < Image<T, DP>::SLABS; ++s) {
             const int c = 2 * s + (lane >> 5);
-            typename Type<T>::Frag v = {};
-            if (c * PER < width) v = *reinterpret_cast<const typename Type<T>::Frag*>(p + c * PER);
-            f[s] = v;
+            union { u32x4 u; typename Type<T>::Frag f; } v;
+            v.u = __builtin_amdgcn_raw_buffer_load_b128(
+                from, c * 16 < rows.width ? static_cast<uint32_t>((lane & 31) * static_cast<int>(rows.token) + c * 16) : NO_COLUMN, 0, 0);
+            f[s] = v.f;
         }
     }
 };
@@ -292,14 +310,14 @@ __device__ __forceinline__ void zero_rows(T* base, int64_t token, int row0, int 
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
-template <class T, int DP, int BK>
-__global__ __launch_bounds__(THREADS, 1) void attention_forward_kernel(const Args a) {
+template <class T, int DP, int BK, int WAVES>
+__global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const Args a) {
     typedef Image<T, DP> Img;
     typedef typename Type<T>::Frag Frag;
     constexpr int TILE = BK * Img::ROW_BYTES, SECOND = 16 / Type<T>::SLAB_REGS;
     extern __shared__ __align__(16) char lds[];   // [2][k tile, v tile]
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t item = work_item(blockIdx.x, gridDim.x);
     const int member = static_cast<int>(item % a.group);
     const int slot = static_cast<int>(item / a.group % a.slots);
@@ -313,20 +331,19 @@ __global__ __launch_bounds__(THREADS, 1) void attention_forward_kernel(const Arg
         if (lse && tid < ROWS && w.row0 + tid < w.written) lse[w.row0 + tid] = INFINITY;
         return;
     }
-    const T* k = rows_of<T>(a.k, w, kv_head);
-    const T* v = rows_of<T>(a.v, w, kv_head);
+    const Rows k = input_rows<T>(a, a.k, w, kv_head), v = input_rows<T>(a, a.v, w, kv_head);
     const int first = w.row0 + 32 * wave, query = first + (lane & 31), half = lane >> 5;
 
     Held<T, DP> q;
-    q.load(rows_of<T>(a.q, w, head), a.q.token, query, w.length, a.width, lane);
+    q.load(input_rows<T>(a, a.q, w, head), first, lane);
     f32x16 acc[DP / 32] = {};
     const float c = a.scale * LOG2E;
     float top = -INFINITY, sum = 0.0f;   // running maximum of c s; this half's part of the running sum
 
     const int end = a.causal ? min(w.length, w.row0 + ROWS) : w.length, tiles = (end + BK - 1) / BK;
     Stage<T, DP, BK> sk, sv;
-    sk.load(k, a.k.token, 0, w.length, a.width, tid);
-    sv.load(v, a.v.token, 0, w.length, a.width, tid);
+    sk.load(k, 0, tid);
+    sv.load(v, 0, tid);
     sk.store(lds, tid);
     sv.store(lds + TILE, tid);
     for (int t = 0; t < tiles; ++t) {
@@ -335,8 +352,8 @@ __global__ __launch_bounds__(THREADS, 1) void attention_forward_kernel(const Arg
         const int k0 = t * BK;
         __syncthreads();   // tile t is written; everybody is done with tile t - 1, whose place t + 1 takes below
         if (t + 1 < tiles) {
-            sk.load(k, a.k.token, k0 + BK, w.length, a.width, tid);
-            sv.load(v, a.v.token, k0 + BK, w.length, a.width, tid);
+            sk.load(k, k0 + BK, tid);
+            sv.load(v, k0 + BK, tid);
         }
         if (!(a.causal && k0 > first + 31)) {   // (wave-uniform)
             f32x16 s[BK / 32];
@@ -395,14 +412,14 @@ __global__ __launch_bounds__(THREADS, 1) void attention_forward_kernel(const Arg
 }
 
 // ---- backward: dq (and D for the second kernel) ---------------------------------------------------------------------------
-template <class T, int DP, int BK>
-__global__ __launch_bounds__(THREADS, 1) void attention_dq_kernel(const Args a) {
+template <class T, int DP, int BK, int WAVES>
+__global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args a) {
     typedef Image<T, DP> Img;
     typedef typename Type<T>::Frag Frag;
     constexpr int TILE = BK * Img::ROW_BYTES, SECOND = 16 / Type<T>::SLAB_REGS;
     extern __shared__ __align__(16) char lds[];   // [2][k tile, v tile]
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t item = work_item(blockIdx.x, gridDim.x);
     const int member = static_cast<int>(item % a.group);
     const int slot = static_cast<int>(item / a.group % a.slots);
@@ -414,18 +431,17 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dq_kernel(const Args a) 
         zero_rows<T, DP>(dq, a.dq.token, w.row0, w.written, a.width, tid);
         return;   // (D of rows that hold no token is never read)
     }
-    const T* k = rows_of<T>(a.k, w, kv_head);
-    const T* v = rows_of<T>(a.v, w, kv_head);
+    const Rows k = input_rows<T>(a, a.k, w, kv_head), v = input_rows<T>(a, a.v, w, kv_head);
     const int first = w.row0 + 32 * wave, query = first + (lane & 31), half = lane >> 5;
     const bool real = query < w.length;
 
     Held<T, DP> q, g;
-    q.load(rows_of<T>(a.q, w, head), a.q.token, query, w.length, a.width, lane);
-    g.load(rows_of<T>(a.g, w, head), a.g.token, query, w.length, a.width, lane);
+    q.load(input_rows<T>(a, a.q, w, head), first, lane);
+    g.load(input_rows<T>(a, a.g, w, head), first, lane);
     float delta = 0.0f;
     {
         Held<T, DP> o;
-        o.load(rows_of<T>(a.o, w, head), a.o.token, query, w.length, a.width, lane);
+        o.load(input_rows<T>(a, a.o, w, head), first, lane);
 #pragma unroll
         for (int s = 0; s < Img::SLABS; ++s) delta = Type<T>::dot(o.f[s], g.f[s], delta);
         delta += other_half(delta);
@@ -438,8 +454,8 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dq_kernel(const Args a) 
     const float c = a.scale * LOG2E;
     const int end = a.causal ? min(w.length, w.row0 + ROWS) : w.length, tiles = (end + BK - 1) / BK;
     Stage<T, DP, BK> sk, sv;
-    sk.load(k, a.k.token, 0, w.length, a.width, tid);
-    sv.load(v, a.v.token, 0, w.length, a.width, tid);
+    sk.load(k, 0, tid);
+    sv.load(v, 0, tid);
     sk.store(lds, tid);
     sv.store(lds + TILE, tid);
     for (int t = 0; t < tiles; ++t) {
@@ -448,8 +464,8 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dq_kernel(const Args a) 
         const int k0 = t * BK;
         __syncthreads();
         if (t + 1 < tiles) {
-            sk.load(k, a.k.token, k0 + BK, w.length, a.width, tid);
-            sv.load(v, a.v.token, k0 + BK, w.length, a.width, tid);
+            sk.load(k, k0 + BK, tid);
+            sv.load(v, k0 + BK, tid);
         }
         if (!(a.causal && k0 > first + 31)) {
             const bool masked = k0 + BK > w.length || (a.causal && k0 + BK - 1 > first);
@@ -491,14 +507,14 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dq_kernel(const Args a) 
 }
 
 // ---- backward: dk and dv --------------------------------------------------------------------------------------------------
-template <class T, int DP, int BQ>
-__global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(const Args a) {
+template <class T, int DP, int BQ, int WAVES>
+__global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Args a) {
     typedef Image<T, DP> Img;
     typedef typename Type<T>::Frag Frag;
     constexpr int TILE = BQ * Img::ROW_BYTES, STAGE = 2 * TILE + 2 * BQ * 4, SECOND = 16 / Type<T>::SLAB_REGS;
     extern __shared__ __align__(16) char lds[];   // [2][q tile, g tile, L of its rows, D of its rows]
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t item = work_item(blockIdx.x, gridDim.x);
     const int slot = static_cast<int>(item % a.slots), kv_head = static_cast<int>(item / a.slots);
     Place w;
@@ -512,8 +528,8 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(const Args a)
     }
     const int first = w.row0 + 32 * wave, key = first + (lane & 31), half = lane >> 5;
     Held<T, DP> k, v;
-    k.load(rows_of<T>(a.k, w, kv_head), a.k.token, key, w.length, a.width, lane);
-    v.load(rows_of<T>(a.v, w, kv_head), a.v.token, key, w.length, a.width, lane);
+    k.load(input_rows<T>(a, a.k, w, kv_head), first, lane);
+    v.load(input_rows<T>(a, a.v, w, kv_head), first, lane);
     f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
     const float c = a.scale * LOG2E;
 
@@ -523,8 +539,8 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(const Args a)
     float stat = 0.0f;   // threads 0 .. BQ-1: L, the next BQ: D, of the staged tile's rows
     auto load = [&](int n) {
         const int head = kv_head * a.group + n / tiles, q0 = (begin + n % tiles) * BQ;
-        sq.load(rows_of<T>(a.q, w, head), a.q.token, q0, w.length, a.width, tid);
-        sg.load(rows_of<T>(a.g, w, head), a.g.token, q0, w.length, a.width, tid);
+        sq.load(input_rows<T>(a, a.q, w, head), q0, tid);
+        sg.load(input_rows<T>(a, a.g, w, head), q0, tid);
         if (tid < 2 * BQ) {
             const int row = q0 + tid % BQ;
             const float* from = (tid < BQ ? a.lse : a.delta) + head * a.rows + w.stat;
@@ -596,20 +612,24 @@ __global__ __launch_bounds__(THREADS, 1) void attention_dkv_kernel(const Args a)
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
-template <class T>
-constexpr int tile_rows() { return sizeof(T) == 2 ? 64 : 32; }
+// Tile rows and waves per SIMD of each kernel.
 template <class T, int DP>
-constexpr int key_lds() { return 2 * 2 * tile_rows<T>() * Image<T, DP>::ROW_BYTES; }
-template <class T, int DP>
-constexpr int query_lds() { return 2 * (2 * tile_rows<T>() * Image<T, DP>::ROW_BYTES + 2 * tile_rows<T>() * 4); }
+struct Shape {
+    static constexpr int KEYS = sizeof(T) == 2 ? 64 : 32, QUERIES = sizeof(T) == 2 && DP <= 96 ? 64 : 32;
+    static constexpr int KEY_LDS = 4 * KEYS * Image<T, DP>::ROW_BYTES, QUERY_LDS = 4 * QUERIES * Image<T, DP>::ROW_BYTES + 4 * QUERIES * 4;
+    static constexpr int FORWARD_WAVES = sizeof(T) == 2 ? 2 : 1, DQ_WAVES = sizeof(T) == 2 ? 2 : 1, DKV_WAVES = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
+    static constexpr auto forward = &attention_forward_kernel<T, DP, KEYS, FORWARD_WAVES>;
+    static constexpr auto dq = &attention_dq_kernel<T, DP, KEYS, DQ_WAVES>;
+    static constexpr auto dkv = &attention_dkv_kernel<T, DP, QUERIES, DKV_WAVES>;
+};
 
 template <class T, int DP>
 bool configure() {
-    constexpr int B = tile_rows<T>();
-    auto set = [](const void* f, int bytes) { return hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess; };
-    return set(reinterpret_cast<const void*>(attention_forward_kernel<T, DP, B>), key_lds<T, DP>()) &&
-           set(reinterpret_cast<const void*>(attention_dq_kernel<T, DP, B>), key_lds<T, DP>()) &&
-           set(reinterpret_cast<const void*>(attention_dkv_kernel<T, DP, B>), query_lds<T, DP>());
+    typedef Shape<T, DP> S;
+    auto set = [](auto f, int bytes) {
+        return hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
+    };
+    return set(S::forward, S::KEY_LDS) && set(S::dq, S::KEY_LDS) && set(S::dkv, S::QUERY_LDS);
 }
 
 // One-time kernel attribute set-up, thread-safe.
@@ -626,13 +646,13 @@ int configure_kernels() {
 
 template <class T, int DP>
 int launch_width(Args& a, bool backward, hipStream_t stream) {
-    constexpr int B = tile_rows<T>();
+    typedef Shape<T, DP> S;
     const unsigned items = static_cast<unsigned>(static_cast<int64_t>(a.slots) * a.heads);
     if (!backward) {
-        attention_forward_kernel<T, DP, B><<<items, THREADS, key_lds<T, DP>(), stream>>>(a);
+        S::forward<<<items, THREADS, S::KEY_LDS, stream>>>(a);
     } else {
-        attention_dq_kernel<T, DP, B><<<items, THREADS, key_lds<T, DP>(), stream>>>(a);
-        attention_dkv_kernel<T, DP, B><<<items / a.group, THREADS, query_lds<T, DP>(), stream>>>(a);
+        S::dq<<<items, THREADS, S::KEY_LDS, stream>>>(a);
+        S::dkv<<<items / a.group, THREADS, S::QUERY_LDS, stream>>>(a);
     }
     return hipGetLastError() == hipSuccess ? KF_OK : KF_ERR_LAUNCH_FAILED;
 }
@@ -647,9 +667,11 @@ int launch_type(Args& a, bool backward, hipStream_t stream) {
 
 Tensor tensor_of(const kf_heads_view* v) { return Tensor{v->p, v->batch_stride, v->token_stride, v->head_stride}; }
 
-bool aligned(const kf_heads_view* v, int64_t per) {
+// 16-byte chunks, rows that do not overlap (a load behind the last row must fall behind the buffer's end), and a tile's span below
+// 2^30 bytes
+bool usable(const kf_heads_view* v, int64_t per, int64_t width) {
     return v != nullptr && v->p != nullptr && reinterpret_cast<uintptr_t>(v->p) % 16 == 0 && v->batch_stride % per == 0 && v->token_stride % per == 0 &&
-           v->head_stride % per == 0;
+           v->head_stride % per == 0 && v->token_stride >= width && v->token_stride <= (int64_t{1} << 23) / (16 / per);
 }
 
 int fill(Args& a, int dtype, int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width, const int32_t* lengths,
@@ -686,7 +708,7 @@ int kf_attention_forward(const kf_heads_view* out, float* lse, const kf_heads_vi
     Args a = {};
     if (int s = fill(a, dtype, sequences, length, rows, heads, kv_heads, width, lengths, offsets, causal, scale)) return s;
     const int64_t per = dtype == KF_BF16 ? 8 : 4;
-    if (!aligned(out, per) || !aligned(q, per) || !aligned(k, per) || !aligned(v, per)) return KF_ERR_INVALID_ARGUMENT;
+    if (!usable(out, per, width) || !usable(q, per, width) || !usable(k, per, width) || !usable(v, per, width)) return KF_ERR_INVALID_ARGUMENT;
     if (int s = configure_kernels()) return s;
     a.q = tensor_of(q); a.k = tensor_of(k); a.v = tensor_of(v); a.o = tensor_of(out);
     a.lse = lse;
@@ -705,7 +727,7 @@ int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, cons
     const int64_t per = dtype == KF_BF16 ? 8 : 4;
     const kf_heads_view* all[] = {dq, dk, dv, grad, out, q, k, v};
     for (const kf_heads_view* t : all)
-        if (!aligned(t, per)) return KF_ERR_INVALID_ARGUMENT;
+        if (!usable(t, per, width)) return KF_ERR_INVALID_ARGUMENT;
     if (lse == nullptr) return KF_ERR_INVALID_ARGUMENT;
     if (workspace == nullptr || workspace_bytes < kf_attention_backward_workspace_bytes(rows, heads)) return KF_ERR_WORKSPACE_TOO_SMALL;
     if (int s = configure_kernels()) return s;

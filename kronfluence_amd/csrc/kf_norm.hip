@@ -347,7 +347,13 @@ __global__ __launch_bounds__(64 * STRANDS) void norm_reduce_kernel(const float* 
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
     float s = 0.0f;
     if (c < width)
-        for (int64_t n = strand; n < count; n += STRANDS) s += partial[(n * parts + part) * width + c];
+        for (int64_t n = strand; n < count; n += 8 * STRANDS) {   // eight loads in flight
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = n + i * STRANDS < count ? partial[((n + i * STRANDS) * parts + part) * width + c] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s += v[i];
+        }
     sums[strand][lane] = s;
     __syncthreads();
     if (strand != 0 || c >= width) return;

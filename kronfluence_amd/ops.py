@@ -8,6 +8,7 @@ from PyTorch's caching allocator.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import logging
 import math
@@ -1007,51 +1008,63 @@ def cast(src: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 # Model passes: attention and norms (autograd on top of these: kronfluence_amd/functional.py)
 # ---------------------------------------------------------------------------------------------
 ATTENTION_MAX_WIDTH = 128
+_MAX_TOKEN_BYTES = 1 << 23
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on_device_of(t: torch.Tensor):
+    """Context in which a launch goes to ``t``'s device (nothing to do when that is the current one, as it nearly always is)."""
+    return _NO_GUARD if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _heads_operand(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself if the kernels can read it in place (``[..., heads, width]``: contiguous width, 16-byte aligned start and
     strides), else a contiguous copy."""
-    size = t.element_size()
-    if (t.data_ptr() % 16 == 0 and (t.stride(-1) == 1 or t.shape[-1] == 1)
-            and all(n == 1 or s * size % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]))):
-        return t
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():   # (the width is whole 16-byte chunks: so are the strides)
+            return t
+        size, tokens = t.element_size(), t.stride(-3)
+        if (t.stride(-1) == 1 and all(n == 1 or s * size % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
+                and (t.shape[-3] == 1 or t.shape[-1] <= tokens <= _MAX_TOKEN_BYTES // size)):
+            return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _heads_view(t: torch.Tensor) -> nat.kf_heads_view:
-    strides = [0 if n == 1 else s for n, s in zip(t.shape[:-1], t.stride()[:-1])]
-    return nat.kf_heads_view(t.data_ptr(), 0 if t.dim() == 3 else strides[0], strides[-2], strides[-1])
+    # an axis of one element may carry any stride: it is never multiplied by anything but 0
+    shape, strides = t.shape, t.stride()
+    batch = strides[0] if t.dim() == 4 and shape[0] > 1 else 0
+    return nat.kf_heads_view(t.data_ptr(), batch, strides[-3] if shape[-3] > 1 else shape[-1], strides[-2] if shape[-2] > 1 else 0)
 
 
 def _attention_shape(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tensor],
-                     cu_seqlens: Optional[torch.Tensor], scale: float) -> Tuple[int, int, int]:
-    """Checks the operands of one attention call; ``(sequences, length, token rows)``."""
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        nat.require_device(t, name)
-        _require(t.dtype == q.dtype and t.device == q.device, "q, k and v share one dtype and one device")
+                     cu_seqlens: Optional[torch.Tensor], scale: float) -> Tuple[int, int, int, int, int, int]:
+    """Checks the operands of one attention call; ``(sequences, length, token rows, heads, kv_heads, width)``."""
+    nat.require_device(q, "q"), nat.require_device(k, "k"), nat.require_device(v, "v")
+    _require(k.dtype == q.dtype == v.dtype and k.device == q.device == v.device, "q, k and v share one dtype and one device")
     _require(q.dtype in (torch.bfloat16, torch.float32), f"attention takes bfloat16 or float32 tensors, not {q.dtype}")
     packed = cu_seqlens is not None
     _require(not (packed and lengths is not None), "lengths (padded batch) and cu_seqlens (packed batch) exclude each other")
-    _require(q.dim() == (3 if packed else 4),
+    shape, kv_shape = tuple(q.shape), tuple(k.shape)
+    _require(len(shape) == (3 if packed else 4),
              "q is [tokens, heads, width] with cu_seqlens, [batch, length, heads, width] without")
-    _require(k.dim() == q.dim() and k.shape[:-2] == q.shape[:-2] and v.shape == k.shape and k.shape[-1] == q.shape[-1],
+    _require(kv_shape == tuple(v.shape) and kv_shape[:-2] == shape[:-2] and kv_shape[-1] == shape[-1],
              "k and v have the shape of q, but for the number of heads")
-    heads, kv_heads, width = q.shape[-2], k.shape[-2], q.shape[-1]
+    heads, kv_heads, width = shape[-2], kv_shape[-2], shape[-1]
     _require(kv_heads > 0 and heads > 0 and heads % kv_heads == 0, "the number of heads is a multiple of the number of key / value heads")
     _require(0 < width <= ATTENTION_MAX_WIDTH, f"head widths up to {ATTENTION_MAX_WIDTH}")
     _require(width * q.element_size() % 16 == 0, "the head width is a whole number of 16-byte chunks")
     _require(math.isfinite(scale) and scale > 0, "scale is positive and finite")
-    for name, t, count in (("lengths", lengths, None if packed else q.shape[0]), ("cu_seqlens", cu_seqlens, None)):
+    for name, t in (("lengths", lengths), ("cu_seqlens", cu_seqlens)):
         if t is not None:
             nat.require_device(t, name)
             _require(t.device == q.device and t.dim() == 1 and t.dtype in (torch.int32, torch.int64),
                      f"{name} is a vector of int32 or int64 on the device of q")
-            _require(count is None or t.numel() == count, f"{name} has one entry per row of the batch")
     if packed:
         _require(cu_seqlens.numel() >= 1, "cu_seqlens holds the first row of every sequence and the last row's end")
-        return cu_seqlens.numel() - 1, 0, q.shape[0]
-    return q.shape[0], q.shape[1], q.shape[0] * q.shape[1]
+        return cu_seqlens.numel() - 1, 0, shape[0], heads, kv_heads, width
+    _require(lengths is None or lengths.numel() == shape[0], "lengths has one entry per row of the batch")
+    return shape[0], shape[1], shape[0] * shape[1], heads, kv_heads, width
 
 
 def _row_counts(t: Optional[torch.Tensor], most: int) -> Optional[torch.Tensor]:
@@ -1066,19 +1079,18 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal:
                       with_lse: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``softmax(scale q k^T + mask) v`` over whole prompts (kf_attention_forward): the output and, for the backward call, the fp32
     ``[heads, token rows]`` log-sum of every row."""
-    sequences, length, rows = _attention_shape(q, k, v, lengths, cu_seqlens, scale)
-    heads, kv_heads, width = q.shape[-2], k.shape[-2], q.shape[-1]
+    sequences, length, rows, heads, kv_heads, width = _attention_shape(q, k, v, lengths, cu_seqlens, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((heads, rows), dtype=torch.float32, device=q.device) if with_lse else None
     if sequences == 0 or rows == 0:
         return out.zero_(), lse
     q, k, v = _heads_operand(q), _heads_operand(k), _heads_operand(v)
     lengths, offsets = _row_counts(lengths, length), _row_counts(cu_seqlens, rows)
-    with torch.cuda.device(q.device):
+    with _on_device_of(q):
         nat.check(
             nat.lib().kf_attention_forward(_heads_view(out), _ptr(lse), _heads_view(q), _heads_view(k), _heads_view(v),
                                            nat.dtype_code(q.dtype), sequences, length, rows, heads, kv_heads, width, _ptr(lengths),
-                                           _ptr(offsets), int(causal), scale, nat.stream_ptr(q.device)),
+                                           _ptr(offsets), int(causal), scale, nat.launch_stream(q)),
             "kf_attention_forward",
         )
     return out, lse
@@ -1088,24 +1100,25 @@ def attention_backward(grad: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
                        causal: bool, scale: float, lengths: Optional[torch.Tensor] = None,
                        cu_seqlens: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients of :func:`attention_forward` with respect to ``q``, ``k`` and ``v`` (kf_attention_backward), contiguous."""
-    sequences, length, rows = _attention_shape(q, k, v, lengths, cu_seqlens, scale)
-    heads, kv_heads, width = q.shape[-2], k.shape[-2], q.shape[-1]
+    sequences, length, rows, heads, kv_heads, width = _attention_shape(q, k, v, lengths, cu_seqlens, scale)
     _require(grad.shape == out.shape == q.shape and grad.dtype == out.dtype == q.dtype and grad.device == out.device == q.device,
              "grad and out have the shape, dtype and device of q")
-    _require(lse.dtype == torch.float32 and lse.is_contiguous() and tuple(lse.shape) == (heads, rows), "lse is what the forward call returned")
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    _require(lse.dtype == torch.float32 and lse.is_contiguous() and lse.shape == (heads, rows), "lse is what the forward call returned")
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk, dv = torch.empty(k.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=q.dtype, device=q.device)
     if sequences == 0 or rows == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     grad, out, q, k, v = (_heads_operand(t) for t in (grad, out, q, k, v))
     lengths, offsets = _row_counts(lengths, length), _row_counts(cu_seqlens, rows)
-    ws_bytes = nat.lib().kf_attention_backward_workspace_bytes(rows, heads)
-    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=q.device)
-    with torch.cuda.device(q.device):
+    library = nat.lib()
+    ws_bytes = library.kf_attention_backward_workspace_bytes(rows, heads)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    with _on_device_of(q):
         nat.check(
-            nat.lib().kf_attention_backward(_heads_view(dq), _heads_view(dk), _heads_view(dv), _heads_view(grad), _heads_view(out),
-                                            lse.data_ptr(), _heads_view(q), _heads_view(k), _heads_view(v), nat.dtype_code(q.dtype),
-                                            sequences, length, rows, heads, kv_heads, width, _ptr(lengths), _ptr(offsets), int(causal),
-                                            scale, ws.data_ptr(), ws_bytes, nat.stream_ptr(q.device)),
+            library.kf_attention_backward(_heads_view(dq), _heads_view(dk), _heads_view(dv), _heads_view(grad), _heads_view(out),
+                                          lse.data_ptr(), _heads_view(q), _heads_view(k), _heads_view(v), nat.dtype_code(q.dtype),
+                                          sequences, length, rows, heads, kv_heads, width, _ptr(lengths), _ptr(offsets), int(causal),
+                                          scale, ws.data_ptr(), ws_bytes, nat.launch_stream(q)),
             "kf_attention_backward",
         )
     return dq, dk, dv
@@ -1114,10 +1127,14 @@ def attention_backward(grad: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
 _NORM_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _norm_rows(x: torch.Tensor) -> torch.Tensor:
-    """``x`` as ``[rows, width]`` with a contiguous width (in place where its strides allow it)."""
-    flat = x.reshape(-1, x.shape[-1])
-    return flat if flat.stride(1) == 1 or flat.shape[1] == 1 else flat.contiguous()
+def _norm_rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """``x`` with a contiguous last axis and its rows' stride (in place where the strides of ``x`` allow it)."""
+    width = x.shape[-1]
+    if x.is_contiguous():
+        return x, width
+    flat = x.reshape(-1, width)
+    flat = flat if flat.stride(1) == 1 or width == 1 else flat.contiguous()
+    return flat, flat.stride(0)
 
 
 def _norm_check(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]) -> None:
@@ -1139,19 +1156,21 @@ def norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional
     _norm_check(x, weight, bias)
     _require(out_dtype in _NORM_DTYPES, f"norms return float32, bfloat16 or float16 tensors, not {out_dtype}")
     _require(math.isfinite(eps) and eps >= 0, "eps is finite and not negative")
-    flat = _norm_rows(x)
-    rows, width = flat.shape
+    width = x.shape[-1]
+    rows = x.numel() // width
     out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
     stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if with_stats else None
     if rows == 0:
         return out, stats
-    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    x, stride = _norm_rows(x)
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
     vector = weight if weight is not None else bias
-    with torch.cuda.device(x.device):
+    with _on_device_of(x):
         nat.check(
-            nat.lib().kf_norm_forward(out.data_ptr(), nat.dtype_code(out_dtype), _ptr(stats), flat.data_ptr(), nat.dtype_code(x.dtype), rows,
-                                      width, flat.stride(0), _ptr(weight), _ptr(bias), 0 if vector is None else nat.dtype_code(vector.dtype),
-                                      int(centred), eps, nat.stream_ptr(x.device)),
+            nat.lib().kf_norm_forward(out.data_ptr(), nat.dtype_code(out_dtype), _ptr(stats), x.data_ptr(), nat.dtype_code(x.dtype), rows,
+                                      width, stride, _ptr(weight), _ptr(bias), 0 if vector is None else nat.dtype_code(vector.dtype),
+                                      int(centred), eps, nat.launch_stream(x)),
             "kf_norm_forward",
         )
     return out, stats
@@ -1164,27 +1183,30 @@ def norm_backward(grad: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weig
     of the vector whose gradient is wanted; one dtype for both)."""
     _norm_check(x, weight, None)
     _require(grad.shape == x.shape and grad.device == x.device and grad.dtype in _NORM_DTYPES, "grad has the shape and device of x")
-    flat = _norm_rows(x)
-    rows, width = flat.shape
-    _require(stats.dtype == torch.float32 and stats.is_contiguous() and tuple(stats.shape) == (rows, 2), "stats is what the forward call returned")
+    width = x.shape[-1]
+    rows = x.numel() // width
+    _require(stats.dtype == torch.float32 and stats.is_contiguous() and stats.shape == (rows, 2), "stats is what the forward call returned")
     dtype = weight_dtype if weight_dtype is not None else bias_dtype
     _require(bias_dtype in (None, dtype) and (weight is None or dtype in (None, weight.dtype)), "weight and bias share one dtype")
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if with_input else None
-    dweight, dbias = (None if t is None else torch.empty(width, dtype=t, device=x.device) for t in (weight_dtype, bias_dtype))
+    dweight = None if weight_dtype is None else torch.empty(width, dtype=dtype, device=x.device)
+    dbias = None if bias_dtype is None else torch.empty(width, dtype=dtype, device=x.device)
     if rows == 0:
         return dx, None if dweight is None else dweight.zero_(), None if dbias is None else dbias.zero_()
+    x, stride = _norm_rows(x)
     grad, weight = grad.contiguous(), None if weight is None else weight.contiguous()
-    ws = None
-    ws_bytes = 0
+    library, ws, ws_bytes, code = nat.lib(), None, 0, 0
     if dtype is not None:
-        ws_bytes = nat.lib().kf_norm_backward_workspace_bytes(rows, width)
+        ws_bytes = library.kf_norm_backward_workspace_bytes(rows, width)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
-    code = 0 if weight is None and dtype is None else nat.dtype_code(weight.dtype if weight is not None else dtype)
-    with torch.cuda.device(x.device):
+        code = nat.dtype_code(dtype)
+    elif weight is not None:
+        code = nat.dtype_code(weight.dtype)
+    with _on_device_of(x):
         nat.check(
-            nat.lib().kf_norm_backward(_ptr(dx), _ptr(dweight), _ptr(dbias), grad.data_ptr(), nat.dtype_code(grad.dtype), flat.data_ptr(),
-                                       nat.dtype_code(x.dtype), stats.data_ptr(), rows, width, flat.stride(0), _ptr(weight), code,
-                                       int(centred), _ptr(ws), ws_bytes, nat.stream_ptr(x.device)),
+            library.kf_norm_backward(_ptr(dx), _ptr(dweight), _ptr(dbias), grad.data_ptr(), nat.dtype_code(grad.dtype), x.data_ptr(),
+                                     nat.dtype_code(x.dtype), stats.data_ptr(), rows, width, stride, _ptr(weight), code, int(centred),
+                                     _ptr(ws), ws_bytes, nat.launch_stream(x)),
             "kf_norm_backward",
         )
     return dx, dweight, dbias

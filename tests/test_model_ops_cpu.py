@@ -31,7 +31,7 @@ def anywhere(monkeypatch):
         raise Reached
 
     monkeypatch.setattr(nat, "require_device", lambda t, name: None)
-    monkeypatch.setattr(torch.cuda, "device", stop)
+    monkeypatch.setattr(torch.cuda, "current_device", stop)
     return Reached
 
 
