@@ -57,6 +57,7 @@ struct Args {
     int sequences, length;         // length: token rows per sequence (padded batch)
     int heads, group, width, causal;
     int slots;                     // tile slots of all sequences
+    int chunk;                     // tile slots that go to one XCD together
     float scale;
 };
 
@@ -134,31 +135,62 @@ struct Image {
     }
     static __device__ __forceinline__ int at(int row, int chunk) { return row * ROW_BYTES + swizzle(row, chunk) * 16; }
 
-    // the lane's fragment of rows row0 .. row0 + 31, contraction slab `slab`
-    static __device__ __forceinline__ typename Type<T>::Frag row_fragment(const char* tile, int row0, int slab, int lane) {
-        return *reinterpret_cast<const typename Type<T>::Frag*>(tile + at(row0 + (lane & 31), 2 * slab + (lane >> 5)));
-    }
-    // the lane's fragment of the TRANSPOSED tile: columns d0 .. d0 + 31 as rows, contraction over the tile rows that registers
-    // [SLAB_REGS * slab, SLAB_REGS * (slab + 1)) of an accumulator over rows row0 .. row0 + 31 stand for
-    static __device__ __forceinline__ typename Type<T>::Frag column_fragment(const char* tile, int row0, int slab, int d0, int lane) {
+};
+
+// The lane's LDS addresses of the fragments a wave reads: one register each for row and for transposed fragments.  Every tile starts
+// at a multiple of 256 bytes and the image repeats every 16 rows, so the address of another slab, block or column group differs by
+// an exclusive or and an addition of constants.
+template <class T, int DP>
+struct Reader {
+    typedef Image<T, DP> Img;
+    typedef typename Type<T>::Frag Frag;
+    typedef __attribute__((address_space(3))) const Frag* FragPointer;
+    // chunk bits the swizzle reaches above bit 0: they change by exclusive or, the ones above them by addition
+    static constexpr uint32_t XORED = sizeof(T) == 2 ? (Img::CHUNKS == 16 ? 0xe0 : Img::CHUNKS == 8 ? 0x60 : 0x20) : (Img::CHUNKS % 16 == 0 ? 0xe0 : 0x60);
+    uint32_t row, column;
+    __device__ __forceinline__ explicit Reader(int lane) {
+        row = Img::at(lane & 31, lane >> 5);
         if constexpr (sizeof(T) == 2) {
-            const int g = lane >> 4, s = lane & 15;
-            const int row = row0 + 16 * slab + 4 * (g >> 1) + (s >> 2), d = d0 + 16 * (g & 1) + 4 * (s & 3);
+            const int g = lane >> 4, s = lane & 15, d = 16 * (g & 1) + 4 * (s & 3);
+            column = Img::at(4 * (g >> 1) + (s >> 2), d >> 3) + (d & 7) * 2;
+        } else {
+            const int d = lane & 31;
+            column = Img::at(4 * (lane >> 5), d >> 2) + (d & 3) * 4;
+        }
+    }
+    static __device__ __forceinline__ uint32_t moved(uint32_t address, uint32_t bytes) { return (address ^ (bytes & XORED)) + (bytes & ~XORED); }
+    // rows row0 .. row0 + 31 of the tile at LDS address `tile` (row0 a multiple of 32), contraction slab `slab`
+    __device__ __forceinline__ Frag rows(uint32_t tile, int row0, int slab) const {
+        return *reinterpret_cast<FragPointer>(moved(tile + row, slab * 32) + row0 * Img::ROW_BYTES);
+    }
+    // the TRANSPOSED tile: columns 32 t .. 32 t + 31 as rows, contraction over the tile rows that registers [SLAB_REGS * slab,
+    // SLAB_REGS * (slab + 1)) of an accumulator over rows row0 .. row0 + 31 stand for
+    __device__ __forceinline__ Frag columns(uint32_t tile, int row0, int slab, int t) const {
+        if constexpr (sizeof(T) == 2) {
             union { s16x4 h[2]; bf16x8 v; } u;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                u.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s16x4*)(tile + at(row + 8 * i, d >> 3) + (d & 7) * 2));
+                u.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4*>(
+                    (moved(tile + column, 64 * t) ^ (32 * i)) + (row0 + 16 * slab + 8 * i) * Img::ROW_BYTES));
             return u.v;
         } else {
             f32x4 v;
-            const int row = row0 + 8 * slab + 4 * (lane >> 5), d = d0 + (lane & 31);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const float*>(tile + at(row + i, d >> 2) + (d & 3) * 4);
+            for (int i = 0; i < 4; ++i) {
+                // what rows 8 slab + i of the block add to the swizzle
+                constexpr bool SIXTEEN = Img::CHUNKS % 16 == 0;
+                const uint32_t turn = SIXTEEN ? (i << 4) ^ ((slab & 1) << 7) : ((i >> 1) << 4) ^ ((slab & 1) << 6);
+                const uint32_t from = SIXTEEN ? moved(tile + column, 128 * t) : tile + column + 128 * t;
+                v[i] = *reinterpret_cast<__attribute__((address_space(3))) const float*>((from ^ turn) + (row0 + 8 * slab + i) * Img::ROW_BYTES);
+            }
             return v;
         }
     }
 };
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void*)p));
+}
 
 // Rows of one head of one sequence as a buffer: a load behind the last row, or of a column behind the head width, returns 0 without
 // touching memory -- what stands there may be anything, and its weight is 0.  The descriptor is rebuilt per tile (scalar
@@ -176,29 +208,30 @@ struct Rows {
     }
 };
 
-// N rows of a tile into registers (every thread a few 16-byte chunks), and from there to LDS.
-template <class T, int DP, int N>
+// N rows of a tile into registers (every thread of the N_THREADS a few 16-byte chunks), and from there to LDS.
+template <class T, int DP, int N, int N_THREADS = THREADS>
 struct Stage {
     typedef Image<T, DP> Img;
-    static constexpr int PER = N * Img::CHUNKS / THREADS;
-    static_assert(PER * THREADS == N * Img::CHUNKS, "whole chunks per thread");
+    static constexpr int ALL = N * Img::CHUNKS, PER = (ALL + N_THREADS - 1) / N_THREADS;
     u32x4 r[PER];
-    // byte offset of the thread's chunk i inside a tile whose rows are `token` bytes apart
-    static __device__ __forceinline__ uint32_t offset(int i, int64_t token, int width, int tid) {
-        const int n = tid + i * THREADS, chunk = n % Img::CHUNKS;
-        return chunk * 16 < width ? static_cast<uint32_t>(n / Img::CHUNKS * static_cast<int>(token) + chunk * 16) : NO_COLUMN;
-    }
-    __device__ __forceinline__ void load(const Rows& rows, int row0, int tid) {
-        const __amdgpu_buffer_rsrc_t from = rows.from(row0);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) r[i] = __builtin_amdgcn_raw_buffer_load_b128(from, offset(i, rows.token, rows.width, tid), 0, 0);
-    }
-    __device__ __forceinline__ void store(char* tile, int tid) const {
+    uint32_t at[PER];   // byte offsets of the thread's chunks inside a tile in memory, and in LDS
+    int to[PER];
+    __device__ __forceinline__ Stage(int64_t token, int width, int tid) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int n = tid + i * THREADS;
-            *reinterpret_cast<u32x4*>(tile + Img::at(n / Img::CHUNKS, n % Img::CHUNKS)) = r[i];
+            const int n = tid + i * N_THREADS, row = n / Img::CHUNKS, chunk = n % Img::CHUNKS;
+            at[i] = n < ALL && chunk * 16 < width ? static_cast<uint32_t>(row * static_cast<int>(token) + chunk * 16) : NO_COLUMN;
+            to[i] = n < ALL ? Img::at(row, chunk) : N * Img::ROW_BYTES;
         }
+    }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rows) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) r[i] = __builtin_amdgcn_raw_buffer_load_b128(rows, at[i], 0, 0);
+    }
+    __device__ __forceinline__ void store(char* tile) const {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (ALL % N_THREADS == 0 || i + 1 < PER || to[i] < N * Img::ROW_BYTES) *reinterpret_cast<u32x4*>(tile + to[i]) = r[i];
     }
 };
 
@@ -243,13 +276,21 @@ __device__ __forceinline__ bool locate(const Args& a, int slot, bool last_first,
     return true;
 }
 
-// Workgroup -> (slot, head).  Consecutive workgroup ids go to the eight XCDs in turn and each has an L2 of its own: an XCD gets a
-// contiguous run of work items, ordered so that the items that read the same k and v (the query heads of a group, the tiles of a
-// sequence) are neighbours.
-__device__ __forceinline__ int64_t work_item(int64_t id, int64_t count) {
-    constexpr int XCDS = 8;
-    const int64_t per = count / XCDS, rest = count % XCDS, x = id % XCDS, n = id / XCDS;
-    return x * per + min(x, rest) + n;
+// Workgroup -> (slot, kv_head, member of its group).  Consecutive workgroup ids go to the eight XCDs in turn, and each has an L2 of its
+// own: what reads the same k and v should go to one XCD, but no XCD may be left with the longest sequences.  Where (sequence, key /
+// value head) pairs of equal size are many, whole pairs are dealt to the XCDs (a.chunk = the slots of a sequence).  Otherwise
+// single tiles are, the heads of a tile one after the other: with 1, 2, 4 or a multiple of 8 heads an XCD then sees the same heads
+// in every tile.  The `members` query heads of a group stay together.  False: nothing left (the grid is rounded up).
+constexpr int XCDS = 8;
+struct Item { int slot, kv_head, member; };
+__device__ __forceinline__ bool work_item(const Args& a, int members, Item& w) {
+    const int64_t id = blockIdx.x, chunk = static_cast<int64_t>(a.chunk) * members, n = id / XCDS;
+    const int64_t item = (n / chunk * XCDS + id % XCDS) * chunk + n % chunk, pair = item / members;
+    const int kv_heads = a.heads / a.group;
+    w.member = static_cast<int>(item % members);
+    w.slot = static_cast<int>(a.chunk > 1 ? pair % a.slots : pair / kv_heads);
+    w.kv_head = static_cast<int>(a.chunk > 1 ? pair / a.slots : pair % kv_heads);
+    return pair < static_cast<int64_t>(a.slots) * kv_heads;
 }
 
 template <class T>
@@ -299,11 +340,11 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[DP / 32], T* base
         }
 }
 
-template <class T, int DP>
+template <class T, int DP, int N_THREADS = THREADS>
 __device__ __forceinline__ void zero_rows(T* base, int64_t token, int row0, int written, int width, int tid) {
     constexpr int PER = 16 / static_cast<int>(sizeof(T));
     const int chunks = width / PER;
-    for (int n = tid; n < ROWS * chunks; n += THREADS) {
+    for (int n = tid; n < ROWS * chunks; n += N_THREADS) {
         const int row = row0 + n / chunks;
         if (row < written) *reinterpret_cast<u32x4*>(base + row * token + (n % chunks) * PER) = u32x4{0, 0, 0, 0};
     }
@@ -318,12 +359,10 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
     extern __shared__ __align__(16) char lds[];   // [2][k tile, v tile]
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t item = work_item(blockIdx.x, gridDim.x);
-    const int member = static_cast<int>(item % a.group);
-    const int slot = static_cast<int>(item / a.group % a.slots);
-    const int kv_head = static_cast<int>(item / a.group / a.slots), head = kv_head * a.group + member;
+    Item item;
     Place w;
-    if (!locate(a, slot, a.causal, w)) return;
+    if (!work_item(a, a.group, item) || !locate(a, item.slot, a.causal, w)) return;
+    const int kv_head = item.kv_head, head = kv_head * a.group + item.member;
     T* o = rows_out<T>(a.o, w, head);
     float* lse = a.lse ? a.lse + head * a.rows + w.stat : nullptr;
     if (w.row0 >= w.length) {
@@ -341,19 +380,19 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
     float top = -INFINITY, sum = 0.0f;   // running maximum of c s; this half's part of the running sum
 
     const int end = a.causal ? min(w.length, w.row0 + ROWS) : w.length, tiles = (end + BK - 1) / BK;
-    Stage<T, DP, BK> sk, sv;
-    sk.load(k, 0, tid);
-    sv.load(v, 0, tid);
-    sk.store(lds, tid);
-    sv.store(lds + TILE, tid);
+    Stage<T, DP, BK> sk(k.token, k.width, tid), sv(v.token, v.width, tid);
+    const Reader<T, DP> read(lane);
+    sk.load(k.from(0));
+    sv.load(v.from(0));
+    sk.store(lds);
+    sv.store(lds + TILE);
     for (int t = 0; t < tiles; ++t) {
-        const char* kt = lds + (t & 1) * 2 * TILE;
-        const char* vt = kt + TILE;
+        const uint32_t kt = lds_address(lds) + (t & 1) * 2 * TILE, vt = kt + TILE;
         const int k0 = t * BK;
         __syncthreads();   // tile t is written; everybody is done with tile t - 1, whose place t + 1 takes below
         if (t + 1 < tiles) {
-            sk.load(k, k0 + BK, tid);
-            sv.load(v, k0 + BK, tid);
+            sk.load(k.from(k0 + BK));
+            sv.load(v.from(k0 + BK));
         }
         if (!(a.causal && k0 > first + 31)) {   // (wave-uniform)
             f32x16 s[BK / 32];
@@ -361,7 +400,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
             for (int b = 0; b < BK / 32; ++b) {
                 s[b] = f32x16{};
 #pragma unroll
-                for (int i = 0; i < Img::SLABS; ++i) s[b] = Type<T>::mma(Img::row_fragment(kt, 32 * b, i, lane), q.f[i], s[b]);
+                for (int i = 0; i < Img::SLABS; ++i) s[b] = Type<T>::mma(read.rows(kt, 32 * b, i), q.f[i], s[b]);
             }
             if (k0 + BK > w.length || (a.causal && k0 + BK - 1 > first)) {
                 const int visible = a.causal ? min(w.length, query + 1) : w.length;
@@ -396,13 +435,13 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
                 for (int i = 0; i < SECOND; ++i) {
                     const Frag p = Type<T>::from_acc(s[b], i);
 #pragma unroll
-                    for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mma(Img::column_fragment(vt, 32 * b, i, 32 * d, lane), p, acc[d]);
+                    for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mma(read.columns(vt, 32 * b, i, d), p, acc[d]);
                 }
             }
         }
         if (t + 1 < tiles) {
-            sk.store(lds + ((t + 1) & 1) * 2 * TILE, tid);
-            sv.store(lds + ((t + 1) & 1) * 2 * TILE + TILE, tid);
+            sk.store(lds + ((t + 1) & 1) * 2 * TILE);
+            sv.store(lds + ((t + 1) & 1) * 2 * TILE + TILE);
         }
     }
     sum += other_half(sum);
@@ -420,12 +459,10 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
     extern __shared__ __align__(16) char lds[];   // [2][k tile, v tile]
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t item = work_item(blockIdx.x, gridDim.x);
-    const int member = static_cast<int>(item % a.group);
-    const int slot = static_cast<int>(item / a.group % a.slots);
-    const int kv_head = static_cast<int>(item / a.group / a.slots), head = kv_head * a.group + member;
+    Item item;
     Place w;
-    if (!locate(a, slot, a.causal, w)) return;
+    if (!work_item(a, a.group, item) || !locate(a, item.slot, a.causal, w)) return;
+    const int kv_head = item.kv_head, head = kv_head * a.group + item.member;
     T* dq = rows_out<T>(a.dq, w, head);
     if (w.row0 >= w.length) {
         zero_rows<T, DP>(dq, a.dq.token, w.row0, w.written, a.width, tid);
@@ -453,19 +490,19 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
     f32x16 acc[DP / 32] = {};
     const float c = a.scale * LOG2E;
     const int end = a.causal ? min(w.length, w.row0 + ROWS) : w.length, tiles = (end + BK - 1) / BK;
-    Stage<T, DP, BK> sk, sv;
-    sk.load(k, 0, tid);
-    sv.load(v, 0, tid);
-    sk.store(lds, tid);
-    sv.store(lds + TILE, tid);
+    Stage<T, DP, BK> sk(k.token, k.width, tid), sv(v.token, v.width, tid);
+    const Reader<T, DP> read(lane);
+    sk.load(k.from(0));
+    sv.load(v.from(0));
+    sk.store(lds);
+    sv.store(lds + TILE);
     for (int t = 0; t < tiles; ++t) {
-        const char* kt = lds + (t & 1) * 2 * TILE;
-        const char* vt = kt + TILE;
+        const uint32_t kt = lds_address(lds) + (t & 1) * 2 * TILE, vt = kt + TILE;
         const int k0 = t * BK;
         __syncthreads();
         if (t + 1 < tiles) {
-            sk.load(k, k0 + BK, tid);
-            sv.load(v, k0 + BK, tid);
+            sk.load(k.from(k0 + BK));
+            sv.load(v.from(k0 + BK));
         }
         if (!(a.causal && k0 > first + 31)) {
             const bool masked = k0 + BK > w.length || (a.causal && k0 + BK - 1 > first);
@@ -474,9 +511,9 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
             for (int b = 0; b < BK / 32; ++b) {
                 f32x16 s = {}, dp = {};
 #pragma unroll
-                for (int i = 0; i < Img::SLABS; ++i) s = Type<T>::mma(Img::row_fragment(kt, 32 * b, i, lane), q.f[i], s);
+                for (int i = 0; i < Img::SLABS; ++i) s = Type<T>::mma(read.rows(kt, 32 * b, i), q.f[i], s);
 #pragma unroll
-                for (int i = 0; i < Img::SLABS; ++i) dp = Type<T>::mma(Img::row_fragment(vt, 32 * b, i, lane), g.f[i], dp);
+                for (int i = 0; i < Img::SLABS; ++i) dp = Type<T>::mma(read.rows(vt, 32 * b, i), g.f[i], dp);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
                 if (masked) {
@@ -488,13 +525,13 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
                 for (int i = 0; i < SECOND; ++i) {
                     const Frag ds = Type<T>::from_acc(s, i);
 #pragma unroll
-                    for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mma(Img::column_fragment(kt, 32 * b, i, 32 * d, lane), ds, acc[d]);
+                    for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mma(read.columns(kt, 32 * b, i, d), ds, acc[d]);
                 }
             }
         }
         if (t + 1 < tiles) {
-            sk.store(lds + ((t + 1) & 1) * 2 * TILE, tid);
-            sv.store(lds + ((t + 1) & 1) * 2 * TILE + TILE, tid);
+            sk.store(lds + ((t + 1) & 1) * 2 * TILE);
+            sv.store(lds + ((t + 1) & 1) * 2 * TILE + TILE);
         }
     }
     // a row that sees one key has p = 1 whatever its score: ds is exactly 0, not the difference of two roundings
@@ -507,18 +544,21 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
 }
 
 // ---- backward: dk and dv --------------------------------------------------------------------------------------------------
-template <class T, int DP, int BQ, int WAVES>
+// VL: the wave's v fragments are re-read from LDS instead of kept in registers (width 128: two 32 x 128 fp32 accumulators and k alone
+// take 160 of the 256 registers a wave has when two share a SIMD).
+template <class T, int DP, int BQ, bool VL, int WAVES>
 __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Args a) {
     typedef Image<T, DP> Img;
     typedef typename Type<T>::Frag Frag;
     constexpr int TILE = BQ * Img::ROW_BYTES, STAGE = 2 * TILE + 2 * BQ * 4, SECOND = 16 / Type<T>::SLAB_REGS;
-    extern __shared__ __align__(16) char lds[];   // [2][q tile, g tile, L of its rows, D of its rows]
+    static_assert(STAGE % 256 == 0, "tiles start at multiples of 256 bytes");
+    extern __shared__ __align__(16) char lds[];   // [2][q tile, g tile, L of its rows, D of its rows], with VL the workgroup's v rows
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t item = work_item(blockIdx.x, gridDim.x);
-    const int slot = static_cast<int>(item % a.slots), kv_head = static_cast<int>(item / a.slots);
+    Item item;
     Place w;
-    if (!locate(a, slot, false, w)) return;
+    if (!work_item(a, 1, item) || !locate(a, item.slot, false, w)) return;
+    const int kv_head = item.kv_head;
     T* dk = rows_out<T>(a.dk, w, kv_head);
     T* dv = rows_out<T>(a.dv, w, kv_head);
     if (w.row0 >= w.length) {
@@ -527,81 +567,101 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
         return;
     }
     const int first = w.row0 + 32 * wave, key = first + (lane & 31), half = lane >> 5;
+    const Reader<T, DP> read(lane);
+    const uint32_t own_v = lds_address(lds) + 2 * STAGE + 32 * wave * Img::ROW_BYTES;
     Held<T, DP> k, v;
     k.load(input_rows<T>(a, a.k, w, kv_head), first, lane);
-    v.load(input_rows<T>(a, a.v, w, kv_head), first, lane);
+    if constexpr (VL) {
+        const Rows rows = input_rows<T>(a, a.v, w, kv_head);
+        Stage<T, DP, ROWS> sv(rows.token, rows.width, tid);
+        sv.load(rows.from(w.row0));
+        sv.store(lds + 2 * STAGE);
+    } else {
+        v.load(input_rows<T>(a, a.v, w, kv_head), first, lane);
+    }
     f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
     const float c = a.scale * LOG2E;
 
-    // the query tiles of the group's heads, one after the other: step n is tile begin + n % tiles of head n / tiles
+    // the query tiles of the group's heads, one after the other: tile begin + n of head `member`
     const int begin = a.causal ? w.row0 / BQ : 0, tiles = (w.length + BQ - 1) / BQ - begin, steps = tiles * a.group;
-    Stage<T, DP, BQ> sq, sg;
+    int next_head = kv_head * a.group, next_tile = begin;   // the tile to stage next
+    Rows q = input_rows<T>(a, a.q, w, next_head), g = input_rows<T>(a, a.g, w, next_head);
+    Stage<T, DP, BQ> sq(q.token, q.width, tid), sg(g.token, g.width, tid);
     float stat = 0.0f;   // threads 0 .. BQ-1: L, the next BQ: D, of the staged tile's rows
-    auto load = [&](int n) {
-        const int head = kv_head * a.group + n / tiles, q0 = (begin + n % tiles) * BQ;
-        sq.load(input_rows<T>(a, a.q, w, head), q0, tid);
-        sg.load(input_rows<T>(a, a.g, w, head), q0, tid);
+    auto load = [&] {
+        const int q0 = next_tile * BQ;
+        sq.load(q.from(q0));
+        sg.load(g.from(q0));
         if (tid < 2 * BQ) {
             const int row = q0 + tid % BQ;
-            const float* from = (tid < BQ ? a.lse : a.delta) + head * a.rows + w.stat;
+            const float* from = (tid < BQ ? a.lse : a.delta) + next_head * a.rows + w.stat;
             stat = row < w.length ? from[row] : tid < BQ ? INFINITY : 0.0f;   // L = inf: p = 0 for rows that hold no token
         }
-    };
-    auto store = [&](int n) {
-        char* at = lds + (n & 1) * STAGE;
-        sq.store(at, tid);
-        sg.store(at + TILE, tid);
-        if (tid < 2 * BQ) reinterpret_cast<float*>(at + 2 * TILE)[tid] = stat;
-    };
-    load(0);
-    store(0);
-    for (int n = 0; n < steps; ++n) {
-        const char* qt = lds + (n & 1) * STAGE;
-        const char* gt = qt + TILE;
-        const float* lse = reinterpret_cast<const float*>(qt + 2 * TILE);
-        const float* delta = lse + BQ;
-        const int q0 = (begin + n % tiles) * BQ;
-        __syncthreads();
-        if (n + 1 < steps) load(n + 1);
-        if (!(a.causal && q0 + BQ <= first)) {
-            const bool masked = (a.causal && q0 < first + 31) || w.length == 1;
-#pragma unroll
-            for (int b = 0; b < BQ / 32; ++b) {
-                f32x16 s = {}, dp = {};
-#pragma unroll
-                for (int i = 0; i < Img::SLABS; ++i) s = Type<T>::mma(Img::row_fragment(qt, 32 * b, i, lane), k.f[i], s);
-#pragma unroll
-                for (int i = 0; i < Img::SLABS; ++i) dp = Type<T>::mma(Img::row_fragment(gt, 32 * b, i, lane), v.f[i], dp);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + 32 * b + 8 * i + 4 * half);
-                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(delta + 32 * b + 8 * i + 4 * half);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int r = 4 * i + j;
-                        s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -l4[j]));
-                        dp[r] = s[r] * (dp[r] - d4[j]);
-                    }
-                }
-                if (masked) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int query = q0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4;
-                        if (a.causal && query < key) { s[r] = 0.0f; dp[r] = 0.0f; }
-                        if (a.causal ? query == 0 : w.length == 1) dp[r] = 0.0f;   // one visible key: ds is exactly 0
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < SECOND; ++i) {
-                    const Frag p = Type<T>::from_acc(s, i), ds = Type<T>::from_acc(dp, i);
-#pragma unroll
-                    for (int d = 0; d < DP / 32; ++d) av[d] = Type<T>::mma(Img::column_fragment(gt, 32 * b, i, 32 * d, lane), p, av[d]);
-#pragma unroll
-                    for (int d = 0; d < DP / 32; ++d) ak[d] = Type<T>::mma(Img::column_fragment(qt, 32 * b, i, 32 * d, lane), ds, ak[d]);
-                }
+        if (++next_tile == begin + tiles) {
+            next_tile = begin;
+            if (++next_head < (kv_head + 1) * a.group) {
+                q.base += a.q.head * static_cast<int64_t>(sizeof(T));
+                g.base += a.g.head * static_cast<int64_t>(sizeof(T));
             }
         }
-        if (n + 1 < steps) store(n + 1);
+    };
+    auto store = [&](char* at) {
+        sq.store(at);
+        sg.store(at + TILE);
+        if (tid < 2 * BQ) reinterpret_cast<float*>(at + 2 * TILE)[tid] = stat;
+    };
+    load();
+    store(lds);
+    int tile = begin;
+    for (int n = 0; n < steps; ++n) {
+        const uint32_t qt = lds_address(lds) + (n & 1) * STAGE, gt = qt + TILE;
+        const float* lse = reinterpret_cast<const float*>(lds + (n & 1) * STAGE + 2 * TILE);
+        const float* delta = lse + BQ;
+        const int q0 = tile * BQ;
+        if (++tile == begin + tiles) tile = begin;
+        __syncthreads();
+        if (n + 1 < steps) load();
+#pragma unroll
+        for (int b = 0; b < BQ / 32; ++b) {
+            if (a.causal && q0 + 32 * b + 32 <= first) continue;   // (wave-uniform)
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int i = 0; i < Img::SLABS; ++i) s = Type<T>::mma(read.rows(qt, 32 * b, i), k.f[i], s);
+#pragma unroll
+            for (int i = 0; i < Img::SLABS; ++i) {
+                if constexpr (VL) dp = Type<T>::mma(read.rows(gt, 32 * b, i), read.rows(own_v, 0, i), dp);
+                else dp = Type<T>::mma(read.rows(gt, 32 * b, i), v.f[i], dp);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + 32 * b + 8 * i + 4 * half);
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(delta + 32 * b + 8 * i + 4 * half);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = 4 * i + j;
+                    s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -l4[j]));
+                    dp[r] = s[r] * (dp[r] - d4[j]);
+                }
+            }
+            if ((a.causal && q0 + 32 * b < first + 31) || w.length == 1) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int query = q0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4;
+                    const bool seen = !a.causal || query >= key, lone = a.causal ? query == 0 : true;
+                    if (!seen) s[r] = 0.0f;
+                    if (!seen || lone) dp[r] = 0.0f;   // a row that sees one key: ds is exactly 0
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < SECOND; ++i) {
+                const Frag p = Type<T>::from_acc(s, i), ds = Type<T>::from_acc(dp, i);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) av[d] = Type<T>::mma(read.columns(gt, 32 * b, i, d), p, av[d]);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) ak[d] = Type<T>::mma(read.columns(qt, 32 * b, i, d), ds, ak[d]);
+            }
+        }
+        if (n + 1 < steps) store(lds + ((n + 1) & 1) * STAGE);
     }
     if (key >= w.length) {
 #pragma unroll
@@ -615,12 +675,13 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
 // Tile rows and waves per SIMD of each kernel.
 template <class T, int DP>
 struct Shape {
-    static constexpr int KEYS = sizeof(T) == 2 ? 64 : 32, QUERIES = sizeof(T) == 2 && DP <= 96 ? 64 : 32;
-    static constexpr int KEY_LDS = 4 * KEYS * Image<T, DP>::ROW_BYTES, QUERY_LDS = 4 * QUERIES * Image<T, DP>::ROW_BYTES + 4 * QUERIES * 4;
-    static constexpr int FORWARD_WAVES = sizeof(T) == 2 ? 2 : 1, DQ_WAVES = sizeof(T) == 2 ? 2 : 1, DKV_WAVES = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
-    static constexpr auto forward = &attention_forward_kernel<T, DP, KEYS, FORWARD_WAVES>;
-    static constexpr auto dq = &attention_dq_kernel<T, DP, KEYS, DQ_WAVES>;
-    static constexpr auto dkv = &attention_dkv_kernel<T, DP, QUERIES, DKV_WAVES>;
+    static constexpr bool TWO = sizeof(T) == 2, VL = TWO && DP > 96;
+    static constexpr int KEYS = TWO ? 64 : 32, QUERIES = TWO && DP <= 96 ? 64 : 32, WAVES = TWO ? 2 : 1;
+    static constexpr int KEY_LDS = 4 * KEYS * Image<T, DP>::ROW_BYTES;
+    static constexpr int QUERY_LDS = 4 * QUERIES * Image<T, DP>::ROW_BYTES + 4 * QUERIES * 4 + (VL ? ROWS * Image<T, DP>::ROW_BYTES : 0);
+    static constexpr auto forward = &attention_forward_kernel<T, DP, KEYS, WAVES>;
+    static constexpr auto dq = &attention_dq_kernel<T, DP, KEYS, WAVES>;
+    static constexpr auto dkv = &attention_dkv_kernel<T, DP, QUERIES, VL, WAVES>;
 };
 
 template <class T, int DP>
@@ -647,12 +708,13 @@ int configure_kernels() {
 template <class T, int DP>
 int launch_width(Args& a, bool backward, hipStream_t stream) {
     typedef Shape<T, DP> S;
-    const unsigned items = static_cast<unsigned>(static_cast<int64_t>(a.slots) * a.heads);
+    const int64_t round = XCDS * a.chunk, slots = (static_cast<int64_t>(a.slots) * (a.heads / a.group) + round - 1) / round * round;
+    const unsigned items = static_cast<unsigned>(slots * a.group);
     if (!backward) {
         S::forward<<<items, THREADS, S::KEY_LDS, stream>>>(a);
     } else {
         S::dq<<<items, THREADS, S::KEY_LDS, stream>>>(a);
-        S::dkv<<<items / a.group, THREADS, S::QUERY_LDS, stream>>>(a);
+        S::dkv<<<static_cast<unsigned>(slots), THREADS, S::QUERY_LDS, stream>>>(a);
     }
     return hipGetLastError() == hipSuccess ? KF_OK : KF_ERR_LAUNCH_FAILED;
 }
@@ -683,7 +745,10 @@ int fill(Args& a, int dtype, int64_t sequences, int64_t length, int64_t rows, in
         return KF_ERR_INVALID_ARGUMENT;
     if (offsets ? lengths != nullptr : (length <= 0 || sequences > limit / length || rows != sequences * length)) return KF_ERR_INVALID_ARGUMENT;
     const int64_t slots = offsets ? rows / ROWS + sequences + 1 : sequences * ((length + ROWS - 1) / ROWS);
-    if (sequences >= limit || slots > limit / heads) return KF_ERR_INVALID_ARGUMENT;
+    const int64_t tiles = offsets ? 0 : slots / sequences, groups = offsets ? 0 : sequences * kv_heads;
+    const int64_t chunk = groups >= 64 ? tiles : 1;
+    if (sequences >= limit || slots > (limit - XCDS * chunk * heads) / heads) return KF_ERR_INVALID_ARGUMENT;
+    a.chunk = static_cast<int>(chunk);
     a.lengths = lengths;
     a.offsets = offsets;
     a.rows = rows;
