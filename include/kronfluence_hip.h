@@ -470,7 +470,8 @@ typedef struct kf_heads_view {
 int kf_attention_forward(const kf_heads_view* out, float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v,
                          int dtype, int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width,
                          const int32_t* lengths, const int32_t* offsets, int causal, float scale, void* stream);
-int64_t kf_attention_backward_workspace_bytes(int64_t rows, int64_t heads);
+int64_t kf_attention_backward_workspace_bytes(int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width,
+                                              int packed, int causal);
 int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, const kf_heads_view* dv, const kf_heads_view* grad,
                           const kf_heads_view* out, const float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v,
                           int dtype, int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width,

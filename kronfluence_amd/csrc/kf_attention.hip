@@ -39,6 +39,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int THREADS = 256;      // 4 waves
 constexpr int ROWS = 128;         // rows (queries; keys in the dK / dV kernel) of a workgroup: 32 per wave
+constexpr float SLACK = 8.0f;     // the sum of n terms stays below 2^8 n
 constexpr float LOG2E = 1.44269504088896340736f;
 
 struct Tensor {   // [batch][token][head][width], the width contiguous; strides in elements
@@ -51,6 +52,8 @@ struct Args {
     Tensor dq, dk, dv;
     float* lse;                    // [heads][rows]: L
     float* delta;                  // [heads][rows]: D
+    float* partial;                // [parts][dk, dv][kv_heads][rows][width], if the dk / dv kernel's work is split (parts > 1)
+    int parts;
     const int32_t* lengths;        // per sequence (padded batch), or null
     const int32_t* offsets;        // [sequences + 1] (packed batch), or null
     int64_t rows;                  // token rows in all: batch * length, or the packed total
@@ -113,55 +116,32 @@ struct Type<float> {
     }
 };
 
-// ---- an operand tile in LDS: [row][16-byte chunk], the chunk XORed with a function of the row --------------------------------
-// Two kinds of reads meet the same image.  Row fragments: 32 consecutive rows, one 16-byte chunk each -- any 16 consecutive rows
-// must fall into the 16 different 16-byte slots of the 256-byte bank space.  Transposed reads of 2-byte types: 4 consecutive rows,
-// 64 consecutive bytes each -- the four must fall into its four quarters.
-template <class T, int DP>
+// ---- an operand tile of N rows in LDS: [64-byte column block][row][4 chunks of 16 bytes], the chunk XORed with (row / 4) % 4 -----
+// Two kinds of reads meet the same image.  Row fragments: 32 consecutive rows, one chunk each -- any 16 consecutive rows fall into the
+// 16 different slots of the 256-byte bank space.  Transposed reads of 2-byte types: 4 consecutive rows, 64 bytes each -- 256
+// consecutive bytes.  The address of any other slab, block or half differs by a constant of the instruction, but for one bit that
+// changes by exclusive or: a lane keeps one register per kind of read.
+template <class T, int DP, int N>
 struct Image {
-    static constexpr int CHUNKS = DP * static_cast<int>(sizeof(T)) / 16;
-    static constexpr int ROW_BYTES = CHUNKS * 16;
-    static constexpr int SLABS = CHUNKS / 2;
-    static __device__ __forceinline__ int swizzle(int row, int chunk) {
-        if constexpr (sizeof(T) == 2) {
-            const int low = (row >> 2) & 3;
-            if constexpr (CHUNKS == 16) return chunk ^ (((row & 3) << 2) | low);
-            else if constexpr (CHUNKS == 8) return chunk ^ ((((row >> 1) & 1) << 2) | low);
-            else return chunk ^ low;
-        } else {
-            if constexpr (CHUNKS % 16 == 0) return chunk ^ (row & 15);
-            else return chunk ^ ((row >> 1) & 7);
-        }
-    }
-    static __device__ __forceinline__ int at(int row, int chunk) { return row * ROW_BYTES + swizzle(row, chunk) * 16; }
-
+    static constexpr int CHUNKS = DP * static_cast<int>(sizeof(T)) / 16, SLABS = CHUNKS / 2;
+    static constexpr int BLOCK = N * 64, BYTES = CHUNKS / 4 * BLOCK;
 };
 
-// The lane's LDS addresses of the fragments a wave reads: one register each for row and for transposed fragments.  Every tile starts
-// at a multiple of 256 bytes and the image repeats every 16 rows, so the address of another slab, block or column group differs by
-// an exclusive or and an addition of constants.
-template <class T, int DP>
+template <class T, int DP, int N>
 struct Reader {
-    typedef Image<T, DP> Img;
+    typedef Image<T, DP, N> Img;
     typedef typename Type<T>::Frag Frag;
     typedef __attribute__((address_space(3))) const Frag* FragPointer;
-    // chunk bits the swizzle reaches above bit 0: they change by exclusive or, the ones above them by addition
-    static constexpr uint32_t XORED = sizeof(T) == 2 ? (Img::CHUNKS == 16 ? 0xe0 : Img::CHUNKS == 8 ? 0x60 : 0x20) : (Img::CHUNKS % 16 == 0 ? 0xe0 : 0x60);
     uint32_t row, column;
     __device__ __forceinline__ explicit Reader(int lane) {
-        row = Img::at(lane & 31, lane >> 5);
-        if constexpr (sizeof(T) == 2) {
-            const int g = lane >> 4, s = lane & 15, d = 16 * (g & 1) + 4 * (s & 3);
-            column = Img::at(4 * (g >> 1) + (s >> 2), d >> 3) + (d & 7) * 2;
-        } else {
-            const int d = lane & 31;
-            column = Img::at(4 * (lane >> 5), d >> 2) + (d & 3) * 4;
-        }
+        const int r = lane & 31, g = lane >> 4, s = lane & 15;
+        row = r * 64 + (((lane >> 5) ^ (r >> 2)) & 3) * 16;
+        if constexpr (sizeof(T) == 2) column = (4 * (g >> 1) + (s >> 2)) * 64 + ((2 * (g & 1) + ((s & 3) >> 1)) ^ (g >> 1)) * 16 + (s & 1) * 8;
+        else column = (r >> 4) * Img::BLOCK + 4 * (lane >> 5) * 64 + ((s >> 2) ^ (lane >> 5)) * 16 + (s & 3) * 4;
     }
-    static __device__ __forceinline__ uint32_t moved(uint32_t address, uint32_t bytes) { return (address ^ (bytes & XORED)) + (bytes & ~XORED); }
     // rows row0 .. row0 + 31 of the tile at LDS address `tile` (row0 a multiple of 32), contraction slab `slab`
     __device__ __forceinline__ Frag rows(uint32_t tile, int row0, int slab) const {
-        return *reinterpret_cast<FragPointer>(moved(tile + row, slab * 32) + row0 * Img::ROW_BYTES);
+        return *reinterpret_cast<FragPointer>(((tile + row) ^ (slab % 2 * 32)) + slab / 2 * Img::BLOCK + row0 * 64);
     }
     // the TRANSPOSED tile: columns 32 t .. 32 t + 31 as rows, contraction over the tile rows that registers [SLAB_REGS * slab,
     // SLAB_REGS * (slab + 1)) of an accumulator over rows row0 .. row0 + 31 stand for
@@ -171,18 +151,14 @@ struct Reader {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 u.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4*>(
-                    (moved(tile + column, 64 * t) ^ (32 * i)) + (row0 + 16 * slab + 8 * i) * Img::ROW_BYTES));
+                    ((tile + column) ^ (32 * i)) + t * Img::BLOCK + (row0 + 16 * slab + 8 * i) * 64));
             return u.v;
         } else {
             f32x4 v;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // what rows 8 slab + i of the block add to the swizzle
-                constexpr bool SIXTEEN = Img::CHUNKS % 16 == 0;
-                const uint32_t turn = SIXTEEN ? (i << 4) ^ ((slab & 1) << 7) : ((i >> 1) << 4) ^ ((slab & 1) << 6);
-                const uint32_t from = SIXTEEN ? moved(tile + column, 128 * t) : tile + column + 128 * t;
-                v[i] = *reinterpret_cast<__attribute__((address_space(3))) const float*>((from ^ turn) + (row0 + 8 * slab + i) * Img::ROW_BYTES);
-            }
+            for (int i = 0; i < 4; ++i)
+                v[i] = *reinterpret_cast<__attribute__((address_space(3))) const float*>(((tile + column) ^ (slab % 2 * 32)) + 2 * t * Img::BLOCK +
+                                                                                        (row0 + 8 * slab + i) * 64);
             return v;
         }
     }
@@ -208,20 +184,21 @@ struct Rows {
     }
 };
 
-// N rows of a tile into registers (every thread of the N_THREADS a few 16-byte chunks), and from there to LDS.
-template <class T, int DP, int N, int N_THREADS = THREADS>
+// N rows of a tile into registers (every thread a few 16-byte chunks: four threads a 64-byte piece of a row), and from there to LDS,
+// where the n-th chunk of the workgroup goes to byte 16 n but for the exclusive or.
+template <class T, int DP, int N>
 struct Stage {
-    typedef Image<T, DP> Img;
-    static constexpr int ALL = N * Img::CHUNKS, PER = (ALL + N_THREADS - 1) / N_THREADS;
+    typedef Image<T, DP, N> Img;
+    static constexpr int ALL = Img::BYTES / 16, PER = (ALL + THREADS - 1) / THREADS;
     u32x4 r[PER];
-    uint32_t at[PER];   // byte offsets of the thread's chunks inside a tile in memory, and in LDS
-    int to[PER];
+    uint32_t at[PER];   // byte offsets of the thread's chunks inside a tile in memory
+    int to;             // byte offset of the first one in LDS; the others follow every 16 THREADS bytes
     __device__ __forceinline__ Stage(int64_t token, int width, int tid) {
+        to = (tid * 16) ^ ((tid >> 4 & 3) * 16);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int n = tid + i * N_THREADS, row = n / Img::CHUNKS, chunk = n % Img::CHUNKS;
-            at[i] = n < ALL && chunk * 16 < width ? static_cast<uint32_t>(row * static_cast<int>(token) + chunk * 16) : NO_COLUMN;
-            to[i] = n < ALL ? Img::at(row, chunk) : N * Img::ROW_BYTES;
+            const int n = tid + i * THREADS, row = n / 4 % N, chunk = n / 4 / N * 4 + n % 4;
+            at[i] = chunk * 16 < width ? static_cast<uint32_t>(row * static_cast<int>(token) + chunk * 16) : NO_COLUMN;
         }
     }
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rows) {
@@ -231,7 +208,7 @@ struct Stage {
     __device__ __forceinline__ void store(char* tile) const {
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-            if (ALL % N_THREADS == 0 || i + 1 < PER || to[i] < N * Img::ROW_BYTES) *reinterpret_cast<u32x4*>(tile + to[i]) = r[i];
+            if (ALL % THREADS == 0 || i + 1 < PER || to + i * 16 * THREADS < Img::BYTES) *reinterpret_cast<u32x4*>(tile + to + i * 16 * THREADS) = r[i];
     }
 };
 
@@ -310,11 +287,12 @@ __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32);
 // The fragments of 32 rows straight from memory (lane & 31 = row): the operand a wave keeps for the whole kernel.
 template <class T, int DP>
 struct Held {
-    typename Type<T>::Frag f[Image<T, DP>::SLABS];
+    static constexpr int SLABS = DP * static_cast<int>(sizeof(T)) / 32;
+    typename Type<T>::Frag f[SLABS];
     __device__ __forceinline__ void load(const Rows& rows, int row0, int lane) {
         const __amdgpu_buffer_rsrc_t from = rows.from(row0);
 #pragma unroll
-        for (int s = 0; s < Image<T, DP>::SLABS; ++s) {
+        for (int s = 0; s < SLABS; ++s) {
             const int c = 2 * s + (lane >> 5);
             union { u32x4 u; typename Type<T>::Frag f; } v;
             v.u = __builtin_amdgcn_raw_buffer_load_b128(
@@ -353,9 +331,9 @@ __device__ __forceinline__ void zero_rows(T* base, int64_t token, int row0, int 
 // ---- forward ------------------------------------------------------------------------------------------------------------
 template <class T, int DP, int BK, int WAVES>
 __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const Args a) {
-    typedef Image<T, DP> Img;
+    typedef Image<T, DP, BK> Img;
     typedef typename Type<T>::Frag Frag;
-    constexpr int TILE = BK * Img::ROW_BYTES, SECOND = 16 / Type<T>::SLAB_REGS;
+    constexpr int TILE = Img::BYTES, SECOND = 16 / Type<T>::SLAB_REGS;
     extern __shared__ __align__(16) char lds[];   // [2][k tile, v tile]
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -377,11 +355,11 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
     q.load(input_rows<T>(a, a.q, w, head), first, lane);
     f32x16 acc[DP / 32] = {};
     const float c = a.scale * LOG2E;
-    float top = -INFINITY, sum = 0.0f;   // running maximum of c s; this half's part of the running sum
+    float top = -INFINITY, sum = 0.0f;   // a running reference near the maximum of c s; this half's part of the running sum
 
     const int end = a.causal ? min(w.length, w.row0 + ROWS) : w.length, tiles = (end + BK - 1) / BK;
     Stage<T, DP, BK> sk(k.token, k.width, tid), sv(v.token, v.width, tid);
-    const Reader<T, DP> read(lane);
+    const Reader<T, DP, BK> read(lane);
     sk.load(k.from(0));
     sv.load(v.from(0));
     sk.store(lds);
@@ -416,14 +394,17 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
 #pragma unroll
                 for (int r = 0; r < 16; ++r) m = fmaxf(m, s[b][r]);
             m = fmaxf(m, other_half(m)) * c;
-            const float now = fmaxf(top, m), base = now == -INFINITY ? 0.0f : now;
-            if (__any(now != top)) {
-                const float shrink = __builtin_amdgcn_exp2f(top - base);
-                sum *= shrink;
+            // any reference does that keeps 2^(c s - top) in range: it moves up only when a row has outgrown it by 2^SLACK
+            if (__any(m > top + SLACK)) {
+                const float now = fmaxf(top, m), shrink = __builtin_amdgcn_exp2f(top - now);   // (m is finite where it is greater)
+                if (m > top + SLACK) {
+                    sum *= shrink;
 #pragma unroll
-                for (int d = 0; d < DP / 32; ++d) acc[d] *= shrink;
+                    for (int d = 0; d < DP / 32; ++d) acc[d] *= shrink;
+                    top = now;
+                }
             }
-            top = now;
+            const float base = top == -INFINITY ? 0.0f : top;   // (a row with no finite score yet)
 #pragma unroll
             for (int b = 0; b < BK / 32; ++b) {
 #pragma unroll
@@ -453,9 +434,9 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
 // ---- backward: dq (and D for the second kernel) ---------------------------------------------------------------------------
 template <class T, int DP, int BK, int WAVES>
 __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args a) {
-    typedef Image<T, DP> Img;
+    typedef Image<T, DP, BK> Img;
     typedef typename Type<T>::Frag Frag;
-    constexpr int TILE = BK * Img::ROW_BYTES, SECOND = 16 / Type<T>::SLAB_REGS;
+    constexpr int TILE = Img::BYTES, SECOND = 16 / Type<T>::SLAB_REGS;
     extern __shared__ __align__(16) char lds[];   // [2][k tile, v tile]
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -491,7 +472,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
     const float c = a.scale * LOG2E;
     const int end = a.causal ? min(w.length, w.row0 + ROWS) : w.length, tiles = (end + BK - 1) / BK;
     Stage<T, DP, BK> sk(k.token, k.width, tid), sv(v.token, v.width, tid);
-    const Reader<T, DP> read(lane);
+    const Reader<T, DP, BK> read(lane);
     sk.load(k.from(0));
     sv.load(v.from(0));
     sk.store(lds);
@@ -548,27 +529,29 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
 // take 160 of the 256 registers a wave has when two share a SIMD).
 template <class T, int DP, int BQ, bool VL, int WAVES>
 __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Args a) {
-    typedef Image<T, DP> Img;
+    typedef Image<T, DP, BQ> Img;
     typedef typename Type<T>::Frag Frag;
-    constexpr int TILE = BQ * Img::ROW_BYTES, STAGE = 2 * TILE + 2 * BQ * 4, SECOND = 16 / Type<T>::SLAB_REGS;
-    static_assert(STAGE % 256 == 0, "tiles start at multiples of 256 bytes");
+    constexpr int TILE = Img::BYTES, STAGE = 2 * TILE + 2 * BQ * 4, SECOND = 16 / Type<T>::SLAB_REGS;
+    static_assert(STAGE % 64 == 0, "tiles start at multiples of 64 bytes");
     extern __shared__ __align__(16) char lds[];   // [2][q tile, g tile, L of its rows, D of its rows], with VL the workgroup's v rows
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     Item item;
     Place w;
-    if (!work_item(a, 1, item) || !locate(a, item.slot, false, w)) return;
+    if (!work_item(a, a.parts, item) || !locate(a, item.slot, false, w)) return;
     const int kv_head = item.kv_head;
     T* dk = rows_out<T>(a.dk, w, kv_head);
     T* dv = rows_out<T>(a.dv, w, kv_head);
     if (w.row0 >= w.length) {
+        if (a.parts > 1) return;   // (the joining kernel's)
         zero_rows<T, DP>(dk, a.dk.token, w.row0, w.written, a.width, tid);
         zero_rows<T, DP>(dv, a.dv.token, w.row0, w.written, a.width, tid);
         return;
     }
     const int first = w.row0 + 32 * wave, key = first + (lane & 31), half = lane >> 5;
-    const Reader<T, DP> read(lane);
-    const uint32_t own_v = lds_address(lds) + 2 * STAGE + 32 * wave * Img::ROW_BYTES;
+    const Reader<T, DP, BQ> read(lane);
+    const Reader<T, DP, ROWS> read_v(lane);
+    const uint32_t own_v = lds_address(lds) + 2 * STAGE + 32 * wave * 64;
     Held<T, DP> k, v;
     k.load(input_rows<T>(a, a.k, w, kv_head), first, lane);
     if constexpr (VL) {
@@ -582,9 +565,11 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
     f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
     const float c = a.scale * LOG2E;
 
-    // the query tiles of the group's heads, one after the other: tile begin + n of head `member`
-    const int begin = a.causal ? w.row0 / BQ : 0, tiles = (w.length + BQ - 1) / BQ - begin, steps = tiles * a.group;
-    int next_head = kv_head * a.group, next_tile = begin;   // the tile to stage next
+    // The query tiles of the group's heads, one head after the other; the workgroup takes its part of these steps.
+    const int begin = a.causal ? w.row0 / BQ : 0, tiles = (w.length + BQ - 1) / BQ - begin;
+    const int all = tiles * a.group, from = static_cast<int>(static_cast<int64_t>(all) * item.member / a.parts);
+    const int steps = static_cast<int>(static_cast<int64_t>(all) * (item.member + 1) / a.parts) - from;
+    int next_head = kv_head * a.group + from / tiles, next_tile = begin + from % tiles;   // the tile to stage next
     Rows q = input_rows<T>(a, a.q, w, next_head), g = input_rows<T>(a, a.g, w, next_head);
     Stage<T, DP, BQ> sq(q.token, q.width, tid), sg(g.token, g.width, tid);
     float stat = 0.0f;   // threads 0 .. BQ-1: L, the next BQ: D, of the staged tile's rows
@@ -594,8 +579,8 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
         sg.load(g.from(q0));
         if (tid < 2 * BQ) {
             const int row = q0 + tid % BQ;
-            const float* from = (tid < BQ ? a.lse : a.delta) + next_head * a.rows + w.stat;
-            stat = row < w.length ? from[row] : tid < BQ ? INFINITY : 0.0f;   // L = inf: p = 0 for rows that hold no token
+            const float* stats = (tid < BQ ? a.lse : a.delta) + next_head * a.rows + w.stat;
+            stat = row < w.length ? stats[row] : tid < BQ ? INFINITY : 0.0f;   // L = inf: p = 0 for rows that hold no token
         }
         if (++next_tile == begin + tiles) {
             next_tile = begin;
@@ -610,9 +595,11 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
         sg.store(at + TILE);
         if (tid < 2 * BQ) reinterpret_cast<float*>(at + 2 * TILE)[tid] = stat;
     };
-    load();
-    store(lds);
-    int tile = begin;
+    int tile = next_tile;
+    if (steps > 0) {
+        load();
+        store(lds);
+    }
     for (int n = 0; n < steps; ++n) {
         const uint32_t qt = lds_address(lds) + (n & 1) * STAGE, gt = qt + TILE;
         const float* lse = reinterpret_cast<const float*>(lds + (n & 1) * STAGE + 2 * TILE);
@@ -629,7 +616,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
             for (int i = 0; i < Img::SLABS; ++i) s = Type<T>::mma(read.rows(qt, 32 * b, i), k.f[i], s);
 #pragma unroll
             for (int i = 0; i < Img::SLABS; ++i) {
-                if constexpr (VL) dp = Type<T>::mma(read.rows(gt, 32 * b, i), read.rows(own_v, 0, i), dp);
+                if constexpr (VL) dp = Type<T>::mma(read.rows(gt, 32 * b, i), read_v.rows(own_v, 0, i), dp);
                 else dp = Type<T>::mma(read.rows(gt, 32 * b, i), v.f[i], dp);
             }
 #pragma unroll
@@ -663,6 +650,13 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
         }
         if (n + 1 < steps) store(lds + ((n + 1) & 1) * STAGE);
     }
+    if (a.parts > 1) {   // (w.stat + key: the token's row among all)
+        const int64_t head = a.rows * a.width, kv_heads = a.heads / a.group;
+        float* to = a.partial + (static_cast<int64_t>(item.member) * 2 * kv_heads + kv_head) * head + w.stat * a.width;
+        store_rows<float, DP>(ak, to, a.width, key, w.length, a.width, a.scale, lane);
+        store_rows<float, DP>(av, to + kv_heads * head, a.width, key, w.length, a.width, 1.0f, lane);
+        return;
+    }
     if (key >= w.length) {
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) { ak[d] = f32x16{}; av[d] = f32x16{}; }
@@ -671,14 +665,43 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
     store_rows<T, DP>(av, dv, a.dv.token, key, w.written, a.width, 1.0f, lane);
 }
 
+// dk and dv as the sums of the parts in order; zero in rows of no sequence.  One thread per four columns.
+template <class T>
+__global__ __launch_bounds__(THREADS) void attention_join_kernel(const Args a) {
+    const int quads = a.width / 4, kv_heads = a.heads / a.group;
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * THREADS + threadIdx.x, all = a.rows * kv_heads;
+    const int64_t line = n / quads, row = line / kv_heads;
+    if (line >= all) return;
+    const int column = static_cast<int>(n % quads) * 4, head = static_cast<int>(line % kv_heads);
+    int64_t sequence = 0, token = row;
+    bool real;
+    if (a.offsets) {
+        real = row < a.offsets[a.sequences];
+    } else {
+        sequence = row / a.length;
+        token = row % a.length;
+        real = !a.lengths || token < a.lengths[sequence];
+    }
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        f32x4 sum = {};
+        if (real)
+            for (int i = 0; i < a.parts; ++i)
+                sum += *reinterpret_cast<const f32x4*>(a.partial + (((static_cast<int64_t>(i) * 2 + which) * kv_heads + head) * a.rows + row) * a.width + column);
+        const Tensor& to = which ? a.dv : a.dk;
+        Type<T>::store4(const_cast<T*>(reinterpret_cast<const T*>(to.p)) + sequence * to.batch + token * to.token + head * to.head + column, sum[0], sum[1],
+                        sum[2], sum[3]);
+    }
+}
+
 // ---- host -----------------------------------------------------------------------------------------------------------------
 // Tile rows and waves per SIMD of each kernel.
 template <class T, int DP>
 struct Shape {
     static constexpr bool TWO = sizeof(T) == 2, VL = TWO && DP > 96;
     static constexpr int KEYS = TWO ? 64 : 32, QUERIES = TWO && DP <= 96 ? 64 : 32, WAVES = TWO ? 2 : 1;
-    static constexpr int KEY_LDS = 4 * KEYS * Image<T, DP>::ROW_BYTES;
-    static constexpr int QUERY_LDS = 4 * QUERIES * Image<T, DP>::ROW_BYTES + 4 * QUERIES * 4 + (VL ? ROWS * Image<T, DP>::ROW_BYTES : 0);
+    static constexpr int KEY_LDS = 4 * Image<T, DP, KEYS>::BYTES;
+    static constexpr int QUERY_LDS = 4 * Image<T, DP, QUERIES>::BYTES + 4 * QUERIES * 4 + (VL ? Image<T, DP, ROWS>::BYTES : 0);
     static constexpr auto forward = &attention_forward_kernel<T, DP, KEYS, WAVES>;
     static constexpr auto dq = &attention_dq_kernel<T, DP, KEYS, WAVES>;
     static constexpr auto dkv = &attention_dkv_kernel<T, DP, QUERIES, VL, WAVES>;
@@ -714,7 +737,11 @@ int launch_width(Args& a, bool backward, hipStream_t stream) {
         S::forward<<<items, THREADS, S::KEY_LDS, stream>>>(a);
     } else {
         S::dq<<<items, THREADS, S::KEY_LDS, stream>>>(a);
-        S::dkv<<<static_cast<unsigned>(slots), THREADS, S::QUERY_LDS, stream>>>(a);
+        S::dkv<<<static_cast<unsigned>(slots * a.parts), THREADS, S::QUERY_LDS, stream>>>(a);
+        if (a.parts > 1) {
+            const int64_t threads = a.rows * (a.heads / a.group) * (a.width / 4);
+            attention_join_kernel<T><<<static_cast<unsigned>((threads + THREADS - 1) / THREADS), THREADS, 0, stream>>>(a);
+        }
     }
     return hipGetLastError() == hipSuccess ? KF_OK : KF_ERR_LAUNCH_FAILED;
 }
@@ -725,6 +752,25 @@ int launch_type(Args& a, bool backward, hipStream_t stream) {
     if (a.width <= 64) return launch_width<T, 64>(a, backward, stream);
     if (a.width <= 96) return launch_width<T, 96>(a, backward, stream);
     return launch_width<T, 128>(a, backward, stream);
+}
+
+int64_t tile_slots(int64_t sequences, int64_t length, int64_t rows, bool packed) {
+    return packed ? rows / ROWS + sequences + 1 : sequences * ((length + ROWS - 1) / ROWS);
+}
+
+constexpr int64_t MAX_PARTS = 4;
+
+int64_t delta_bytes(int64_t rows, int64_t heads) { return (rows * heads * 4 + 15) / 16 * 16; }
+
+// How many workgroups share the queries of one key tile in the dk / dv kernel.  512 workgroups of it fit the card at a time, and
+// the first tile of a causal sequence has twice the mean work: with all of them resident at once the kernel takes as long as its
+// largest item.  Measured (32/8 heads x 128): one document of 8192 tokens, 512 items: 2064 us whole, 1233 + 27 us (join) in two parts,
+// 1218 + 58 in four; 24 documents of 12011 tokens in all, 16/4 heads, 472 items: 467 us whole, 294 + 21 in two, 218 + 36 in four;
+// 16 x 512 tokens, 512 items of equal cost at four steps a head: 173 us whole, 182 + 29 in two.
+int64_t dkv_parts(int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, bool packed, bool causal) {
+    const int64_t items = tile_slots(sequences, length, rows, packed) * kv_heads, steps = ((packed ? rows : length) + 31) / 32 * (heads / kv_heads);
+    const int64_t wanted = ((packed ? 2048 : causal ? 1024 : 512) + items - 1) / items;
+    return std::max<int64_t>(1, std::min(std::min(wanted, MAX_PARTS), steps / 128));
 }
 
 Tensor tensor_of(const kf_heads_view* v) { return Tensor{v->p, v->batch_stride, v->token_stride, v->head_stride}; }
@@ -744,10 +790,10 @@ int fill(Args& a, int dtype, int64_t sequences, int64_t length, int64_t rows, in
         width % per != 0 || !(scale > 0.0f) || !isfinite(scale))
         return KF_ERR_INVALID_ARGUMENT;
     if (offsets ? lengths != nullptr : (length <= 0 || sequences > limit / length || rows != sequences * length)) return KF_ERR_INVALID_ARGUMENT;
-    const int64_t slots = offsets ? rows / ROWS + sequences + 1 : sequences * ((length + ROWS - 1) / ROWS);
+    const int64_t slots = tile_slots(sequences, length, rows, offsets != nullptr);
     const int64_t tiles = offsets ? 0 : slots / sequences, groups = offsets ? 0 : sequences * kv_heads;
     const int64_t chunk = groups >= 64 ? tiles : 1;
-    if (sequences >= limit || slots > (limit - XCDS * chunk * heads) / heads) return KF_ERR_INVALID_ARGUMENT;
+    if (sequences >= limit || slots > (limit / MAX_PARTS - XCDS * chunk * heads) / heads) return KF_ERR_INVALID_ARGUMENT;
     a.chunk = static_cast<int>(chunk);
     a.lengths = lengths;
     a.offsets = offsets;
@@ -781,7 +827,12 @@ int kf_attention_forward(const kf_heads_view* out, float* lse, const kf_heads_vi
     return dtype == KF_BF16 ? launch_type<__bf16>(a, false, on) : launch_type<float>(a, false, on);
 }
 
-int64_t kf_attention_backward_workspace_bytes(int64_t rows, int64_t heads) { return rows > 0 && heads > 0 ? rows * heads * 4 : 0; }
+int64_t kf_attention_backward_workspace_bytes(int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width, int packed,
+                                              int causal) {
+    if (sequences <= 0 || rows <= 0 || heads <= 0 || kv_heads <= 0 || width <= 0 || (!packed && length <= 0)) return 0;
+    const int64_t parts = dkv_parts(sequences, length, rows, heads, kv_heads, packed, causal);
+    return delta_bytes(rows, heads) + (parts > 1 ? parts * 2 * kv_heads * rows * width * 4 : 0);
+}
 
 int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, const kf_heads_view* dv, const kf_heads_view* grad, const kf_heads_view* out,
                           const float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v, int dtype, int64_t sequences,
@@ -794,12 +845,16 @@ int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, cons
     for (const kf_heads_view* t : all)
         if (!usable(t, per, width)) return KF_ERR_INVALID_ARGUMENT;
     if (lse == nullptr) return KF_ERR_INVALID_ARGUMENT;
-    if (workspace == nullptr || workspace_bytes < kf_attention_backward_workspace_bytes(rows, heads)) return KF_ERR_WORKSPACE_TOO_SMALL;
+    if (workspace == nullptr ||
+        workspace_bytes < kf_attention_backward_workspace_bytes(sequences, length, rows, heads, kv_heads, width, offsets != nullptr, causal))
+        return KF_ERR_WORKSPACE_TOO_SMALL;
     if (int s = configure_kernels()) return s;
     a.q = tensor_of(q); a.k = tensor_of(k); a.v = tensor_of(v); a.o = tensor_of(out); a.g = tensor_of(grad);
     a.dq = tensor_of(dq); a.dk = tensor_of(dk); a.dv = tensor_of(dv);
     a.lse = const_cast<float*>(lse);
     a.delta = reinterpret_cast<float*>(workspace);
+    a.partial = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + delta_bytes(rows, heads));
+    a.parts = static_cast<int>(dkv_parts(sequences, length, rows, heads, kv_heads, offsets != nullptr, causal));
     const hipStream_t on = reinterpret_cast<hipStream_t>(stream);
     return dtype == KF_BF16 ? launch_type<__bf16>(a, true, on) : launch_type<float>(a, true, on);
 }

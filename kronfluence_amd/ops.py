@@ -1111,7 +1111,7 @@ def attention_backward(grad: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
     grad, out, q, k, v = (_heads_operand(t) for t in (grad, out, q, k, v))
     lengths, offsets = _row_counts(lengths, length), _row_counts(cu_seqlens, rows)
     library = nat.lib()
-    ws_bytes = library.kf_attention_backward_workspace_bytes(rows, heads)
+    ws_bytes = library.kf_attention_backward_workspace_bytes(sequences, length, rows, heads, kv_heads, width, int(offsets is not None), int(causal))
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
     with _on_device_of(q):
         nat.check(

@@ -126,7 +126,7 @@ def test_c_entries_refuse_without_touching_memory():
         views = [kw.pop("dq", ok)] + [ok] * 4
         return lib.kf_attention_backward(*views, lse, ok, ok, ok, nat.KF_BF16, 1, 4, kw.get("rows", 4), 2, 2, 64, None, None, 1, 1.0, workspace, bytes_, None)
 
-    assert lib.kf_attention_backward_workspace_bytes(4, 2) == 4 * 2 * 4
+    assert lib.kf_attention_backward_workspace_bytes(1, 4, 4, 2, 2, 64, 0, 1) == 4 * 2 * 4
     assert backward(bytes_=31) == WORKSPACE and backward(workspace=None) == WORKSPACE
     assert backward(lse=None) == INVALID and backward(dq=view(pointer=4)) == INVALID and backward(rows=3) == INVALID
 
