@@ -282,7 +282,11 @@ __device__ __forceinline__ Rows input_rows(const Args& a, const Tensor& t, const
 template <class T>
 __device__ __forceinline__ T* rows_out(const Tensor& t, const Place& w, int head) { return const_cast<T*>(rows_of<T>(t, w, head)); }
 
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+// the value of lane ^ 32
+__device__ __forceinline__ float other_half(float x) {
+    const auto swapped = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(threadIdx.x & 32 ? swapped[0] : swapped[1]);
+}
 
 // The fragments of 32 rows straight from memory (lane & 31 = row): the operand a wave keeps for the whole kernel.
 template <class T, int DP>
@@ -325,6 +329,18 @@ __device__ __forceinline__ void zero_rows(T* base, int64_t token, int row0, int 
     for (int n = tid; n < ROWS * chunks; n += N_THREADS) {
         const int row = row0 + n / chunks;
         if (row < written) *reinterpret_cast<u32x4*>(base + row * token + (n % chunks) * PER) = u32x4{0, 0, 0, 0};
+    }
+}
+
+// A read of a matrix instruction's result needs wait states that the compiler inserts; where a branch stands between the two it has
+// left them out on one of the paths (fp32: 16-pass instructions, the first read behind the branch saw row 15 of the tile before it
+// was written).  Put between the last matrix instruction and such a branch.  tests/test_wait_states_cpu.py follows every path of the built code.
+template <class T>
+__device__ __forceinline__ void settle() {
+    if constexpr (sizeof(T) == 4) {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_nop 15\n\ts_nop 3");
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -380,6 +396,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
 #pragma unroll
                 for (int i = 0; i < Img::SLABS; ++i) s[b] = Type<T>::mma(read.rows(kt, 32 * b, i), q.f[i], s[b]);
             }
+            settle<T>();
             if (k0 + BK > w.length || (a.causal && k0 + BK - 1 > first)) {
                 const int visible = a.causal ? min(w.length, query + 1) : w.length;
 #pragma unroll
@@ -420,6 +437,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
                 }
             }
         }
+        settle<T>();
         if (t + 1 < tiles) {
             sk.store(lds + ((t + 1) & 1) * 2 * TILE);
             sv.store(lds + ((t + 1) & 1) * 2 * TILE + TILE);
@@ -497,6 +515,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
                 for (int i = 0; i < Img::SLABS; ++i) dp = Type<T>::mma(read.rows(vt, 32 * b, i), g.f[i], dp);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
+                settle<T>();
                 if (masked) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
@@ -510,6 +529,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
                 }
             }
         }
+        settle<T>();
         if (t + 1 < tiles) {
             sk.store(lds + ((t + 1) & 1) * 2 * TILE);
             sv.store(lds + ((t + 1) & 1) * 2 * TILE + TILE);
@@ -611,6 +631,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
 #pragma unroll
         for (int b = 0; b < BQ / 32; ++b) {
             if (a.causal && q0 + 32 * b + 32 <= first) continue;   // (wave-uniform)
+            // s; then dp beside p = 2^(c s - L); then dv beside ds = p (dp - D); then dk
             f32x16 s = {}, dp = {};
 #pragma unroll
             for (int i = 0; i < Img::SLABS; ++i) s = Type<T>::mma(read.rows(qt, 32 * b, i), k.f[i], s);
@@ -619,35 +640,43 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
                 if constexpr (VL) dp = Type<T>::mma(read.rows(gt, 32 * b, i), read_v.rows(own_v, 0, i), dp);
                 else dp = Type<T>::mma(read.rows(gt, 32 * b, i), v.f[i], dp);
             }
+            const float* rows_lse = lse + 32 * b + 4 * half;
+            const float* rows_delta = delta + 32 * b + 4 * half;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + 32 * b + 8 * i + 4 * half);
-                const f32x4 d4 = *reinterpret_cast<const f32x4*>(delta + 32 * b + 8 * i + 4 * half);
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(rows_lse + 8 * i);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = 4 * i + j;
-                    s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -l4[j]));
-                    dp[r] = s[r] * (dp[r] - d4[j]);
-                }
+                for (int j = 0; j < 4; ++j) s[4 * i + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * i + j], c, -l4[j]));
             }
+            settle<T>();
             if ((a.causal && q0 + 32 * b < first + 31) || w.length == 1) {
+                const int hidden = a.causal ? key - q0 - 32 * b - 4 * half : -32;   // rows of the block in front of the key
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int query = q0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4;
-                    const bool seen = !a.causal || query >= key, lone = a.causal ? query == 0 : true;
-                    if (!seen) s[r] = 0.0f;
-                    if (!seen || lone) dp[r] = 0.0f;   // a row that sees one key: ds is exactly 0
-                }
+                for (int r = 0; r < 16; ++r)
+                    if (8 * (r / 4) + r % 4 < hidden) s[r] = 0.0f;
+                // the first row of a causal sequence, or the only one, sees one key: ds is exactly 0
+                if (q0 + 32 * b + 4 * half == 0) dp[0] = rows_delta[0];
             }
 #pragma unroll
             for (int i = 0; i < SECOND; ++i) {
-                const Frag p = Type<T>::from_acc(s, i), ds = Type<T>::from_acc(dp, i);
+                const Frag p = Type<T>::from_acc(s, i);
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) av[d] = Type<T>::mma(read.columns(gt, 32 * b, i, d), p, av[d]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(rows_delta + 8 * i);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) dp[4 * i + j] = s[4 * i + j] * (dp[4 * i + j] - d4[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < SECOND; ++i) {
+                const Frag ds = Type<T>::from_acc(dp, i);
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) ak[d] = Type<T>::mma(read.columns(qt, 32 * b, i, d), ds, ak[d]);
             }
         }
+        settle<T>();
         if (n + 1 < steps) store(lds + ((n + 1) & 1) * STAGE);
     }
     if (a.parts > 1) {   // (w.stat + key: the token's row among all)
@@ -699,7 +728,7 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(const Args a) {
 template <class T, int DP>
 struct Shape {
     static constexpr bool TWO = sizeof(T) == 2, VL = TWO && DP > 96;
-    static constexpr int KEYS = TWO ? 64 : 32, QUERIES = TWO && DP <= 96 ? 64 : 32, WAVES = TWO ? 2 : 1;
+    static constexpr int KEYS = TWO ? 64 : 32, QUERIES = TWO && DP <= 64 ? 64 : 32, WAVES = TWO ? 2 : 1;
     static constexpr int KEY_LDS = 4 * Image<T, DP, KEYS>::BYTES;
     static constexpr int QUERY_LDS = 4 * Image<T, DP, QUERIES>::BYTES + 4 * QUERIES * 4 + (VL ? Image<T, DP, ROWS>::BYTES : 0);
     static constexpr auto forward = &attention_forward_kernel<T, DP, KEYS, WAVES>;

@@ -13,42 +13,53 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/kronfluence_hip.h"
 
 namespace {
 
 constexpr int THREADS = 256, WIDE_THREADS = 512;
-constexpr int VEC = 8;                       // columns per chunk
-constexpr int WAVE_MAX = 64 * VEC * 4;       // columns a wave holds in registers
-constexpr int WIDE_MAX = WIDE_THREADS * VEC * 4;
+constexpr int WAVE_MAX = 2048, WIDE_MAX = 16384;   // columns a wave / a workgroup of WIDE_THREADS holds in registers (32 per lane)
+
+// Columns per chunk: 16 bytes of the wider of the two types a kernel streams, so that every wave access to it is 1 KB without gaps
+// (with 8 fp32 columns per lane a store instruction wrote every second 16 bytes: 131072 x 768 bf16 -> fp32 166 us).
+template <class A, class B>
+constexpr int vec_of() { return 16 / static_cast<int>(sizeof(A) > sizeof(B) ? sizeof(A) : sizeof(B)); }
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int launch_status() { return hipGetLastError() == hipSuccess ? KF_OK : KF_ERR_LAUNCH_FAILED; }
 
-// Eight consecutive elements at any element-aligned address (rows of odd widths start anywhere).
-template <class T>
+// VEC consecutive elements at any element-aligned address (rows of odd widths start anywhere).
+template <class T, int VEC>
 struct __attribute__((packed, aligned(sizeof(T)))) Chunk { T v[VEC]; };
 
-template <class T>
-__device__ __forceinline__ void load8(float (&x)[VEC], const T* p, int64_t column, int64_t width) {
+template <int VEC, class T>
+__device__ __forceinline__ Chunk<T, VEC> load_chunk(const T* p, int64_t column, int64_t width) {
+    Chunk<T, VEC> c;
     if (column + VEC <= width) {
-        const Chunk<T> c = *reinterpret_cast<const Chunk<T>*>(p + column);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) x[i] = static_cast<float>(c.v[i]);
+        c = *reinterpret_cast<const Chunk<T, VEC>*>(p + column);
     } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) x[i] = column + i < width ? static_cast<float>(p[column + i]) : 0.0f;
+        for (int i = 0; i < VEC; ++i) c.v[i] = column + i < width ? p[column + i] : static_cast<T>(0.0f);
     }
+    return c;
 }
+template <int VEC, class T>
+__device__ __forceinline__ void widen(float (&x)[VEC], const Chunk<T, VEC>& c) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) x[i] = static_cast<float>(c.v[i]);
+}
+template <int VEC, class T>
+__device__ __forceinline__ void load(float (&x)[VEC], const T* p, int64_t column, int64_t width) { widen(x, load_chunk<VEC>(p, column, width)); }
 
-template <class T>
-__device__ __forceinline__ void store8(T* p, int64_t column, int64_t width, const float (&x)[VEC]) {
+template <int VEC, class T>
+__device__ __forceinline__ void store(T* p, int64_t column, int64_t width, const float (&x)[VEC]) {
     if (column + VEC <= width) {
-        Chunk<T> c;
+        Chunk<T, VEC> c;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) c.v[i] = static_cast<T>(x[i]);
-        *reinterpret_cast<Chunk<T>*>(p + column) = c;
+        *reinterpret_cast<Chunk<T, VEC>*>(p + column) = c;
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
@@ -56,11 +67,12 @@ __device__ __forceinline__ void store8(T* p, int64_t column, int64_t width, cons
     }
 }
 
-// eight elements of a vector whose type is known at run time only (weight, bias: read once per workgroup)
-__device__ __forceinline__ void load8_as(float (&x)[VEC], const void* p, int dtype, int64_t column, int64_t width) {
-    if (dtype == KF_F32) load8(x, reinterpret_cast<const float*>(p), column, width);
-    else if (dtype == KF_BF16) load8(x, reinterpret_cast<const __bf16*>(p), column, width);
-    else load8(x, reinterpret_cast<const _Float16*>(p), column, width);
+// elements of a vector whose type is known at run time only (weight, bias: read once per workgroup)
+template <int VEC>
+__device__ __forceinline__ void load_as(float (&x)[VEC], const void* p, int dtype, int64_t column, int64_t width) {
+    if (dtype == KF_F32) load(x, reinterpret_cast<const float*>(p), column, width);
+    else if (dtype == KF_BF16) load(x, reinterpret_cast<const __bf16*>(p), column, width);
+    else load(x, reinterpret_cast<const _Float16*>(p), column, width);
 }
 
 __device__ __forceinline__ float wave_sum(float x) {
@@ -111,7 +123,7 @@ struct ForwardArgs {
 // LANES lanes per row, NV chunks per lane: width <= LANES * NV * VEC.  The weights stay in registers for the workgroup's rows.
 template <class X, class Y, int LANES, int NV>
 __global__ __launch_bounds__(LANES > 64 ? LANES : THREADS) void norm_forward_kernel(const ForwardArgs a) {
-    constexpr int BLOCK = LANES > 64 ? LANES : THREADS, GROUPS = BLOCK / LANES;
+    constexpr int BLOCK = LANES > 64 ? LANES : THREADS, GROUPS = BLOCK / LANES, VEC = vec_of<X, Y>();
     __shared__ float scratch[16];
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
     const float inv = 1.0f / static_cast<float>(a.width);
@@ -121,14 +133,23 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : THREADS) void norm_forward_ker
         const int64_t c = (lane + j * LANES) * VEC;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) { w[j][i] = 1.0f; b[j][i] = 0.0f; }
-        if (a.weight) load8_as(w[j], a.weight, a.w_dtype, c, a.width);
-        if (a.bias) load8_as(b[j], a.bias, a.w_dtype, c, a.width);
+        if (a.weight) load_as(w[j], a.weight, a.w_dtype, c, a.width);
+        if (a.bias) load_as(b[j], a.bias, a.w_dtype, c, a.width);
     }
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group; row < a.rows; row += static_cast<int64_t>(gridDim.x) * GROUPS) {
-        const X* x = reinterpret_cast<const X*>(a.x) + row * a.ld;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * GROUPS;
+    int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group;
+    Chunk<X, VEC> next[NV];   // the next row is on its way while this one is worked on
+    auto fetch = [&](int64_t at) {
+        const X* x = reinterpret_cast<const X*>(a.x) + at * a.ld;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) next[j] = load_chunk<VEC>(x, (lane + j * LANES) * VEC, a.width);
+    };
+    if (row < a.rows) fetch(row);
+    for (; row < a.rows; row += step) {
         float v[NV][VEC];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) load8(v[j], x, (lane + j * LANES) * VEC, a.width);
+        for (int j = 0; j < NV; ++j) widen(v[j], next[j]);
+        if (row + step < a.rows) fetch(row + step);
         float mu = 0.0f;
         if (a.centred) {
 #pragma unroll
@@ -153,7 +174,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : THREADS) void norm_forward_ker
 #pragma unroll
             for (int i = 0; i < VEC; ++i) out[i] = fmaf(v[j][i] * r, w[j][i], b[j][i]);
             const int64_t c = (lane + j * LANES) * VEC;
-            if (c < a.width) store8(y, c, a.width, out);
+            if (c < a.width) store(y, c, a.width, out);
         }
         if (a.stats && lane == 0) { a.stats[2 * row] = mu; a.stats[2 * row + 1] = r; }
     }
@@ -162,6 +183,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : THREADS) void norm_forward_ker
 // Rows wider than the registers: the row is read three times (from memory once, then from the cache).
 template <class X, class Y>
 __global__ __launch_bounds__(WIDE_THREADS) void norm_forward_long_kernel(const ForwardArgs a) {
+    constexpr int VEC = vec_of<X, Y>();
     __shared__ float scratch[16];
     const float inv = 1.0f / static_cast<float>(a.width);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -169,14 +191,14 @@ __global__ __launch_bounds__(WIDE_THREADS) void norm_forward_long_kernel(const F
         float mu = 0.0f, ss = 0.0f, v[VEC], w[VEC], b[VEC];
         if (a.centred) {
             for (int64_t c = threadIdx.x * VEC; c < a.width; c += WIDE_THREADS * VEC) {
-                load8(v, x, c, a.width);
+                load(v, x, c, a.width);
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) mu += v[i];
             }
             mu = group_sum<WIDE_THREADS>(mu, scratch) * inv;
         }
         for (int64_t c = threadIdx.x * VEC; c < a.width; c += WIDE_THREADS * VEC) {
-            load8(v, x, c, a.width);
+            load(v, x, c, a.width);
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
                 if (c + i < a.width) ss = fmaf(v[i] - mu, v[i] - mu, ss);
@@ -186,12 +208,12 @@ __global__ __launch_bounds__(WIDE_THREADS) void norm_forward_long_kernel(const F
         for (int64_t c = threadIdx.x * VEC; c < a.width; c += WIDE_THREADS * VEC) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) { w[i] = 1.0f; b[i] = 0.0f; }
-            if (a.weight) load8_as(w, a.weight, a.w_dtype, c, a.width);
-            if (a.bias) load8_as(b, a.bias, a.w_dtype, c, a.width);
-            load8(v, x, c, a.width);
+            if (a.weight) load_as(w, a.weight, a.w_dtype, c, a.width);
+            if (a.bias) load_as(b, a.bias, a.w_dtype, c, a.width);
+            load(v, x, c, a.width);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) v[i] = fmaf((v[i] - mu) * r, w[i], b[i]);
-            store8(y, c, a.width, v);
+            store(y, c, a.width, v);
         }
         if (a.stats && threadIdx.x == 0) { a.stats[2 * row] = mu; a.stats[2 * row + 1] = r; }
     }
@@ -209,7 +231,7 @@ struct BackwardArgs {
 // As the forward kernel; every group adds up the columns of its rows for dw and db beside writing dx.
 template <class X, class G, int LANES, int NV>
 __global__ __launch_bounds__(LANES > 64 ? LANES : THREADS) void norm_backward_kernel(const BackwardArgs a) {
-    constexpr int BLOCK = LANES > 64 ? LANES : THREADS, GROUPS = BLOCK / LANES, COLUMNS = LANES * NV * VEC;
+    constexpr int VEC = vec_of<X, G>(), BLOCK = LANES > 64 ? LANES : THREADS, GROUPS = BLOCK / LANES, COLUMNS = LANES * NV * VEC;
     __shared__ float scratch[16];
     __shared__ float joined[GROUPS > 1 ? COLUMNS : 1];
     const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
@@ -219,7 +241,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : THREADS) void norm_backward_ke
     for (int j = 0; j < NV; ++j) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) { w[j][i] = 1.0f; dw[j][i] = 0.0f; db[j][i] = 0.0f; }
-        if (a.weight) load8_as(w[j], a.weight, a.w_dtype, (lane + j * LANES) * VEC, a.width);
+        if (a.weight) load_as(w[j], a.weight, a.w_dtype, (lane + j * LANES) * VEC, a.width);
     }
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * GROUPS + group; row < a.rows; row += static_cast<int64_t>(gridDim.x) * GROUPS) {
         const X* x = reinterpret_cast<const X*>(a.x) + row * a.ld;
@@ -229,8 +251,8 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : THREADS) void norm_backward_ke
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int64_t c = (lane + j * LANES) * VEC;
-            load8(h[j], x, c, a.width);
-            load8(u[j], g, c, a.width);
+            load(h[j], x, c, a.width);
+            load(u[j], g, c, a.width);
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j)
@@ -254,7 +276,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : THREADS) void norm_backward_ke
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) out[i] = r * (u[j][i] - mean_u - h[j][i] * mean_uh);
                 const int64_t c = (lane + j * LANES) * VEC;
-                if (c < a.width) store8(dx, c, a.width, out);
+                if (c < a.width) store(dx, c, a.width, out);
             }
         }
     }
@@ -282,7 +304,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : THREADS) void norm_backward_ke
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int64_t c = (lane + j * LANES) * VEC;
-                if (c < a.width) store8(out + part * a.width, c, a.width, part ? db[j] : dw[j]);
+                if (c < a.width) store(out + part * a.width, c, a.width, part ? db[j] : dw[j]);
             }
         }
     }
@@ -292,6 +314,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : THREADS) void norm_backward_ke
 // reads and writes.
 template <class X, class G>
 __global__ __launch_bounds__(WIDE_THREADS) void norm_backward_long_kernel(const BackwardArgs a) {
+    constexpr int VEC = vec_of<X, G>();
     __shared__ float scratch[16];
     const float inv = 1.0f / static_cast<float>(a.width);
     float* dw = a.partial ? a.partial + static_cast<int64_t>(blockIdx.x) * (a.with_bias ? 2 : 1) * a.width : nullptr;
@@ -303,11 +326,11 @@ __global__ __launch_bounds__(WIDE_THREADS) void norm_backward_long_kernel(const 
         const float mu = a.stats[2 * row], r = a.stats[2 * row + 1];
         float mean_u = 0.0f, mean_uh = 0.0f, h[VEC], u[VEC], w[VEC];
         for (int64_t c = threadIdx.x * VEC; c < a.width; c += WIDE_THREADS * VEC) {
-            load8(h, x, c, a.width);
-            load8(u, g, c, a.width);
+            load(h, x, c, a.width);
+            load(u, g, c, a.width);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) w[i] = 1.0f;
-            if (a.weight) load8_as(w, a.weight, a.w_dtype, c, a.width);
+            if (a.weight) load_as(w, a.weight, a.w_dtype, c, a.width);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 h[i] = (h[i] - mu) * r;
@@ -326,14 +349,14 @@ __global__ __launch_bounds__(WIDE_THREADS) void norm_backward_long_kernel(const 
         mean_uh *= inv;
         X* dx = reinterpret_cast<X*>(a.dx) + row * a.width;
         for (int64_t c = threadIdx.x * VEC; c < a.width; c += WIDE_THREADS * VEC) {
-            load8(h, x, c, a.width);
-            load8(u, g, c, a.width);
+            load(h, x, c, a.width);
+            load(u, g, c, a.width);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) w[i] = 1.0f;
-            if (a.weight) load8_as(w, a.weight, a.w_dtype, c, a.width);
+            if (a.weight) load_as(w, a.weight, a.w_dtype, c, a.width);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) h[i] = r * (u[i] * w[i] - mean_u - (h[i] - mu) * r * mean_uh);
-            store8(dx, c, a.width, h);
+            store(dx, c, a.width, h);
         }
     }
 }
@@ -373,29 +396,46 @@ __global__ __launch_bounds__(64 * STRANDS) void norm_reduce_kernel(const float* 
 int64_t forward_groups(int64_t rows, int64_t width) { return std::min<int64_t>(width <= WAVE_MAX ? cdiv(rows, 4) : rows, 2048); }
 int64_t backward_groups(int64_t rows, int64_t width) { return std::min<int64_t>(width <= WAVE_MAX ? cdiv(rows, 4) : rows, width <= WAVE_MAX ? 1024 : 512); }
 
+// f(LANES, NV) with the smallest group that holds a row of `width` columns in registers; LANES 0: none does
+template <int VEC, class F>
+void with_group(int64_t width, F f) {
+    using std::integral_constant;
+    const int64_t wave = cdiv(width, 64 * VEC), wide = cdiv(width, WIDE_THREADS * VEC);
+    constexpr integral_constant<int, 64> one;
+    constexpr integral_constant<int, WIDE_THREADS> eight;
+    if (width > WIDE_MAX) return f(integral_constant<int, 0>(), integral_constant<int, 0>());
+    if (width > WAVE_MAX) {
+        if (wide == 1) return f(eight, integral_constant<int, 1>());
+        if (wide == 2) return f(eight, integral_constant<int, 2>());
+        if (wide <= 4) return f(eight, integral_constant<int, 4>());
+        if constexpr (VEC < 8) return f(eight, integral_constant<int, 8>());
+    }
+    if (wave == 1) return f(one, integral_constant<int, 1>());
+    if (wave == 2) return f(one, integral_constant<int, 2>());
+    if constexpr (VEC < 8) {
+        if (wave == 3) return f(one, integral_constant<int, 3>());
+        if (wave > 4) return f(one, integral_constant<int, 8>());
+    }
+    f(one, integral_constant<int, 4>());
+}
+
 template <class X, class Y>
 int forward_as(const ForwardArgs& a, hipStream_t stream) {
     const unsigned grid = static_cast<unsigned>(forward_groups(a.rows, a.width));
-    if (a.width <= 64 * VEC) norm_forward_kernel<X, Y, 64, 1><<<grid, THREADS, 0, stream>>>(a);
-    else if (a.width <= 64 * VEC * 2) norm_forward_kernel<X, Y, 64, 2><<<grid, THREADS, 0, stream>>>(a);
-    else if (a.width <= WAVE_MAX) norm_forward_kernel<X, Y, 64, 4><<<grid, THREADS, 0, stream>>>(a);
-    else if (a.width <= WIDE_THREADS * VEC) norm_forward_kernel<X, Y, WIDE_THREADS, 1><<<grid, WIDE_THREADS, 0, stream>>>(a);
-    else if (a.width <= WIDE_THREADS * VEC * 2) norm_forward_kernel<X, Y, WIDE_THREADS, 2><<<grid, WIDE_THREADS, 0, stream>>>(a);
-    else if (a.width <= WIDE_MAX) norm_forward_kernel<X, Y, WIDE_THREADS, 4><<<grid, WIDE_THREADS, 0, stream>>>(a);
-    else norm_forward_long_kernel<X, Y><<<grid, WIDE_THREADS, 0, stream>>>(a);
+    with_group<vec_of<X, Y>()>(a.width, [&](auto lanes, auto nv) {
+        if constexpr (lanes == 0) norm_forward_long_kernel<X, Y><<<grid, WIDE_THREADS, 0, stream>>>(a);
+        else norm_forward_kernel<X, Y, lanes, nv><<<grid, lanes > 64 ? WIDE_THREADS : THREADS, 0, stream>>>(a);
+    });
     return launch_status();
 }
 
 template <class X, class G>
 int backward_as(const BackwardArgs& a, hipStream_t stream) {
     const unsigned grid = static_cast<unsigned>(backward_groups(a.rows, a.width));
-    if (a.width <= 64 * VEC) norm_backward_kernel<X, G, 64, 1><<<grid, THREADS, 0, stream>>>(a);
-    else if (a.width <= 64 * VEC * 2) norm_backward_kernel<X, G, 64, 2><<<grid, THREADS, 0, stream>>>(a);
-    else if (a.width <= WAVE_MAX) norm_backward_kernel<X, G, 64, 4><<<grid, THREADS, 0, stream>>>(a);
-    else if (a.width <= WIDE_THREADS * VEC) norm_backward_kernel<X, G, WIDE_THREADS, 1><<<grid, WIDE_THREADS, 0, stream>>>(a);
-    else if (a.width <= WIDE_THREADS * VEC * 2) norm_backward_kernel<X, G, WIDE_THREADS, 2><<<grid, WIDE_THREADS, 0, stream>>>(a);
-    else if (a.width <= WIDE_MAX) norm_backward_kernel<X, G, WIDE_THREADS, 4><<<grid, WIDE_THREADS, 0, stream>>>(a);
-    else norm_backward_long_kernel<X, G><<<grid, WIDE_THREADS, 0, stream>>>(a);
+    with_group<vec_of<X, G>()>(a.width, [&](auto lanes, auto nv) {
+        if constexpr (lanes == 0) norm_backward_long_kernel<X, G><<<grid, WIDE_THREADS, 0, stream>>>(a);
+        else norm_backward_kernel<X, G, lanes, nv><<<grid, lanes > 64 ? WIDE_THREADS : THREADS, 0, stream>>>(a);
+    });
     return launch_status();
 }
 

@@ -1017,6 +1017,11 @@ def _on_device_of(t: torch.Tensor):
     return _NO_GUARD if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of ``t``'s shape, dtype and device."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _heads_operand(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself if the kernels can read it in place (``[..., heads, width]``: contiguous width, 16-byte aligned start and
     strides), else a contiguous copy."""
@@ -1080,8 +1085,8 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal:
     """``softmax(scale q k^T + mask) v`` over whole prompts (kf_attention_forward): the output and, for the backward call, the fp32
     ``[heads, token rows]`` log-sum of every row."""
     sequences, length, rows, heads, kv_heads, width = _attention_shape(q, k, v, lengths, cu_seqlens, scale)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((heads, rows), dtype=torch.float32, device=q.device) if with_lse else None
+    out = _like(q)
+    lse = q.new_empty((heads, rows), dtype=torch.float32) if with_lse else None
     if sequences == 0 or rows == 0:
         return out.zero_(), lse
     q, k, v = _heads_operand(q), _heads_operand(k), _heads_operand(v)
@@ -1104,15 +1109,14 @@ def attention_backward(grad: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
     _require(grad.shape == out.shape == q.shape and grad.dtype == out.dtype == q.dtype and grad.device == out.device == q.device,
              "grad and out have the shape, dtype and device of q")
     _require(lse.dtype == torch.float32 and lse.is_contiguous() and lse.shape == (heads, rows), "lse is what the forward call returned")
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk, dv = torch.empty(k.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    dq, dk, dv = _like(q), _like(k), _like(v)
     if sequences == 0 or rows == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     grad, out, q, k, v = (_heads_operand(t) for t in (grad, out, q, k, v))
     lengths, offsets = _row_counts(lengths, length), _row_counts(cu_seqlens, rows)
     library = nat.lib()
     ws_bytes = library.kf_attention_backward_workspace_bytes(sequences, length, rows, heads, kv_heads, width, int(offsets is not None), int(causal))
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    ws = q.new_empty(ws_bytes, dtype=torch.uint8)
     with _on_device_of(q):
         nat.check(
             library.kf_attention_backward(_heads_view(dq), _heads_view(dk), _heads_view(dv), _heads_view(grad), _heads_view(out),
@@ -1158,8 +1162,8 @@ def norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional
     _require(math.isfinite(eps) and eps >= 0, "eps is finite and not negative")
     width = x.shape[-1]
     rows = x.numel() // width
-    out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=x.device) if with_stats else None
+    out = _like(x) if out_dtype == x.dtype else x.new_empty(x.shape, dtype=out_dtype)
+    stats = x.new_empty((rows, 2), dtype=torch.float32) if with_stats else None
     if rows == 0:
         return out, stats
     x, stride = _norm_rows(x)
@@ -1188,9 +1192,9 @@ def norm_backward(grad: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weig
     _require(stats.dtype == torch.float32 and stats.is_contiguous() and stats.shape == (rows, 2), "stats is what the forward call returned")
     dtype = weight_dtype if weight_dtype is not None else bias_dtype
     _require(bias_dtype in (None, dtype) and (weight is None or dtype in (None, weight.dtype)), "weight and bias share one dtype")
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if with_input else None
-    dweight = None if weight_dtype is None else torch.empty(width, dtype=dtype, device=x.device)
-    dbias = None if bias_dtype is None else torch.empty(width, dtype=dtype, device=x.device)
+    dx = _like(x) if with_input else None
+    dweight = None if weight_dtype is None else x.new_empty(width, dtype=dtype)
+    dbias = None if bias_dtype is None else x.new_empty(width, dtype=dtype)
     if rows == 0:
         return dx, None if dweight is None else dweight.zero_(), None if dbias is None else dbias.zero_()
     x, stride = _norm_rows(x)
@@ -1198,7 +1202,7 @@ def norm_backward(grad: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weig
     library, ws, ws_bytes, code = nat.lib(), None, 0, 0
     if dtype is not None:
         ws_bytes = library.kf_norm_backward_workspace_bytes(rows, width)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(ws_bytes, dtype=torch.uint8)
         code = nat.dtype_code(dtype)
     elif weight is not None:
         code = nat.dtype_code(weight.dtype)
