@@ -1047,7 +1047,8 @@ def _attention_shape(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths:
     """Checks the operands of one attention call; ``(sequences, length, token rows, heads, kv_heads, width)``."""
     nat.require_device(q, "q"), nat.require_device(k, "k"), nat.require_device(v, "v")
     _require(k.dtype == q.dtype == v.dtype and k.device == q.device == v.device, "q, k and v share one dtype and one device")
-    _require(q.dtype in (torch.bfloat16, torch.float32), f"attention takes bfloat16 or float32 tensors, not {q.dtype}")
+    if q.dtype not in (torch.bfloat16, torch.float32):
+        _require(False, f"attention takes bfloat16 or float32 tensors, not {q.dtype}")
     packed = cu_seqlens is not None
     _require(not (packed and lengths is not None), "lengths (padded batch) and cu_seqlens (packed batch) exclude each other")
     shape, kv_shape = tuple(q.shape), tuple(k.shape)
@@ -1057,7 +1058,8 @@ def _attention_shape(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths:
              "k and v have the shape of q, but for the number of heads")
     heads, kv_heads, width = shape[-2], kv_shape[-2], shape[-1]
     _require(kv_heads > 0 and heads > 0 and heads % kv_heads == 0, "the number of heads is a multiple of the number of key / value heads")
-    _require(0 < width <= ATTENTION_MAX_WIDTH, f"head widths up to {ATTENTION_MAX_WIDTH}")
+    if not 0 < width <= ATTENTION_MAX_WIDTH:
+        _require(False, f"head widths up to {ATTENTION_MAX_WIDTH}")
     _require(width * q.element_size() % 16 == 0, "the head width is a whole number of 16-byte chunks")
     _require(math.isfinite(scale) and scale > 0, "scale is positive and finite")
     for name, t in (("lengths", lengths), ("cu_seqlens", cu_seqlens)):
@@ -1128,7 +1130,7 @@ def attention_backward(grad: torch.Tensor, out: torch.Tensor, lse: torch.Tensor,
     return dq, dk, dv
 
 
-_NORM_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_NORM_CODES = {dtype: nat.dtype_code(dtype) for dtype in (torch.float32, torch.bfloat16, torch.float16)}
 
 
 def _norm_rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
@@ -1141,42 +1143,49 @@ def _norm_rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return flat, flat.stride(0)
 
 
-def _norm_check(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]) -> None:
+def _norm_vector(t: Optional[torch.Tensor], name: str, x: torch.Tensor) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    nat.require_device(t, name)
+    # (messages are put together only when they are needed: a norm of a few rows takes less time than its launch)
+    if t.dim() != 1 or t.numel() != x.shape[-1] or t.get_device() != x.get_device():
+        _require(False, f"{name} is a vector of x's width on x's device")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _norm_operands(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]):
+    """Checks the operands of a norm; ``(rows, width, type code of x, weight, bias, type code of the vectors)``."""
     nat.require_device(x, "x")
     _require(x.dim() >= 1 and x.shape[-1] > 0, "x has a last axis to normalise over")
-    _require(x.dtype in _NORM_DTYPES, f"norms take float32, bfloat16 or float16 tensors, not {x.dtype}")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None:
-            nat.require_device(t, name)
-            _require(t.device == x.device and t.dim() == 1 and t.numel() == x.shape[-1], f"{name} is a vector of x's width on x's device")
-            _require(t.dtype in _NORM_DTYPES and (weight is None or t.dtype == weight.dtype),
-                     "weight and bias share one of the dtypes float32, bfloat16 and float16")
+    code, width = _NORM_CODES.get(x.dtype), x.shape[-1]
+    if code is None:
+        _require(False, f"norms take float32, bfloat16 or float16 tensors, not {x.dtype}")
+    weight, bias = _norm_vector(weight, "weight", x), _norm_vector(bias, "bias", x)
+    vector = weight if weight is not None else bias
+    vector_code = 0 if vector is None else _NORM_CODES.get(vector.dtype)
+    _require(vector_code is not None and (weight is None or bias is None or weight.dtype == bias.dtype),
+             "weight and bias share one of the dtypes float32, bfloat16 and float16")
+    return x.numel() // width, width, code, weight, bias, vector_code
 
 
 def norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float, centred: bool,
                  out_dtype: torch.dtype, with_stats: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Layer norm (``centred``) or RMS norm over the last axis (kf_norm_forward): the output and the fp32 ``[rows, 2]`` statistics
     (mean, reciprocal deviation) the backward call reads."""
-    _norm_check(x, weight, bias)
-    _require(out_dtype in _NORM_DTYPES, f"norms return float32, bfloat16 or float16 tensors, not {out_dtype}")
+    rows, width, code, weight, bias, vector_code = _norm_operands(x, weight, bias)
+    out_code = _NORM_CODES.get(out_dtype)
+    if out_code is None:
+        _require(False, f"norms return float32, bfloat16 or float16 tensors, not {out_dtype}")
     _require(math.isfinite(eps) and eps >= 0, "eps is finite and not negative")
-    width = x.shape[-1]
-    rows = x.numel() // width
-    out = _like(x) if out_dtype == x.dtype else x.new_empty(x.shape, dtype=out_dtype)
+    out = _like(x) if out_code == code else x.new_empty(x.shape, dtype=out_dtype)
     stats = x.new_empty((rows, 2), dtype=torch.float32) if with_stats else None
     if rows == 0:
         return out, stats
     x, stride = _norm_rows(x)
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    vector = weight if weight is not None else bias
     with _on_device_of(x):
-        nat.check(
-            nat.lib().kf_norm_forward(out.data_ptr(), nat.dtype_code(out_dtype), _ptr(stats), x.data_ptr(), nat.dtype_code(x.dtype), rows,
-                                      width, stride, _ptr(weight), _ptr(bias), 0 if vector is None else nat.dtype_code(vector.dtype),
-                                      int(centred), eps, nat.launch_stream(x)),
-            "kf_norm_forward",
-        )
+        status = nat.lib().kf_norm_forward(out.data_ptr(), out_code, _ptr(stats), x.data_ptr(), code, rows, width, stride, _ptr(weight),
+                                           _ptr(bias), vector_code, int(centred), eps, nat.launch_stream(x))
+    nat.check(status, "kf_norm_forward")
     return out, stats
 
 
@@ -1185,10 +1194,9 @@ def norm_backward(grad: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weig
                   ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
     """Gradients of :func:`norm_forward`: ``(dx, dweight, dbias)``, each computed only where asked for (``with_input``, and the dtype
     of the vector whose gradient is wanted; one dtype for both)."""
-    _norm_check(x, weight, None)
-    _require(grad.shape == x.shape and grad.device == x.device and grad.dtype in _NORM_DTYPES, "grad has the shape and device of x")
-    width = x.shape[-1]
-    rows = x.numel() // width
+    rows, width, code, weight, _, vector_code = _norm_operands(x, weight, None)
+    grad_code = _NORM_CODES.get(grad.dtype)
+    _require(grad_code is not None and grad.shape == x.shape and grad.get_device() == x.get_device(), "grad has the shape and device of x")
     _require(stats.dtype == torch.float32 and stats.is_contiguous() and stats.shape == (rows, 2), "stats is what the forward call returned")
     dtype = weight_dtype if weight_dtype is not None else bias_dtype
     _require(bias_dtype in (None, dtype) and (weight is None or dtype in (None, weight.dtype)), "weight and bias share one dtype")
@@ -1198,19 +1206,14 @@ def norm_backward(grad: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weig
     if rows == 0:
         return dx, None if dweight is None else dweight.zero_(), None if dbias is None else dbias.zero_()
     x, stride = _norm_rows(x)
-    grad, weight = grad.contiguous(), None if weight is None else weight.contiguous()
-    library, ws, ws_bytes, code = nat.lib(), None, 0, 0
+    grad = grad if grad.is_contiguous() else grad.contiguous()
+    library, ws, ws_bytes = nat.lib(), None, 0
     if dtype is not None:
         ws_bytes = library.kf_norm_backward_workspace_bytes(rows, width)
         ws = x.new_empty(ws_bytes, dtype=torch.uint8)
-        code = nat.dtype_code(dtype)
-    elif weight is not None:
-        code = nat.dtype_code(weight.dtype)
+        vector_code = nat.dtype_code(dtype)
     with _on_device_of(x):
-        nat.check(
-            library.kf_norm_backward(_ptr(dx), _ptr(dweight), _ptr(dbias), grad.data_ptr(), nat.dtype_code(grad.dtype), x.data_ptr(),
-                                     nat.dtype_code(x.dtype), stats.data_ptr(), rows, width, stride, _ptr(weight), code, int(centred),
-                                     _ptr(ws), ws_bytes, nat.launch_stream(x)),
-            "kf_norm_backward",
-        )
+        status = library.kf_norm_backward(_ptr(dx), _ptr(dweight), _ptr(dbias), grad.data_ptr(), grad_code, x.data_ptr(), code, stats.data_ptr(),
+                                          rows, width, stride, _ptr(weight), vector_code, int(centred), _ptr(ws), ws_bytes, nat.launch_stream(x))
+    nat.check(status, "kf_norm_backward")
     return dx, dweight, dbias
