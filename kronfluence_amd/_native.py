@@ -149,6 +149,23 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def launch_stream(t: torch.Tensor) -> int:
-    """The current stream of ``t``'s device as a raw handle, without the Stream object ``stream_ptr`` builds (2 us of a 4 us launch)."""
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
+_autograd = None
+
+
+def autograd():
+    """The C++ nodes of the differentiable operators (``csrc/kf_autograd.cpp``: what ``functional.py`` calls), loaded once."""
+    global _autograd
+    if _autograd is None:
+        lib()  # the entry points the nodes call
+        try:
+            from kronfluence_amd import _autograd as module
+        except ImportError as exc:
+            raise KfError(
+                f"kronfluence_amd/_autograd.so cannot be loaded ({exc}): the extension is not built. Run `python -c \"import __graft_entry__ "
+                "as g; g.build()\"` (or kronfluence_amd/csrc/build.sh). There is no fallback."
+            ) from exc
+        if module.abi_version() != ABI_VERSION:
+            raise KfError(f"_autograd.so ABI {module.abi_version()} != binding ABI {ABI_VERSION}; rebuild.")
+        module.set_error_type(KfError)
+        _autograd = module
+    return _autograd

@@ -27,3 +27,17 @@ objects=("${units[@]/#/${here}/obj/}")
 objects=("${objects[@]/%/.o}")
 "${HIPCC}" --offload-arch=gfx950 -shared -fPIC "${objects[@]}" -o "${out}"
 echo "built ${out}"
+
+# the autograd nodes over the C ABI (host code: no device code is in it)
+ext="${here}/../_autograd.so"
+stale=0
+for dep in "${here}/kf_autograd.cpp" "${here}/../../include/kronfluence_hip.h" "${here}/build.sh"; do [[ "${dep}" -nt "${ext}" ]] && stale=1; done
+if [[ ! -f "${ext}" || ${stale} -eq 1 ]]; then
+  read -r torch_dir python_include cxx11 < <(python3 -c 'import os, sysconfig, torch
+print(os.path.dirname(torch.__file__), sysconfig.get_paths()["include"], int(torch._C._GLIBCXX_USE_CXX11_ABI))')
+  "${CXX:-g++}" -O2 -std=c++17 -fPIC -shared -Wall -D_GLIBCXX_USE_CXX11_ABI="${cxx11}" -D__HIP_PLATFORM_AMD__=1 -DUSE_ROCM=1 \
+    -I"${torch_dir}/include" -I"${torch_dir}/include/torch/csrc/api/include" -I"${python_include}" -I"${ROCM_PATH:-/opt/rocm}/include" \
+    "${here}/kf_autograd.cpp" -o "${ext}" -L"${torch_dir}/lib" -ltorch_python -ltorch_cpu -lc10 -lc10_hip \
+    -L"${here}/.." -l:libkronfluence_hip.so -Wl,-rpath,'$ORIGIN'
+fi
+echo "built ${ext}"

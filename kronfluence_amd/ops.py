@@ -8,7 +8,6 @@ from PyTorch's caching allocator.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import logging
 import math
@@ -1002,218 +1001,3 @@ def cast(src: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
         "kf_cast",
     )
     return out
-
-
-# ---------------------------------------------------------------------------------------------
-# Model passes: attention and norms (autograd on top of these: kronfluence_amd/functional.py)
-# ---------------------------------------------------------------------------------------------
-ATTENTION_MAX_WIDTH = 128
-_MAX_TOKEN_BYTES = 1 << 23
-_NO_GUARD = contextlib.nullcontext()
-
-
-def _on_device_of(t: torch.Tensor):
-    """Context in which a launch goes to ``t``'s device (nothing to do when that is the current one, as it nearly always is)."""
-    return _NO_GUARD if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-def _like(t: torch.Tensor) -> torch.Tensor:
-    """An uninitialised contiguous tensor of ``t``'s shape, dtype and device."""
-    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
-
-
-def _heads_operand(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself if the kernels can read it in place (``[..., heads, width]``: contiguous width, 16-byte aligned start and
-    strides), else a contiguous copy."""
-    if t.data_ptr() % 16 == 0:
-        if t.is_contiguous():   # (the width is whole 16-byte chunks: so are the strides)
-            return t
-        size, tokens = t.element_size(), t.stride(-3)
-        if (t.stride(-1) == 1 and all(n == 1 or s * size % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
-                and (t.shape[-3] == 1 or t.shape[-1] <= tokens <= _MAX_TOKEN_BYTES // size)):
-            return t
-    return t.clone(memory_format=torch.contiguous_format)
-
-
-def _heads_view(t: torch.Tensor) -> nat.kf_heads_view:
-    # an axis of one element may carry any stride: it is never multiplied by anything but 0
-    shape, strides = t.shape, t.stride()
-    batch = strides[0] if t.dim() == 4 and shape[0] > 1 else 0
-    return nat.kf_heads_view(t.data_ptr(), batch, strides[-3] if shape[-3] > 1 else shape[-1], strides[-2] if shape[-2] > 1 else 0)
-
-
-def _attention_shape(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tensor],
-                     cu_seqlens: Optional[torch.Tensor], scale: float) -> Tuple[int, int, int, int, int, int]:
-    """Checks the operands of one attention call; ``(sequences, length, token rows, heads, kv_heads, width)``."""
-    nat.require_device(q, "q"), nat.require_device(k, "k"), nat.require_device(v, "v")
-    _require(k.dtype == q.dtype == v.dtype and k.device == q.device == v.device, "q, k and v share one dtype and one device")
-    if q.dtype not in (torch.bfloat16, torch.float32):
-        _require(False, f"attention takes bfloat16 or float32 tensors, not {q.dtype}")
-    packed = cu_seqlens is not None
-    _require(not (packed and lengths is not None), "lengths (padded batch) and cu_seqlens (packed batch) exclude each other")
-    shape, kv_shape = tuple(q.shape), tuple(k.shape)
-    _require(len(shape) == (3 if packed else 4),
-             "q is [tokens, heads, width] with cu_seqlens, [batch, length, heads, width] without")
-    _require(kv_shape == tuple(v.shape) and kv_shape[:-2] == shape[:-2] and kv_shape[-1] == shape[-1],
-             "k and v have the shape of q, but for the number of heads")
-    heads, kv_heads, width = shape[-2], kv_shape[-2], shape[-1]
-    _require(kv_heads > 0 and heads > 0 and heads % kv_heads == 0, "the number of heads is a multiple of the number of key / value heads")
-    if not 0 < width <= ATTENTION_MAX_WIDTH:
-        _require(False, f"head widths up to {ATTENTION_MAX_WIDTH}")
-    _require(width * q.element_size() % 16 == 0, "the head width is a whole number of 16-byte chunks")
-    _require(math.isfinite(scale) and scale > 0, "scale is positive and finite")
-    for name, t in (("lengths", lengths), ("cu_seqlens", cu_seqlens)):
-        if t is not None:
-            nat.require_device(t, name)
-            _require(t.device == q.device and t.dim() == 1 and t.dtype in (torch.int32, torch.int64),
-                     f"{name} is a vector of int32 or int64 on the device of q")
-    if packed:
-        _require(cu_seqlens.numel() >= 1, "cu_seqlens holds the first row of every sequence and the last row's end")
-        return cu_seqlens.numel() - 1, 0, shape[0], heads, kv_heads, width
-    _require(lengths is None or lengths.numel() == shape[0], "lengths has one entry per row of the batch")
-    return shape[0], shape[1], shape[0] * shape[1], heads, kv_heads, width
-
-
-def _row_counts(t: Optional[torch.Tensor], most: int) -> Optional[torch.Tensor]:
-    """``lengths`` / ``cu_seqlens`` as the kernels read them: contiguous int32 (which they clamp to the rows that exist)."""
-    if t is None:
-        return None
-    return (t if t.dtype == torch.int32 else t.clamp(0, most).to(torch.int32)).contiguous()
-
-
-def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool, scale: float,
-                      lengths: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None,
-                      with_lse: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """``softmax(scale q k^T + mask) v`` over whole prompts (kf_attention_forward): the output and, for the backward call, the fp32
-    ``[heads, token rows]`` log-sum of every row."""
-    sequences, length, rows, heads, kv_heads, width = _attention_shape(q, k, v, lengths, cu_seqlens, scale)
-    out = _like(q)
-    lse = q.new_empty((heads, rows), dtype=torch.float32) if with_lse else None
-    if sequences == 0 or rows == 0:
-        return out.zero_(), lse
-    q, k, v = _heads_operand(q), _heads_operand(k), _heads_operand(v)
-    lengths, offsets = _row_counts(lengths, length), _row_counts(cu_seqlens, rows)
-    with _on_device_of(q):
-        nat.check(
-            nat.lib().kf_attention_forward(_heads_view(out), _ptr(lse), _heads_view(q), _heads_view(k), _heads_view(v),
-                                           nat.dtype_code(q.dtype), sequences, length, rows, heads, kv_heads, width, _ptr(lengths),
-                                           _ptr(offsets), int(causal), scale, nat.launch_stream(q)),
-            "kf_attention_forward",
-        )
-    return out, lse
-
-
-def attention_backward(grad: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
-                       causal: bool, scale: float, lengths: Optional[torch.Tensor] = None,
-                       cu_seqlens: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """Gradients of :func:`attention_forward` with respect to ``q``, ``k`` and ``v`` (kf_attention_backward), contiguous."""
-    sequences, length, rows, heads, kv_heads, width = _attention_shape(q, k, v, lengths, cu_seqlens, scale)
-    _require(grad.shape == out.shape == q.shape and grad.dtype == out.dtype == q.dtype and grad.device == out.device == q.device,
-             "grad and out have the shape, dtype and device of q")
-    _require(lse.dtype == torch.float32 and lse.is_contiguous() and lse.shape == (heads, rows), "lse is what the forward call returned")
-    dq, dk, dv = _like(q), _like(k), _like(v)
-    if sequences == 0 or rows == 0:
-        return dq.zero_(), dk.zero_(), dv.zero_()
-    grad, out, q, k, v = (_heads_operand(t) for t in (grad, out, q, k, v))
-    lengths, offsets = _row_counts(lengths, length), _row_counts(cu_seqlens, rows)
-    library = nat.lib()
-    ws_bytes = library.kf_attention_backward_workspace_bytes(sequences, length, rows, heads, kv_heads, width, int(offsets is not None), int(causal))
-    ws = q.new_empty(ws_bytes, dtype=torch.uint8)
-    with _on_device_of(q):
-        nat.check(
-            library.kf_attention_backward(_heads_view(dq), _heads_view(dk), _heads_view(dv), _heads_view(grad), _heads_view(out),
-                                          lse.data_ptr(), _heads_view(q), _heads_view(k), _heads_view(v), nat.dtype_code(q.dtype),
-                                          sequences, length, rows, heads, kv_heads, width, _ptr(lengths), _ptr(offsets), int(causal),
-                                          scale, ws.data_ptr(), ws_bytes, nat.launch_stream(q)),
-            "kf_attention_backward",
-        )
-    return dq, dk, dv
-
-
-_NORM_CODES = {dtype: nat.dtype_code(dtype) for dtype in (torch.float32, torch.bfloat16, torch.float16)}
-
-
-def _norm_rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    """``x`` with a contiguous last axis and its rows' stride (in place where the strides of ``x`` allow it)."""
-    width = x.shape[-1]
-    if x.is_contiguous():
-        return x, width
-    flat = x.reshape(-1, width)
-    flat = flat if flat.stride(1) == 1 or width == 1 else flat.contiguous()
-    return flat, flat.stride(0)
-
-
-def _norm_vector(t: Optional[torch.Tensor], name: str, x: torch.Tensor) -> Optional[torch.Tensor]:
-    if t is None:
-        return None
-    nat.require_device(t, name)
-    # (messages are put together only when they are needed: a norm of a few rows takes less time than its launch)
-    if t.dim() != 1 or t.numel() != x.shape[-1] or t.get_device() != x.get_device():
-        _require(False, f"{name} is a vector of x's width on x's device")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _norm_operands(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor]):
-    """Checks the operands of a norm; ``(rows, width, type code of x, weight, bias, type code of the vectors)``."""
-    nat.require_device(x, "x")
-    _require(x.dim() >= 1 and x.shape[-1] > 0, "x has a last axis to normalise over")
-    code, width = _NORM_CODES.get(x.dtype), x.shape[-1]
-    if code is None:
-        _require(False, f"norms take float32, bfloat16 or float16 tensors, not {x.dtype}")
-    weight, bias = _norm_vector(weight, "weight", x), _norm_vector(bias, "bias", x)
-    vector = weight if weight is not None else bias
-    vector_code = 0 if vector is None else _NORM_CODES.get(vector.dtype)
-    _require(vector_code is not None and (weight is None or bias is None or weight.dtype == bias.dtype),
-             "weight and bias share one of the dtypes float32, bfloat16 and float16")
-    return x.numel() // width, width, code, weight, bias, vector_code
-
-
-def norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float, centred: bool,
-                 out_dtype: torch.dtype, with_stats: bool = True) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """Layer norm (``centred``) or RMS norm over the last axis (kf_norm_forward): the output and the fp32 ``[rows, 2]`` statistics
-    (mean, reciprocal deviation) the backward call reads."""
-    rows, width, code, weight, bias, vector_code = _norm_operands(x, weight, bias)
-    out_code = _NORM_CODES.get(out_dtype)
-    if out_code is None:
-        _require(False, f"norms return float32, bfloat16 or float16 tensors, not {out_dtype}")
-    _require(math.isfinite(eps) and eps >= 0, "eps is finite and not negative")
-    out = _like(x) if out_code == code else x.new_empty(x.shape, dtype=out_dtype)
-    stats = x.new_empty((rows, 2), dtype=torch.float32) if with_stats else None
-    if rows == 0:
-        return out, stats
-    x, stride = _norm_rows(x)
-    with _on_device_of(x):
-        status = nat.lib().kf_norm_forward(out.data_ptr(), out_code, _ptr(stats), x.data_ptr(), code, rows, width, stride, _ptr(weight),
-                                           _ptr(bias), vector_code, int(centred), eps, nat.launch_stream(x))
-    nat.check(status, "kf_norm_forward")
-    return out, stats
-
-
-def norm_backward(grad: torch.Tensor, x: torch.Tensor, stats: torch.Tensor, weight: Optional[torch.Tensor], centred: bool,
-                  with_input: bool = True, weight_dtype: Optional[torch.dtype] = None, bias_dtype: Optional[torch.dtype] = None
-                  ) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
-    """Gradients of :func:`norm_forward`: ``(dx, dweight, dbias)``, each computed only where asked for (``with_input``, and the dtype
-    of the vector whose gradient is wanted; one dtype for both)."""
-    rows, width, code, weight, _, vector_code = _norm_operands(x, weight, None)
-    grad_code = _NORM_CODES.get(grad.dtype)
-    _require(grad_code is not None and grad.shape == x.shape and grad.get_device() == x.get_device(), "grad has the shape and device of x")
-    _require(stats.dtype == torch.float32 and stats.is_contiguous() and stats.shape == (rows, 2), "stats is what the forward call returned")
-    dtype = weight_dtype if weight_dtype is not None else bias_dtype
-    _require(bias_dtype in (None, dtype) and (weight is None or dtype in (None, weight.dtype)), "weight and bias share one dtype")
-    dx = _like(x) if with_input else None
-    dweight = None if weight_dtype is None else x.new_empty(width, dtype=dtype)
-    dbias = None if bias_dtype is None else x.new_empty(width, dtype=dtype)
-    if rows == 0:
-        return dx, None if dweight is None else dweight.zero_(), None if dbias is None else dbias.zero_()
-    x, stride = _norm_rows(x)
-    grad = grad if grad.is_contiguous() else grad.contiguous()
-    library, ws, ws_bytes = nat.lib(), None, 0
-    if dtype is not None:
-        ws_bytes = library.kf_norm_backward_workspace_bytes(rows, width)
-        ws = x.new_empty(ws_bytes, dtype=torch.uint8)
-        vector_code = nat.dtype_code(dtype)
-    with _on_device_of(x):
-        status = library.kf_norm_backward(_ptr(dx), _ptr(dweight), _ptr(dbias), grad.data_ptr(), grad_code, x.data_ptr(), code, stats.data_ptr(),
-                                          rows, width, stride, _ptr(weight), vector_code, int(centred), _ptr(ws), ws_bytes, nat.launch_stream(x))
-    nat.check(status, "kf_norm_backward")
-    return dx, dweight, dbias

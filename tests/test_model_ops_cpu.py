@@ -1,4 +1,5 @@
-"""Refusals of kronfluence_amd/functional.py and of the C entries behind it: no GPU is needed to refuse a call."""
+"""Refusals of kronfluence_amd/functional.py and of the C entries behind it: no GPU is needed to refuse a call (what a call asks for
+is checked before where its tensors live)."""
 
 import ctypes
 
@@ -6,7 +7,7 @@ import pytest
 import torch
 
 from kronfluence_amd import _native as nat
-from kronfluence_amd import functional, ops
+from kronfluence_amd import functional
 
 BF16 = torch.bfloat16
 
@@ -19,20 +20,6 @@ def test_tensors_off_the_gpu_are_refused():
         functional.layer_norm(torch.zeros(2, 8))
     with pytest.raises(nat.KfError, match="lives on cpu"):
         functional.rms_norm(torch.zeros(2, 8), torch.ones(8))
-
-
-@pytest.fixture
-def anywhere(monkeypatch):
-    """Argument checks alone: the device check passes, and a call that passes every check stops before it launches anything."""
-    class Reached(Exception):
-        pass
-
-    def stop(*args, **kwargs):
-        raise Reached
-
-    monkeypatch.setattr(nat, "require_device", lambda t, name: None)
-    monkeypatch.setattr(torch.cuda, "current_device", stop)
-    return Reached
 
 
 def heads(*shape, dtype=BF16):
@@ -57,25 +44,17 @@ def heads(*shape, dtype=BF16):
     (dict(lengths=torch.tensor([[4]])), "vector"),
     (dict(scale=0.0), "positive"), (dict(scale=-1.0), "positive"), (dict(scale=float("inf")), "positive"), (dict(scale=float("nan")), "positive"),
 ])
-def test_attention_refuses(anywhere, change, message):
+def test_attention_refuses(change, message):
     call = dict(q=heads(1, 4, 2, 64), k=heads(1, 4, 2, 64), v=heads(1, 4, 2, 64))
     call.update(change)
     with pytest.raises(nat.KfError, match=message):
         functional.attention(**call)
 
 
-def test_attention_packed_refuses_an_empty_offset_vector(anywhere):
+def test_attention_packed_refuses_an_empty_offset_vector():
     q = heads(4, 2, 64)
     with pytest.raises(nat.KfError, match="cu_seqlens"):
         functional.attention(q, q, q, cu_seqlens=torch.zeros(0, dtype=torch.int32))
-
-
-def test_attention_pads_widths_to_whole_chunks(anywhere, monkeypatch):
-    """An odd head width is padded with zero columns and reaches the kernel; the answer has the width asked for."""
-    seen = []
-    monkeypatch.setattr(ops, "attention_forward", lambda q, k, v, *args, **kwargs: (seen.append((q.shape, args[1])), (q, None))[1])
-    out = functional.attention(*(heads(1, 4, 2, 33) for _ in range(3)))
-    assert seen == [((1, 4, 2, 40), 33 ** -0.5)] and out.shape == (1, 4, 2, 33)
 
 
 @pytest.mark.parametrize("change,message", [
@@ -90,14 +69,12 @@ def test_attention_pads_widths_to_whole_chunks(anywhere, monkeypatch):
     (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
     (dict(out_dtype=torch.float64), "return float32"),
 ])
-def test_norms_refuse(anywhere, change, message):
+def test_norms_refuse(change, message):
     call = dict(x=torch.zeros(2, 8))
     call.update(change)
     with pytest.raises(nat.KfError, match=message):
         functional.layer_norm(**call)
     if "bias" not in call:
-        if not call["x"].is_floating_point():
-            return   # (rms_norm's default eps is the machine epsilon of a floating type)
         with pytest.raises(nat.KfError, match=message):
             functional.rms_norm(**call)
 

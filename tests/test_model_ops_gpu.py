@@ -300,6 +300,25 @@ def test_attention_and_norm_in_two_captured_graphs(functional):
                 assert torch.equal(a, e), turn
 
 
+def test_second_derivatives_are_refused(functional):
+    """A graph of the gradients would silently lack these operators."""
+    from kronfluence_amd._native import KfError
+
+    x = make((3, 64), F32, 1).requires_grad_()
+    for y in (functional.layer_norm(x), functional.rms_norm(x), functional.attention(x.view(1, 3, 1, 64), *[x.view(1, 3, 1, 64)] * 2)):
+        with pytest.raises((KfError, RuntimeError), match="first derivatives"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_saved_tensors_are_guarded(functional):
+    """Writing in place to a tensor the backward pass reads is an error, as with torch's own operators."""
+    x, w = make((3, 64), F32, 1).requires_grad_(), make((64,), F32, 2)
+    y = functional.layer_norm(x, w)
+    w.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_attention_empty_batches(functional):
     for shape in ((0, 5, 2, 64), (3, 0, 2, 64)):
         q = torch.zeros(shape, dtype=BF16, device="cuda", requires_grad=True)
@@ -417,6 +436,7 @@ def test_norm_frozen_vectors_and_inputs(functional):
         y = functional.layer_norm(*leaves.values())
         for n, got in zip(names, torch.autograd.grad(y, [leaves[n] for n in names], g)):
             assert torch.equal(got, full[n]), (names, n)
+    check_norm(functional, x.clone(), None, b.clone(), g, True)     # a bias without a weight
 
 
 def test_norm_constant_rows_offsets_and_eps(functional):
