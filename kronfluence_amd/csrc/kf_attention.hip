@@ -255,18 +255,20 @@ __device__ __forceinline__ bool locate(const Args& a, int slot, bool last_first,
 
 // Workgroup -> (slot, kv_head, member of its group).  Consecutive workgroup ids go to the eight XCDs in turn, and each has an L2 of its
 // own: what reads the same k and v should go to one XCD, but no XCD may be left with the longest sequences.  Where (sequence, key /
-// value head) pairs of equal size are many, whole pairs are dealt to the XCDs (a.chunk = the slots of a sequence).  Otherwise
-// single tiles are, the heads of a tile one after the other: with 1, 2, 4 or a multiple of 8 heads an XCD then sees the same heads
-// in every tile.  The `members` query heads of a group stay together.  False: nothing left (the grid is rounded up).
+// value head) pairs of equal size are many, whole pairs are dealt to the XCDs (a.chunk = the tiles of a sequence), the heads of a
+// sequence one after the other (24 sequences of 29 to 233 tokens, 12 heads x 64 fp32: 210 us, 264 us with the sequences of a head one
+// after the other).  Otherwise single tiles are dealt, the heads of a tile one after
+// the other: with 1, 2, 4 or a multiple of 8 heads an XCD then sees the same heads in every tile.  The `members` query heads of a group
+// stay together.  False: nothing left (the grid is rounded up).
 constexpr int XCDS = 8;
 struct Item { int slot, kv_head, member; };
 __device__ __forceinline__ bool work_item(const Args& a, int members, Item& w) {
-    const int64_t id = blockIdx.x, chunk = static_cast<int64_t>(a.chunk) * members, n = id / XCDS;
-    const int64_t item = (n / chunk * XCDS + id % XCDS) * chunk + n % chunk, pair = item / members;
     const int kv_heads = a.heads / a.group;
+    const int64_t id = blockIdx.x, chunk = static_cast<int64_t>(a.chunk) * members, n = id / XCDS;
+    const int64_t item = (n / chunk * XCDS + id % XCDS) * chunk + n % chunk, pair = item / members, unit = pair / a.chunk;
     w.member = static_cast<int>(item % members);
-    w.slot = static_cast<int>(a.chunk > 1 ? pair % a.slots : pair / kv_heads);
-    w.kv_head = static_cast<int>(a.chunk > 1 ? pair / a.slots : pair % kv_heads);
+    w.kv_head = static_cast<int>(unit % kv_heads);
+    w.slot = static_cast<int>(unit / kv_heads * a.chunk + pair % a.chunk);
     return pair < static_cast<int64_t>(a.slots) * kv_heads;
 }
 
@@ -306,20 +308,35 @@ struct Held {
     }
 };
 
-// acc^T (lane = row, registers = columns d) -> memory, times `factor`
-template <class T, int DP>
-__device__ __forceinline__ void store_rows(const f32x16 (&acc)[DP / 32], T* base, int64_t token, int row, int written, int width, float factor,
-                                           int lane) {
-    if (row >= written) return;
-    T* p = base + row * token;
+// acc^T (lane = row, registers = columns d) times the lane's `factor` -> rows first .. first + 31 of memory, through LDS: a lane holds
+// four columns of a row at a time, and stores of 8 bytes per row cost as much as all the rest of a short sequence (256 x 128 x 12 x 64
+// bf16 forward: 43 us, 22 without the stores).  Every wave uses its own piece of `scratch`; the workgroup is done with its tiles.
+constexpr int PASS_BYTES = 256, PASS_STRIDE = PASS_BYTES + 16;   // bytes of a row per pass; rows apart in LDS
+constexpr int SCRATCH = ROWS * PASS_STRIDE;
+template <class S, int DP>
+__device__ __forceinline__ void store_rows(const f32x16 (&acc)[DP / 32], char* scratch, S* base, int64_t token, int first, int written, int width,
+                                           float factor, int wave, int lane) {
+    constexpr int COLUMNS = PASS_BYTES / static_cast<int>(sizeof(S)) < DP ? PASS_BYTES / static_cast<int>(sizeof(S)) : DP;
+    constexpr int CHUNKS = COLUMNS * static_cast<int>(sizeof(S)) / 16, PER = 16 / static_cast<int>(sizeof(S));
+    char* own = scratch + wave * 32 * PASS_STRIDE;
+    asm volatile("" : "+v"(lane));   // addresses are made here, not kept in registers across the caller's loop
 #pragma unroll
-    for (int t = 0; t < DP / 32; ++t)
+    for (int c0 = 0; c0 < DP; c0 += COLUMNS) {
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = 32 * t + 8 * i + 4 * (lane >> 5);
-            if (d < width)
-                Type<T>::store4(p + d, acc[t][4 * i] * factor, acc[t][4 * i + 1] * factor, acc[t][4 * i + 2] * factor, acc[t][4 * i + 3] * factor);
+        for (int t = c0 / 32; t < (c0 + COLUMNS < DP ? c0 + COLUMNS : DP) / 32; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                Type<S>::store4(own + (lane & 31) * PASS_STRIDE + (32 * t - c0 + 8 * i + 4 * (lane >> 5)) * static_cast<int>(sizeof(S)),
+                                acc[t][4 * i] * factor, acc[t][4 * i + 1] * factor, acc[t][4 * i + 2] * factor, acc[t][4 * i + 3] * factor);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < 32 * CHUNKS / 64; ++i) {
+            const int n = lane + 64 * i, row = n / CHUNKS, d = c0 + n % CHUNKS * PER;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(own + row * PASS_STRIDE + n % CHUNKS * 16);
+            if (first + row < written && d < width) *reinterpret_cast<u32x4*>(base + (first + row) * token + d) = v;
         }
+    }
 }
 
 template <class T, int DP, int N_THREADS = THREADS>
@@ -445,7 +462,8 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
     }
     sum += other_half(sum);
     const bool real = query < w.length;
-    store_rows<T, DP>(acc, o, a.o.token, query, w.written, a.width, real ? 1.0f / sum : 0.0f, lane);
+    __syncthreads();
+    store_rows<T, DP>(acc, lds, o, a.o.token, first, w.written, a.width, real ? 1.0f / sum : 0.0f, wave, lane);
     if (lse && half == 0 && query < w.written) lse[query] = real ? top + __builtin_amdgcn_logf(sum) : INFINITY;
 }
 
@@ -541,7 +559,8 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) acc[d] = f32x16{};
     }
-    store_rows<T, DP>(acc, dq, a.dq.token, query, w.written, a.width, a.scale, lane);
+    __syncthreads();
+    store_rows<T, DP>(acc, lds, dq, a.dq.token, first, w.written, a.width, a.scale, wave, lane);
 }
 
 // ---- backward: dk and dv --------------------------------------------------------------------------------------------------
@@ -679,19 +698,20 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
         settle<T>();
         if (n + 1 < steps) store(lds + ((n + 1) & 1) * STAGE);
     }
+    __syncthreads();
     if (a.parts > 1) {   // (w.stat + key: the token's row among all)
         const int64_t head = a.rows * a.width, kv_heads = a.heads / a.group;
         float* to = a.partial + (static_cast<int64_t>(item.member) * 2 * kv_heads + kv_head) * head + w.stat * a.width;
-        store_rows<float, DP>(ak, to, a.width, key, w.length, a.width, a.scale, lane);
-        store_rows<float, DP>(av, to + kv_heads * head, a.width, key, w.length, a.width, 1.0f, lane);
+        store_rows<float, DP>(ak, lds, to, a.width, first, w.length, a.width, a.scale, wave, lane);
+        store_rows<float, DP>(av, lds, to + kv_heads * head, a.width, first, w.length, a.width, 1.0f, wave, lane);
         return;
     }
     if (key >= w.length) {
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) { ak[d] = f32x16{}; av[d] = f32x16{}; }
     }
-    store_rows<T, DP>(ak, dk, a.dk.token, key, w.written, a.width, a.scale, lane);
-    store_rows<T, DP>(av, dv, a.dv.token, key, w.written, a.width, 1.0f, lane);
+    store_rows<T, DP>(ak, lds, dk, a.dk.token, first, w.written, a.width, a.scale, wave, lane);
+    store_rows<T, DP>(av, lds, dv, a.dv.token, first, w.written, a.width, 1.0f, wave, lane);
 }
 
 // dk and dv as the sums of the parts in order; zero in rows of no sequence.  One thread per four columns.
@@ -728,12 +748,15 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(const Args a) {
 template <class T, int DP>
 struct Shape {
     static constexpr bool TWO = sizeof(T) == 2, VL = TWO && DP > 96;
-    static constexpr int KEYS = TWO ? 64 : 32, QUERIES = TWO && DP <= 64 ? 64 : 32, WAVES = TWO ? 2 : 1;
-    static constexpr int KEY_LDS = 4 * Image<T, DP, KEYS>::BYTES;
-    static constexpr int QUERY_LDS = 4 * Image<T, DP, QUERIES>::BYTES + 4 * QUERIES * 4 + (VL ? Image<T, DP, ROWS>::BYTES : 0);
-    static constexpr auto forward = &attention_forward_kernel<T, DP, KEYS, WAVES>;
-    static constexpr auto dq = &attention_dq_kernel<T, DP, KEYS, WAVES>;
-    static constexpr auto dkv = &attention_dkv_kernel<T, DP, QUERIES, VL, WAVES>;
+    static constexpr int KEYS = TWO ? 64 : 32, QUERIES = TWO && DP <= 64 ? 64 : 32;
+    static constexpr int FORWARD_WAVES = !TWO ? 1 : DP <= 64 ? 4 : DP <= 96 ? 3 : 2, DQ_WAVES = !TWO ? 1 : DP <= 32 ? 4 : DP <= 64 ? 3 : 2;
+    static constexpr int DKV_WAVES = !TWO ? 1 : DP <= 32 ? 3 : 2;
+    static constexpr int KEY_LDS = std::max(4 * Image<T, DP, KEYS>::BYTES, SCRATCH);
+    static constexpr int QUERY_LDS =
+        std::max(4 * Image<T, DP, QUERIES>::BYTES + 4 * QUERIES * 4 + (VL ? Image<T, DP, ROWS>::BYTES : 0), SCRATCH);
+    static constexpr auto forward = &attention_forward_kernel<T, DP, KEYS, FORWARD_WAVES>;
+    static constexpr auto dq = &attention_dq_kernel<T, DP, KEYS, DQ_WAVES>;
+    static constexpr auto dkv = &attention_dkv_kernel<T, DP, QUERIES, VL, DKV_WAVES>;
 };
 
 template <class T, int DP>
