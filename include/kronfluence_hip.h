@@ -469,14 +469,19 @@ typedef struct kf_heads_view {
  */
 int kf_attention_forward(const kf_heads_view* out, float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v,
                          int dtype, int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width,
-                         const int32_t* lengths, const int32_t* offsets, int causal, float scale, void* stream);
+                         const int32_t* lengths, const int32_t* offsets, const int32_t* order, int causal, float scale, void* stream);
 int64_t kf_attention_backward_workspace_bytes(int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width,
                                               int packed, int causal);
 int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, const kf_heads_view* dv, const kf_heads_view* grad,
                           const kf_heads_view* out, const float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v,
                           int dtype, int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width,
-                          const int32_t* lengths, const int32_t* offsets, int causal, float scale, void* workspace, int64_t workspace_bytes,
-                          void* stream);
+                          const int32_t* lengths, const int32_t* offsets, const int32_t* order, int causal, float scale, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+/* Packed batches: kf_attention_order writes the order in which the tiles of the batch are best worked on (the longest documents first),
+ * to be handed to the forward and the backward call of the same offsets (nullable there; it changes no result).
+ * kf_attention_order_bytes is 0 where an order gains nothing. */
+int64_t kf_attention_order_bytes(int64_t sequences, int64_t rows, int64_t heads);
+int kf_attention_order(int32_t* order, const int32_t* offsets, int64_t sequences, int64_t rows, int causal, void* stream);
 
 /*
  * y = (x - mu) r w + b over the last axis: layer norm (centred != 0) or RMS norm (centred == 0: mu = 0), r = 1 / sqrt(mean (x - mu)^2

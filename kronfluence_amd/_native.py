@@ -91,9 +91,11 @@ SIGNATURES = {
     "kf_lowrank_rows_dot": (_i, [_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _f, _p]),
     "kf_mul_bcast": (_i, [_p, _p, _i, _p, _i64, _i64, _f, _p]),
     "kf_cast": (_i, [_p, _i, _p, _i, _i64, _p]),
-    "kf_attention_forward": (_i, [_h, _p, _h, _h, _h, _i] + [_i64] * 6 + [_p, _p, _i, _f, _p]),
+    "kf_attention_order_bytes": (_i64, [_i64, _i64, _i64]),
+    "kf_attention_order": (_i, [_p, _p, _i64, _i64, _i, _p]),
+    "kf_attention_forward": (_i, [_h, _p, _h, _h, _h, _i] + [_i64] * 6 + [_p, _p, _p, _i, _f, _p]),
     "kf_attention_backward_workspace_bytes": (_i64, [_i64] * 6 + [_i, _i]),
-    "kf_attention_backward": (_i, [_h] * 5 + [_p] + [_h] * 3 + [_i] + [_i64] * 6 + [_p, _p, _i, _f, _p, _i64, _p]),
+    "kf_attention_backward": (_i, [_h] * 5 + [_p] + [_h] * 3 + [_i] + [_i64] * 6 + [_p, _p, _p, _i, _f, _p, _i64, _p]),
     "kf_norm_forward": (_i, [_p, _i, _p, _p, _i, _i64, _i64, _i64, _p, _p, _i, _i, _f, _p]),
     "kf_norm_backward_workspace_bytes": (_i64, [_i64, _i64]),
     "kf_norm_backward": (_i, [_p, _p, _p, _p, _i, _p, _i, _p, _i64, _i64, _i64, _p, _i, _i, _p, _i64, _p]),

@@ -56,6 +56,7 @@ struct Args {
     int parts;
     const int32_t* lengths;        // per sequence (padded batch), or null
     const int32_t* offsets;        // [sequences + 1] (packed batch), or null
+    const int32_t* order;          // [slots]: the tile slots by falling cost (packed batch), or null
     int64_t rows;                  // token rows in all: batch * length, or the packed total
     int sequences, length;         // length: token rows per sequence (padded batch)
     int heads, group, width, causal;
@@ -269,7 +270,43 @@ __device__ __forceinline__ bool work_item(const Args& a, int members, Item& w) {
     w.member = static_cast<int>(item % members);
     w.kv_head = static_cast<int>(unit % kv_heads);
     w.slot = static_cast<int>(unit / kv_heads * a.chunk + pair % a.chunk);
-    return pair < static_cast<int64_t>(a.slots) * kv_heads;
+    if (pair >= static_cast<int64_t>(a.slots) * kv_heads) return false;
+    if (a.order) w.slot = a.order[w.slot];
+    return true;
+}
+
+// The slots of a packed batch by falling cost: documents come in any order, and a long one whose tiles start last leaves the card
+// waiting for it (24 documents of 12011 tokens, 16/4 heads x 128 bf16: forward 101 to 85 us, dq 131 to 123, dk / dv 183 to 152).  The cost of a slot is that of its tile in the
+// kernels over queries (last tiles first) and in the one over keys (first tiles first) alike: the tiles of its sequence it meets.
+// One workgroup: a histogram of costs, places from the highest down; the order inside a cost is of no consequence.
+constexpr int COSTS = 2048, MAX_ORDERED = 16384;
+__global__ __launch_bounds__(1024) void attention_order_kernel(const Args a, int32_t* order) {
+    __shared__ int place[COSTS], sums[1024];
+    auto cost_of = [&](int slot) {
+        Place w;
+        if (!locate(a, slot, false, w) || w.length == 0) return 0;
+        const int tiles = (w.length + ROWS - 1) / ROWS;
+        return min(a.causal ? tiles - w.row0 / ROWS : tiles, COSTS - 1);
+    };
+    for (int i = threadIdx.x; i < COSTS; i += 1024) place[i] = 0;
+    __syncthreads();
+    for (int s = threadIdx.x; s < a.slots; s += 1024) atomicAdd(&place[cost_of(s)], 1);
+    __syncthreads();
+    // thread t: costs COSTS - 1 - 2 t and the next lower one; sums[t]: the slots of all higher costs
+    const int high = COSTS - 1 - 2 * threadIdx.x, n0 = place[high], n1 = place[high - 1];
+    sums[threadIdx.x] = n0 + n1;
+    __syncthreads();
+    for (int step = 1; step < 1024; step *= 2) {
+        const int other = threadIdx.x >= step ? sums[threadIdx.x - step] : 0;
+        __syncthreads();
+        sums[threadIdx.x] += other;
+        __syncthreads();
+    }
+    const int before = sums[threadIdx.x] - n0 - n1;
+    place[high] = before;
+    place[high - 1] = before + n0;
+    __syncthreads();
+    for (int s = threadIdx.x; s < a.slots; s += 1024) order[atomicAdd(&place[cost_of(s)], 1)] = s;
 }
 
 template <class T>
@@ -311,14 +348,17 @@ struct Held {
 // acc^T (lane = row, registers = columns d) times the lane's `factor` -> rows first .. first + 31 of memory, through LDS: a lane holds
 // four columns of a row at a time, and stores of 8 bytes per row cost as much as all the rest of a short sequence (256 x 128 x 12 x 64
 // bf16 forward: 43 us, 22 without the stores).  Every wave uses its own piece of `scratch`; the workgroup is done with its tiles.
-constexpr int PASS_BYTES = 256, PASS_STRIDE = PASS_BYTES + 16;   // bytes of a row per pass; rows apart in LDS
-constexpr int SCRATCH = ROWS * PASS_STRIDE;
+template <class S, int DP>
+struct Pass {   // the columns of one pass: up to 256 bytes of a row, rows 16 bytes further apart in LDS
+    static constexpr int COLUMNS = std::min(256 / static_cast<int>(sizeof(S)), DP), STRIDE = COLUMNS * static_cast<int>(sizeof(S)) + 16;
+    static constexpr int SCRATCH = ROWS * STRIDE;
+};
 template <class S, int DP>
 __device__ __forceinline__ void store_rows(const f32x16 (&acc)[DP / 32], char* scratch, S* base, int64_t token, int first, int written, int width,
                                            float factor, int wave, int lane) {
-    constexpr int COLUMNS = PASS_BYTES / static_cast<int>(sizeof(S)) < DP ? PASS_BYTES / static_cast<int>(sizeof(S)) : DP;
+    constexpr int COLUMNS = Pass<S, DP>::COLUMNS, STRIDE = Pass<S, DP>::STRIDE;
     constexpr int CHUNKS = COLUMNS * static_cast<int>(sizeof(S)) / 16, PER = 16 / static_cast<int>(sizeof(S));
-    char* own = scratch + wave * 32 * PASS_STRIDE;
+    char* own = scratch + wave * 32 * STRIDE;
     asm volatile("" : "+v"(lane));   // addresses are made here, not kept in registers across the caller's loop
 #pragma unroll
     for (int c0 = 0; c0 < DP; c0 += COLUMNS) {
@@ -327,13 +367,13 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[DP / 32], char* s
         for (int t = c0 / 32; t < (c0 + COLUMNS < DP ? c0 + COLUMNS : DP) / 32; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                Type<S>::store4(own + (lane & 31) * PASS_STRIDE + (32 * t - c0 + 8 * i + 4 * (lane >> 5)) * static_cast<int>(sizeof(S)),
+                Type<S>::store4(own + (lane & 31) * STRIDE + (32 * t - c0 + 8 * i + 4 * (lane >> 5)) * static_cast<int>(sizeof(S)),
                                 acc[t][4 * i] * factor, acc[t][4 * i + 1] * factor, acc[t][4 * i + 2] * factor, acc[t][4 * i + 3] * factor);
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int i = 0; i < 32 * CHUNKS / 64; ++i) {
             const int n = lane + 64 * i, row = n / CHUNKS, d = c0 + n % CHUNKS * PER;
-            const u32x4 v = *reinterpret_cast<const u32x4*>(own + row * PASS_STRIDE + n % CHUNKS * 16);
+            const u32x4 v = *reinterpret_cast<const u32x4*>(own + row * STRIDE + n % CHUNKS * 16);
             if (first + row < written && d < width) *reinterpret_cast<u32x4*>(base + (first + row) * token + d) = v;
         }
     }
@@ -350,13 +390,14 @@ __device__ __forceinline__ void zero_rows(T* base, int64_t token, int row0, int 
 }
 
 // A read of a matrix instruction's result needs wait states that the compiler inserts; where a branch stands between the two it has
-// left them out on one of the paths (fp32: 16-pass instructions, the first read behind the branch saw row 15 of the tile before it
-// was written).  Put between the last matrix instruction and such a branch.  tests/test_wait_states_cpu.py follows every path of the built code.
-template <class T>
+// left some out on one of the paths (fp32: the first read behind the branch saw row 15 of the tile before it was written).  Put between
+// the last matrix instruction and such a branch; tests/test_wait_states_cpu.py follows every path of the built code and says where.
+template <class T, bool TWO_BYTE_TYPES = false>
 __device__ __forceinline__ void settle() {
-    if constexpr (sizeof(T) == 4) {
+    if constexpr (sizeof(T) == 4 || TWO_BYTE_TYPES) {
         __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_nop 15\n\ts_nop 3");
+        if constexpr (sizeof(T) == 4) asm volatile("s_nop 15\n\ts_nop 3");
+        else asm volatile("s_nop 11");
         __builtin_amdgcn_sched_barrier(0);
     }
 }
@@ -413,7 +454,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
 #pragma unroll
                 for (int i = 0; i < Img::SLABS; ++i) s[b] = Type<T>::mma(read.rows(kt, 32 * b, i), q.f[i], s[b]);
             }
-            settle<T>();
+            settle<T, true>();
             if (k0 + BK > w.length || (a.causal && k0 + BK - 1 > first)) {
                 const int visible = a.causal ? min(w.length, query + 1) : w.length;
 #pragma unroll
@@ -747,15 +788,16 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(const Args a) {
 // Tile rows and waves per SIMD of each kernel.
 template <class T, int DP>
 struct Shape {
-    static constexpr bool TWO = sizeof(T) == 2, VL = TWO && DP > 96;
-    static constexpr int KEYS = TWO ? 64 : 32, QUERIES = TWO && DP <= 64 ? 64 : 32;
-    static constexpr int FORWARD_WAVES = !TWO ? 1 : DP <= 64 ? 4 : DP <= 96 ? 3 : 2, DQ_WAVES = !TWO ? 1 : DP <= 32 ? 4 : DP <= 64 ? 3 : 2;
-    static constexpr int DKV_WAVES = !TWO ? 1 : DP <= 32 ? 3 : 2;
-    static constexpr int KEY_LDS = std::max(4 * Image<T, DP, KEYS>::BYTES, SCRATCH);
-    static constexpr int QUERY_LDS =
-        std::max(4 * Image<T, DP, QUERIES>::BYTES + 4 * QUERIES * 4 + (VL ? Image<T, DP, ROWS>::BYTES : 0), SCRATCH);
-    static constexpr auto forward = &attention_forward_kernel<T, DP, KEYS, FORWARD_WAVES>;
-    static constexpr auto dq = &attention_dq_kernel<T, DP, KEYS, DQ_WAVES>;
+    static constexpr bool TWO = sizeof(T) == 2, VL = TWO && (DP == 64 || DP > 96);
+    static constexpr int FORWARD_KEYS = TWO && DP <= 64 ? 64 : 32, DQ_KEYS = TWO && DP > 64 ? 64 : 32, QUERIES = TWO && DP <= 32 ? 64 : 32;
+    static constexpr int FORWARD_WAVES = !TWO ? 1 : DP <= 64 ? 4 : 3, DQ_WAVES = !TWO ? 1 : DP <= 64 ? 4 : 2;
+    static constexpr int DKV_WAVES = !TWO ? 1 : DP <= 64 ? 3 : 2;
+    static constexpr int FORWARD_LDS = std::max(4 * Image<T, DP, FORWARD_KEYS>::BYTES, Pass<T, DP>::SCRATCH);
+    static constexpr int DQ_LDS = std::max(4 * Image<T, DP, DQ_KEYS>::BYTES, Pass<T, DP>::SCRATCH);
+    static constexpr int DKV_LDS =
+        std::max(4 * Image<T, DP, QUERIES>::BYTES + 4 * QUERIES * 4 + (VL ? Image<T, DP, ROWS>::BYTES : 0), Pass<float, DP>::SCRATCH);
+    static constexpr auto forward = &attention_forward_kernel<T, DP, FORWARD_KEYS, FORWARD_WAVES>;
+    static constexpr auto dq = &attention_dq_kernel<T, DP, DQ_KEYS, DQ_WAVES>;
     static constexpr auto dkv = &attention_dkv_kernel<T, DP, QUERIES, VL, DKV_WAVES>;
 };
 
@@ -765,7 +807,7 @@ bool configure() {
     auto set = [](auto f, int bytes) {
         return hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
     };
-    return set(S::forward, S::KEY_LDS) && set(S::dq, S::KEY_LDS) && set(S::dkv, S::QUERY_LDS);
+    return set(S::forward, S::FORWARD_LDS) && set(S::dq, S::DQ_LDS) && set(S::dkv, S::DKV_LDS);
 }
 
 // One-time kernel attribute set-up, thread-safe.
@@ -786,10 +828,10 @@ int launch_width(Args& a, bool backward, hipStream_t stream) {
     const int64_t round = XCDS * a.chunk, slots = (static_cast<int64_t>(a.slots) * (a.heads / a.group) + round - 1) / round * round;
     const unsigned items = static_cast<unsigned>(slots * a.group);
     if (!backward) {
-        S::forward<<<items, THREADS, S::KEY_LDS, stream>>>(a);
+        S::forward<<<items, THREADS, S::FORWARD_LDS, stream>>>(a);
     } else {
-        S::dq<<<items, THREADS, S::KEY_LDS, stream>>>(a);
-        S::dkv<<<static_cast<unsigned>(slots * a.parts), THREADS, S::QUERY_LDS, stream>>>(a);
+        S::dq<<<items, THREADS, S::DQ_LDS, stream>>>(a);
+        S::dkv<<<static_cast<unsigned>(slots * a.parts), THREADS, S::DKV_LDS, stream>>>(a);
         if (a.parts > 1) {
             const int64_t threads = a.rows * (a.heads / a.group) * (a.width / 4);
             attention_join_kernel<T><<<static_cast<unsigned>((threads + THREADS - 1) / THREADS), THREADS, 0, stream>>>(a);
@@ -810,7 +852,7 @@ int64_t tile_slots(int64_t sequences, int64_t length, int64_t rows, bool packed)
     return packed ? rows / ROWS + sequences + 1 : sequences * ((length + ROWS - 1) / ROWS);
 }
 
-constexpr int64_t MAX_PARTS = 4;
+constexpr int64_t MAX_PARTS = 4, RESIDENT = 512;   // (two workgroups on each of 256 compute units)
 
 int64_t delta_bytes(int64_t rows, int64_t heads) { return (rows * heads * 4 + 15) / 16 * 16; }
 
@@ -865,13 +907,34 @@ int fill(Args& a, int dtype, int64_t sequences, int64_t length, int64_t rows, in
 
 extern "C" {
 
+int64_t kf_attention_order_bytes(int64_t sequences, int64_t rows, int64_t heads) {
+    if (sequences <= 0 || rows <= 0 || heads <= 0) return 0;
+    const int64_t slots = tile_slots(sequences, 0, rows, true);
+    return slots <= MAX_ORDERED && slots * heads > RESIDENT ? slots * 4 : 0;
+}
+
+int kf_attention_order(int32_t* order, const int32_t* offsets, int64_t sequences, int64_t rows, int causal, void* stream) {
+    if (order == nullptr || offsets == nullptr || sequences <= 0 || rows <= 0 || tile_slots(sequences, 0, rows, true) > MAX_ORDERED)
+        return KF_ERR_INVALID_ARGUMENT;
+    Args a = {};
+    a.offsets = offsets;
+    a.rows = rows;
+    a.sequences = static_cast<int>(sequences);
+    a.causal = causal != 0;
+    a.slots = static_cast<int>(tile_slots(sequences, 0, rows, true));
+    attention_order_kernel<<<1, 1024, 0, reinterpret_cast<hipStream_t>(stream)>>>(a, order);
+    return hipGetLastError() == hipSuccess ? KF_OK : KF_ERR_LAUNCH_FAILED;
+}
+
 int kf_attention_forward(const kf_heads_view* out, float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v, int dtype,
                          int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width, const int32_t* lengths,
-                         const int32_t* offsets, int causal, float scale, void* stream) {
+                         const int32_t* offsets, const int32_t* order, int causal, float scale, void* stream) {
     Args a = {};
     if (int s = fill(a, dtype, sequences, length, rows, heads, kv_heads, width, lengths, offsets, causal, scale)) return s;
     const int64_t per = dtype == KF_BF16 ? 8 : 4;
     if (!usable(out, per, width) || !usable(q, per, width) || !usable(k, per, width) || !usable(v, per, width)) return KF_ERR_INVALID_ARGUMENT;
+    if (order != nullptr && offsets == nullptr) return KF_ERR_INVALID_ARGUMENT;
+    a.order = order;
     if (int s = configure_kernels()) return s;
     a.q = tensor_of(q); a.k = tensor_of(k); a.v = tensor_of(v); a.o = tensor_of(out);
     a.lse = lse;
@@ -889,7 +952,7 @@ int64_t kf_attention_backward_workspace_bytes(int64_t sequences, int64_t length,
 int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, const kf_heads_view* dv, const kf_heads_view* grad, const kf_heads_view* out,
                           const float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v, int dtype, int64_t sequences,
                           int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width, const int32_t* lengths, const int32_t* offsets,
-                          int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+                          const int32_t* order, int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
     Args a = {};
     if (int s = fill(a, dtype, sequences, length, rows, heads, kv_heads, width, lengths, offsets, causal, scale)) return s;
     const int64_t per = dtype == KF_BF16 ? 8 : 4;
@@ -900,6 +963,8 @@ int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, cons
     if (workspace == nullptr ||
         workspace_bytes < kf_attention_backward_workspace_bytes(sequences, length, rows, heads, kv_heads, width, offsets != nullptr, causal))
         return KF_ERR_WORKSPACE_TOO_SMALL;
+    if (order != nullptr && offsets == nullptr) return KF_ERR_INVALID_ARGUMENT;
+    a.order = order;
     if (int s = configure_kernels()) return s;
     a.q = tensor_of(q); a.k = tensor_of(k); a.v = tensor_of(v); a.o = tensor_of(out); a.g = tensor_of(grad);
     a.dq = tensor_of(dq); a.dk = tensor_of(dk); a.dv = tensor_of(dv);

@@ -148,22 +148,34 @@ Tensor row_counts(const Tensor& t, int64_t most) {
     return (t.scalar_type() == at::kInt ? t : t.clamp(0, most).to(at::kInt)).contiguous();
 }
 
-Tensor attention_forward(const AttentionCall& c, Tensor q, Tensor k, Tensor v, const Tensor& lengths, const Tensor& offsets, Tensor* lse) {
+// the order a packed batch is best worked on in, or an undefined tensor
+Tensor work_order(const AttentionCall& c, const Tensor& starts) {
+    const int64_t bytes = starts.defined() ? kf_attention_order_bytes(c.sequences, c.rows, c.heads) : 0;
+    if (bytes == 0) return Tensor();
+    Tensor order = at::empty({bytes / 4}, starts.options());
+    check(kf_attention_order(order.data_ptr<int32_t>(), starts.data_ptr<int32_t>(), c.sequences, c.rows, c.causal, stream_of(starts)), "kf_attention_order");
+    return order;
+}
+
+Tensor attention_forward(const AttentionCall& c, Tensor q, Tensor k, Tensor v, const Tensor& lengths, const Tensor& offsets, Tensor* lse, Tensor* order_out) {
     Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
     if (lse) *lse = at::empty({c.heads, c.rows}, q.options().dtype(at::kFloat));
     if (c.empty()) return out.zero_();
     const c10::DeviceGuard guard(q.device());
     q = heads_operand(q); k = heads_operand(k); v = heads_operand(v);
     const Tensor counts = row_counts(lengths, c.length), starts = row_counts(offsets, c.rows);
+    const Tensor order = work_order(c, starts);
+    if (order_out) *order_out = order;
     const kf_heads_view vo = view(out), vq = view(q), vk = view(k), vv = view(v);
     check(kf_attention_forward(&vo, lse ? lse->data_ptr<float>() : nullptr, &vq, &vk, &vv, c.dtype, c.sequences, c.length, c.rows, c.heads, c.kv_heads, c.width,
-                               static_cast<const int32_t*>(pointer(counts)), static_cast<const int32_t*>(pointer(starts)), c.causal, c.scale, stream_of(q)),
+                               static_cast<const int32_t*>(pointer(counts)), static_cast<const int32_t*>(pointer(starts)),
+                               static_cast<const int32_t*>(pointer(order)), c.causal, c.scale, stream_of(q)),
           "kf_attention_forward");
     return out;
 }
 
 variable_list attention_backward(const AttentionCall& c, Tensor grad, Tensor out, const Tensor& lse, Tensor q, Tensor k, Tensor v, const Tensor& lengths,
-                                 const Tensor& offsets) {
+                                 const Tensor& offsets, const Tensor& order) {
     const auto plain = q.options().memory_format(at::MemoryFormat::Contiguous);
     Tensor dq = at::empty(q.sizes(), plain), dk = at::empty(k.sizes(), plain), dv = at::empty(v.sizes(), plain);
     if (c.empty()) return {dq.zero_(), dk.zero_(), dv.zero_()};
@@ -174,8 +186,8 @@ variable_list attention_backward(const AttentionCall& c, Tensor grad, Tensor out
     const Tensor workspace = at::empty({bytes}, q.options().dtype(at::kByte));
     const kf_heads_view vdq = view(dq), vdk = view(dk), vdv = view(dv), vg = view(grad), vo = view(out), vq = view(q), vk = view(k), vv = view(v);
     check(kf_attention_backward(&vdq, &vdk, &vdv, &vg, &vo, lse.data_ptr<float>(), &vq, &vk, &vv, c.dtype, c.sequences, c.length, c.rows, c.heads, c.kv_heads,
-                                c.width, static_cast<const int32_t*>(pointer(counts)), static_cast<const int32_t*>(pointer(starts)), c.causal, c.scale,
-                                workspace.data_ptr(), bytes, stream_of(q)),
+                                c.width, static_cast<const int32_t*>(pointer(counts)), static_cast<const int32_t*>(pointer(starts)),
+                                static_cast<const int32_t*>(pointer(order)), c.causal, c.scale, workspace.data_ptr(), bytes, stream_of(q)),
           "kf_attention_backward");
     return {dq, dk, dv};
 }
@@ -184,9 +196,9 @@ struct Attention : torch::autograd::Function<Attention> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& lengths_,
                           const std::optional<Tensor>& offsets_, bool causal, double scale) {
         const Tensor lengths = given(lengths_), offsets = given(offsets_);
-        Tensor lse;
-        const Tensor out = attention_forward(attention_call(q, k, v, lengths, offsets, causal, scale), q, k, v, lengths, offsets, &lse);
-        ctx->save_for_backward({q, k, v, out, lse, lengths, offsets});
+        Tensor lse, order;
+        const Tensor out = attention_forward(attention_call(q, k, v, lengths, offsets, causal, scale), q, k, v, lengths, offsets, &lse, &order);
+        ctx->save_for_backward({q, k, v, out, lse, lengths, offsets, order});
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["scale"] = scale;
         return out;
@@ -197,7 +209,7 @@ struct Attention : torch::autograd::Function<Attention> {
         const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &lengths = saved[5], &offsets = saved[6];
         if (!grads[0].defined()) return variable_list(7);
         const AttentionCall c = attention_call(q, k, v, lengths, offsets, ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
-        variable_list d = attention_backward(c, grads[0], saved[3], saved[4], q, k, v, lengths, offsets);
+        variable_list d = attention_backward(c, grads[0], saved[3], saved[4], q, k, v, lengths, offsets, saved[7]);
         d.resize(7);
         return d;
     }
@@ -217,7 +229,7 @@ Tensor attention(Tensor q, Tensor k, Tensor v, bool causal, const std::optional<
     }
     Tensor out;
     if (wants_graph({&q, &k, &v})) out = Attention::apply(q, k, v, lengths_, offsets_, causal, by);
-    else out = attention_forward(pad ? attention_call(q, k, v, lengths, offsets, causal, by) : c, q, k, v, lengths, offsets, nullptr);
+    else out = attention_forward(pad ? attention_call(q, k, v, lengths, offsets, causal, by) : c, q, k, v, lengths, offsets, nullptr, nullptr);
     return pad ? out.narrow(-1, 0, c.width) : out;
 }
 

@@ -89,23 +89,29 @@ def test_c_entries_refuse_without_touching_memory():
     INVALID, DTYPE, WORKSPACE = -1, -2, -4
 
     def forward(out=ok, q=ok, k=ok, v=ok, dtype=nat.KF_BF16, sequences=1, length=4, rows=4, heads=2, kv_heads=2, width=64, lengths=None,
-                offsets=None, scale=1.0):
-        return lib.kf_attention_forward(out, None, q, k, v, dtype, sequences, length, rows, heads, kv_heads, width, lengths, offsets, 1, scale, None)
+                offsets=None, order=None, scale=1.0):
+        return lib.kf_attention_forward(out, None, q, k, v, dtype, sequences, length, rows, heads, kv_heads, width, lengths, offsets, order, 1, scale, None)
 
     assert forward(dtype=nat.KF_F16) == DTYPE
     for bad in (dict(width=136), dict(width=0), dict(width=60), dict(heads=3), dict(kv_heads=0), dict(rows=5), dict(length=0), dict(sequences=0),
-                dict(scale=0.0), dict(scale=float("nan")), dict(lengths=16, offsets=16), dict(rows=1 << 31, length=1 << 31),
+                dict(scale=0.0), dict(scale=float("nan")), dict(lengths=16, offsets=16), dict(order=16), dict(rows=1 << 31, length=1 << 31),
                 dict(sequences=1 << 40, length=1, rows=1 << 40), dict(q=view(pointer=(1 << 20) + 8)), dict(k=view(width=63)), dict(out=view(pointer=0)),
                 dict(heads=1 << 40, kv_heads=1)):
         assert forward(**bad) == INVALID, bad
 
     def backward(bytes_=4 * 2 * 4, workspace=1 << 20, lse=1 << 20, **kw):
         views = [kw.pop("dq", ok)] + [ok] * 4
-        return lib.kf_attention_backward(*views, lse, ok, ok, ok, nat.KF_BF16, 1, 4, kw.get("rows", 4), 2, 2, 64, None, None, 1, 1.0, workspace, bytes_, None)
+        return lib.kf_attention_backward(*views, lse, ok, ok, ok, nat.KF_BF16, 1, 4, kw.get("rows", 4), 2, 2, 64, None, None, None, 1, 1.0, workspace, bytes_, None)
 
     assert lib.kf_attention_backward_workspace_bytes(1, 4, 4, 2, 2, 64, 0, 1) == 4 * 2 * 4
     assert backward(bytes_=31) == WORKSPACE and backward(workspace=None) == WORKSPACE
     assert backward(lse=None) == INVALID and backward(dq=view(pointer=4)) == INVALID and backward(rows=3) == INVALID
+
+    assert lib.kf_attention_order_bytes(3, 100, 4) == 0            # everything fits the card at once
+    assert lib.kf_attention_order_bytes(24, 12011, 16) == 4 * (12011 // 128 + 25)
+    assert lib.kf_attention_order_bytes(1 << 20, 1 << 28, 8) == 0    # too many to order, and enough to even out
+    for bad in ((None, 16, 2, 8), (16, None, 2, 8), (16, 16, 0, 8), (16, 16, 2, 0), (16, 16, 1 << 20, 1 << 28)):
+        assert lib.kf_attention_order(*bad, 1, None) == INVALID, bad
 
     def norm(y=1 << 20, y_dtype=0, x=1 << 20, x_dtype=0, rows=2, width=8, stride=8, weight=None, w_dtype=0, eps=1e-5):
         return lib.kf_norm_forward(y, y_dtype, None, x, x_dtype, rows, width, stride, weight, None, w_dtype, 1, eps, None)

@@ -152,6 +152,25 @@ def test_attention_packed(functional, dtype, causal, lengths, tail):
     check_attention(functional, q, k, v, g, causal, spans, cu_seqlens=torch.tensor(bounds, dtype=torch.int32, device="cuda"))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_packed_in_order_of_cost(functional, causal):
+    """Enough work that the tiles are ordered: short documents in front of a long one, empty ones between, a tail; heads of a group."""
+    from kronfluence_amd import _native
+
+    lengths, tail = [3, 40, 0, 700, 129, 1, 0, 1500, 64], 20
+    total = sum(lengths) + tail
+    assert _native.lib().kf_attention_order_bytes(len(lengths), total, 32) > 0
+    q, g = make((total, 32, 32), BF16, 1), make((total, 32, 32), BF16, 4, 0.1)
+    k, v = make((total, 2, 32), BF16, 2), make((total, 2, 32), BF16, 3)
+    bounds = [0]
+    for n in lengths:
+        bounds.append(bounds[-1] + n)
+    spans = [(slice(a, b),) for a, b in zip(bounds, bounds[1:]) if b > a]
+    first = check_attention(functional, q, k, v, g, causal, spans, cu_seqlens=torch.tensor(bounds, dtype=torch.int32, device="cuda"))
+    again = check_attention(functional, q, k, v, g, causal, spans, cu_seqlens=torch.tensor(bounds, dtype=torch.int32, device="cuda"))
+    assert all(torch.equal(x, y) for x, y in zip(first, again))
+
+
 def test_attention_packed_is_the_padded_batch(functional):
     """The same sequences packed and padded: the same bits."""
     lengths = [130, 1, 64, 200]
