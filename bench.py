@@ -122,6 +122,32 @@ def resnet9() -> nn.Module:
     )
 
 
+# The transformer workloads' own attention and norms on this package's kernels (kronfluence_amd/functional.py) instead of torch's
+# (``--model-kernels``; off by default: the model is the user's).
+MODEL_KERNELS = False
+
+
+def _key_mask(mask):
+    """What :func:`_attend` takes for a [b, t] mask that is 1 at the real tokens of a row (the first ones): their counts for the package's
+    kernel, a mask over the keys for torch's."""
+    return mask.sum(dim=1) if MODEL_KERNELS and mask.is_cuda else mask[:, None, None, :].to(torch.bool)
+
+
+def _attend(q, k, v, causal: bool, key_mask=None):
+    """Attention of ``q`` [b, t, heads, width] over ``k`` / ``v`` [b, t, kv_heads, width] -> [b, t, heads * width]; padded keys are never
+    attended to."""
+    b, t, heads, _ = q.shape
+    if MODEL_KERNELS and q.is_cuda:
+        from kronfluence_amd import functional
+
+        return functional.attention(q, k, v, causal=causal, lengths=key_mask).reshape(b, t, -1)
+    q, k, v = (z.transpose(1, 2) for z in (q, k, v))
+    rep = heads // k.shape[1]
+    if rep > 1:
+        k, v = k.repeat_interleave(rep, dim=1), v.repeat_interleave(rep, dim=1)
+    return F.scaled_dot_product_attention(q, k, v, attn_mask=key_mask, is_causal=causal).transpose(1, 2).reshape(b, t, -1)
+
+
 class _GPT2Block(nn.Module):
     def __init__(self, width: int, heads: int) -> None:
         super().__init__()
@@ -135,9 +161,7 @@ class _GPT2Block(nn.Module):
     def forward(self, x):
         b, t, d = x.shape
         q, k, v = self.c_attn(self.ln_1(x)).split(d, dim=-1)
-        q, k, v = (z.reshape(b, t, self.heads, d // self.heads).transpose(1, 2) for z in (q, k, v))
-        y = F.scaled_dot_product_attention(q, k, v, is_causal=True).transpose(1, 2).reshape(b, t, d)
-        x = x + self.attn_proj(y)
+        x = x + self.attn_proj(_attend(*(z.reshape(b, t, self.heads, d // self.heads) for z in (q, k, v)), causal=True))
         return x + self.mlp_proj(F.gelu(self.c_fc(self.ln_2(x)), approximate="tanh"))
 
 
@@ -184,14 +208,12 @@ class _LlamaBlock(nn.Module):
         self.down_proj = nn.Linear(inter, width, bias=False)
 
     def forward(self, x):
-        b, t, d = x.shape
+        b, t, _ = x.shape
         h = self.input_norm(x)
-        q = self.q_proj(h).reshape(b, t, self.heads, self.head_dim).transpose(1, 2)
-        k = self.k_proj(h).reshape(b, t, self.kv_heads, self.head_dim).transpose(1, 2)
-        v = self.v_proj(h).reshape(b, t, self.kv_heads, self.head_dim).transpose(1, 2)
-        rep = self.heads // self.kv_heads
-        y = F.scaled_dot_product_attention(q, k.repeat_interleave(rep, dim=1), v.repeat_interleave(rep, dim=1), is_causal=True)
-        x = x + self.o_proj(y.transpose(1, 2).reshape(b, t, d))
+        q = self.q_proj(h).reshape(b, t, self.heads, self.head_dim)
+        k = self.k_proj(h).reshape(b, t, self.kv_heads, self.head_dim)
+        v = self.v_proj(h).reshape(b, t, self.kv_heads, self.head_dim)
+        x = x + self.o_proj(_attend(q, k, v, causal=True))
         h = self.post_norm(x)
         return x + self.down_proj(F.silu(self.gate_proj(h)) * self.up_proj(h))
 
@@ -236,9 +258,8 @@ class _BertLayer(nn.Module):
 
     def forward(self, x, key_mask):
         b, t, d = x.shape
-        q, k, v = (lin(x).reshape(b, t, self.heads, d // self.heads).transpose(1, 2) for lin in (self.query, self.key, self.value))
-        y = F.scaled_dot_product_attention(q, k, v, attn_mask=key_mask).transpose(1, 2).reshape(b, t, d)
-        x = self.ln_attn(x + self.attn_out(y))
+        q, k, v = (lin(x).reshape(b, t, self.heads, d // self.heads) for lin in (self.query, self.key, self.value))
+        x = self.ln_attn(x + self.attn_out(_attend(q, k, v, causal=False, key_mask=key_mask)))
         return self.ln_out(x + self.output(F.gelu(self.intermediate(x))))
 
 
@@ -261,7 +282,7 @@ class Bert(nn.Module):
         t = ids.shape[1]
         x = self.word(ids) + self.position(torch.arange(t, device=ids.device)) + self.kind.weight[0]
         x = self.ln_embed(x)
-        key_mask = mask[:, None, None, :].to(torch.bool)  # padded keys are never attended to
+        key_mask = _key_mask(mask)
         for layer in self.layers:
             x = layer(x, key_mask)
         return self.classifier(torch.tanh(self.pooler(x[:, 0])))
@@ -686,6 +707,10 @@ def run_workload(name: str, state, n_train: Optional[int], n_query: Optional[int
     raw_model = spec["model"]()
     task, make_data, oracle_loss, oracle_measure, oracle_mask, tracked = workload_parts(spec, raw_model)
     model = prepare_model(raw_model, task).to(dev)
+    if MODEL_KERNELS:
+        from kronfluence_amd.utils.model import apply_fused_norms
+
+        model = apply_fused_norms(model)
     train = make_data(spec, n_train, 1, dev)
     query = make_data(spec, n_query, 2, dev)
     if spec.get("channels_last") and spec["kind"] == "image":
@@ -971,6 +996,7 @@ def run_workload(name: str, state, n_train: Optional[int], n_query: Optional[int
                        "parallelism": f"train-shard-dp{world}",
                        **({"memory_format": "channels_last"} if spec.get("channels_last") and spec["kind"] == "image" else {}),
                        **({"model_batch_norm": "aten" if NATIVE_BATCH_NORM else "miopen"} if name == "resnet9" else {}),
+                       **({"model_kernels": "kronfluence_amd"} if MODEL_KERNELS else {}),
                        **({"warmup_n_train": min(warm_n_train, n_train)} if warm_n_train else {}),
                        **({"scaled_from": {"n_train": spec.get("full_n_train"), "n_query": spec.get("full_n_query", spec["n_query"])}}
                           if n_train < spec.get("full_n_train", 0) else {})},
@@ -1193,6 +1219,8 @@ def main() -> None:
                     "format -- MIOpen's bf16 convolution kernels are NHWC kernels; with NCHW tensors it transposes around each of them")
     ap.add_argument("--miopen-batchnorm", action="store_true", help="resnet9: the model's eval-mode batch norm on MIOpen's kernel again "
                     "(default: ATen's; see NATIVE_BATCH_NORM)")
+    ap.add_argument("--model-kernels", action="store_true", help="transformer workloads: the model's own attention and norms on "
+                    "kronfluence_amd.functional (see MODEL_KERNELS)")
     ap.add_argument("--phase-split", action="store_true", help="also report the step's query-phase / train-pass wall seconds (one more "
                     "device synchronisation per held-query window inside the timed region)")
     ap.add_argument("--no-miopen-find", action="store_true", help="leave torch.backends.cudnn.benchmark off (default: on -- MIOpen "
@@ -1214,6 +1242,9 @@ def main() -> None:
     if args.miopen_batchnorm:
         global NATIVE_BATCH_NORM
         NATIVE_BATCH_NORM = False
+    if args.model_kernels:
+        global MODEL_KERNELS
+        MODEL_KERNELS = True
     if not args.no_miopen_find:
         torch.backends.cudnn.benchmark = True
 

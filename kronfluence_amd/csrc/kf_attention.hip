@@ -446,7 +446,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
             sk.load(k.from(k0 + BK));
             sv.load(v.from(k0 + BK));
         }
-        if (!(a.causal && k0 > first + 31)) {   // (wave-uniform)
+        if (first < w.length && !(a.causal && k0 > first + 31)) {   // (wave-uniform)
             f32x16 s[BK / 32];
 #pragma unroll
             for (int b = 0; b < BK / 32; ++b) {
@@ -562,7 +562,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
             sk.load(k.from(k0 + BK));
             sv.load(v.from(k0 + BK));
         }
-        if (!(a.causal && k0 > first + 31)) {
+        if (first < w.length && !(a.causal && k0 > first + 31)) {
             const bool masked = k0 + BK > w.length || (a.causal && k0 + BK - 1 > first);
             const int visible = a.causal ? min(w.length, query + 1) : w.length;
 #pragma unroll
@@ -690,7 +690,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
         if (n + 1 < steps) load();
 #pragma unroll
         for (int b = 0; b < BQ / 32; ++b) {
-            if (a.causal && q0 + 32 * b + 32 <= first) continue;   // (wave-uniform)
+            if (first >= w.length || (a.causal && q0 + 32 * b + 32 <= first)) continue;   // (wave-uniform)
             // s; then dp beside p = 2^(c s - L); then dv beside ds = p (dp - D); then dk
             f32x16 s = {}, dp = {};
 #pragma unroll

@@ -128,3 +128,40 @@ def test_c_entries_refuse_without_touching_memory():
     assert norm_backward(dx=16, grad=None) == INVALID and norm_backward(dx=16, stats=None) == INVALID and norm_backward(dw=16, w_dtype=3) == DTYPE
     assert lib.kf_norm_backward_workspace_bytes(2, 8) >= 2 * 8 * 4
     assert ctypes.sizeof(nat.kf_heads_view) == 32
+
+
+def test_apply_fused_norms_shares_parameters_and_names():
+    from torch import nn
+
+    from kronfluence_amd.module.norm import FusedLayerNorm, FusedRMSNorm
+    from kronfluence_amd.utils.model import apply_fused_norms
+
+    class Own(nn.LayerNorm):
+        def forward(self, x):
+            return super().forward(x) + 1
+
+    class Model(nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.a, self.b, self.c = nn.LayerNorm(8, eps=1e-3), nn.RMSNorm(8), nn.LayerNorm(8, bias=False)
+            self.d, self.e, self.f = nn.LayerNorm(8, elementwise_affine=False), nn.LayerNorm((2, 8)), Own(8)
+            self.again, self.hooked = self.a, nn.LayerNorm(8)
+            self.nest = nn.Sequential(nn.Linear(8, 8), nn.RMSNorm(8, eps=1e-4))
+
+    model = Model()
+    model.hooked.register_forward_hook(lambda *_: None)
+    model.b.weight.requires_grad_(False)
+    before, kept = dict(model.named_parameters()), list(model.state_dict())
+    model.eval()
+    assert apply_fused_norms(model) is model
+    after = dict(model.named_parameters())
+    assert set(after) == set(before) and all(after[name] is before[name] for name in before) and list(model.state_dict()) == kept
+    assert type(model.a) is type(model.again) is type(model.c) is type(model.d) is FusedLayerNorm and model.a.eps == 1e-3
+    assert type(model.b) is type(model.nest[1]) is FusedRMSNorm and model.b.eps is None and model.nest[1].eps == 1e-4
+    assert type(model.e) is type(model.hooked) is nn.LayerNorm and type(model.f) is Own and not model.a.training
+    assert model.c.bias is None and model.d.weight is None
+    assert type(apply_fused_norms(nn.LayerNorm(4))) is FusedLayerNorm
+    apply_fused_norms(model)
+    assert type(model.a) is FusedLayerNorm and list(model.state_dict()) == kept
+    with pytest.raises(nat.KfError, match="lives on cpu"):   # no CPU path, as everywhere in the package
+        model.a(torch.zeros(2, 8))
