@@ -13,8 +13,12 @@
 //     dK / dV:      S   = Q K^T  (lane = key,  registers = queries) ->  dV^T += dO^T P,   dK^T += Q^T dS
 // The accumulator layout (register r of lane half h holds row 8 (r / 4) + 4 h + r % 4) IS the operand layout of the second product
 // once the contraction index is permuted the same way in its other operand, so P and dS go from accumulator to operand by
-// conversion alone, with no cross-lane traffic; the other operand is read from LDS column-wise (ds_read_b64_tr_b16 for 2-byte
-// types, plain 4-byte reads for fp32).  fp32 runs on v_mfma_f32_32x32x2_f32 with the same structure: exact fp32 products.
+// conversion alone, with no cross-lane traffic; the other operand is read from LDS column-wise (ds_read_b64_tr_b16).
+//
+// fp32 runs on the same bf16 instructions: every value is split into three bf16 parts, exactly, and a product is six products of parts
+// (struct Split) -- 6/16 of the time of v_mfma_f32_32x32x2_f32 at fp32's accuracy.  Measured against that instruction in the same
+// kernels: 64 x 256 x 12 heads x 64, forward 131 to 84 us, backward 470 to 325; 2 x 2048 x 16 x 128 causal, 334 to 223 and 1129 to 817.
+// Finite values from 3.39e38 on (their first part rounds to infinity) act as infinities, parts below 2^-126 as 0.
 //
 // Roundings to fewer bits than 32: P and dS are rounded to bf16 as operands of their second product when the inputs are bf16 (one
 // rounding of half a step, 2^-9 relative, per term of a sum whose inputs carry the same rounding), and the outputs once at the end.
@@ -25,6 +29,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "../../include/kronfluence_hip.h"
 
@@ -66,13 +71,18 @@ struct Args {
 };
 
 // ---- element types ---------------------------------------------------------------------------------------------------------
+// fp32 whose products are sums of bf16 products: every value is exactly the sum of three bf16 parts (8 + 8 + 8 bits), and of the nine
+// products of parts the six greater ones are taken -- the three left out are below 2^-26 of the whole, a quarter of fp32's half step.
+struct Split { float value; };
+
 template <class T>
 struct Type;
+template <class T> constexpr int PARTS = std::is_same_v<T, Split> ? 3 : 1;    // bf16 images of a tile in LDS
 
 template <>
 struct Type<__bf16> {
+    typedef __bf16 Memory;
     typedef bf16x8 Frag;                       // 16 bytes: the lane's part of a 16-deep contraction slab
-    static constexpr int SLAB_REGS = 8;        // accumulator registers that make one operand of the second product
     static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ Frag from_acc(const f32x16& s, int slab) {
         Frag f;
@@ -92,76 +102,107 @@ struct Type<__bf16> {
 };
 
 template <>
-struct Type<float> {
-    typedef f32x4 Frag;                        // an 8-deep slab: four instructions of depth 2, one component each
-    static constexpr int SLAB_REGS = 4;
-    static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
-        return c;
-    }
-    static __device__ __forceinline__ Frag from_acc(const f32x16& s, int slab) {
-        Frag f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = s[4 * slab + i];
-        return f;
-    }
+struct Type<float> {                           // (the partial sums of the dk / dv kernel)
     static __device__ __forceinline__ void store4(void* p, float a, float b, float c, float d) {
         f32x4 v = {a, b, c, d};
         *reinterpret_cast<f32x4*>(p) = v;
     }
-    static __device__ __forceinline__ float dot(Frag a, Frag b, float acc) {
+};
+
+template <>
+struct Type<Split> {
+    typedef float Memory;
+    struct Frag { bf16x8 part[3]; };           // a 16-deep slab; the parts from the greatest on
+    static __device__ __forceinline__ f32x16 mma(const Frag& a, const Frag& b, f32x16 c) {
+        c = Type<__bf16>::mma(a.part[2], b.part[0], c);
+        c = Type<__bf16>::mma(a.part[0], b.part[2], c);
+        c = Type<__bf16>::mma(a.part[1], b.part[1], c);
+        c = Type<__bf16>::mma(a.part[1], b.part[0], c);
+        c = Type<__bf16>::mma(a.part[0], b.part[1], c);
+        return Type<__bf16>::mma(a.part[0], b.part[0], c);
+    }
+    // x = part 0 + part 1 + part 2 exactly: each part is the nearest bf16 to what the ones before leave, and the differences are exact
+    template <class Values>
+    static __device__ __forceinline__ Frag split(const Values& x, int first) {
+        Frag f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc = fmaf(a[i], b[i], acc);
+        for (int i = 0; i < 8; ++i) {
+            f.part[0][i] = static_cast<__bf16>(x[first + i]);
+            const float rest = x[first + i] - static_cast<float>(f.part[0][i]);
+            f.part[1][i] = static_cast<__bf16>(rest);
+            f.part[2][i] = static_cast<__bf16>(rest - static_cast<float>(f.part[1][i]));
+        }
+        return f;
+    }
+    static __device__ __forceinline__ Frag from_acc(const f32x16& s, int slab) { return split(s, 8 * slab); }
+    static __device__ __forceinline__ Frag from_memory(u32x4 low, u32x4 high) {
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = __uint_as_float(low[i]);
+            x[4 + i] = __uint_as_float(high[i]);
+        }
+        return split(x, 0);
+    }
+    static __device__ __forceinline__ void store4(void* p, float a, float b, float c, float d) { Type<float>::store4(p, a, b, c, d); }
+    static __device__ __forceinline__ float dot(const Frag& a, const Frag& b, float acc) {
+        auto value = [](const Frag& f, int i) {
+            return static_cast<float>(f.part[2][i]) + static_cast<float>(f.part[1][i]) + static_cast<float>(f.part[0][i]);   // exact again
+        };
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc = fmaf(value(a, i), value(b, i), acc);
         return acc;
     }
 };
 
 // ---- an operand tile of N rows in LDS: [64-byte column block][row][4 chunks of 16 bytes], the chunk XORed with (row / 4) % 4 -----
-// Two kinds of reads meet the same image.  Row fragments: 32 consecutive rows, one chunk each -- any 16 consecutive rows fall into the
-// 16 different slots of the 256-byte bank space.  Transposed reads of 2-byte types: 4 consecutive rows, 64 bytes each -- 256
+// (fp32: one such image per part).  Two kinds of reads meet the same image.  Row fragments: 32 consecutive rows, one chunk each -- any 16 consecutive rows fall into the
+// 16 different slots of the 256-byte bank space.  Transposed reads: 4 consecutive rows, 64 bytes each -- 256
 // consecutive bytes.  The address of any other slab, block or half differs by a constant of the instruction, but for one bit that
 // changes by exclusive or: a lane keeps one register per kind of read.
 template <class T, int DP, int N>
 struct Image {
-    static constexpr int CHUNKS = DP * static_cast<int>(sizeof(T)) / 16, SLABS = CHUNKS / 2;
-    static constexpr int BLOCK = N * 64, BYTES = CHUNKS / 4 * BLOCK;
+    static constexpr int CHUNKS = DP / 8, SLABS = CHUNKS / 2;
+    static constexpr int BLOCK = N * 64, PART = CHUNKS / 4 * BLOCK, BYTES = PARTS<T> * PART;
 };
 
 template <class T, int DP, int N>
 struct Reader {
     typedef Image<T, DP, N> Img;
-    typedef typename Type<T>::Frag Frag;
-    typedef __attribute__((address_space(3))) const Frag* FragPointer;
+    typedef __attribute__((address_space(3))) const bf16x8* FragPointer;
     uint32_t row, column;
     __device__ __forceinline__ explicit Reader(int lane) {
         const int r = lane & 31, g = lane >> 4, s = lane & 15;
         row = r * 64 + (((lane >> 5) ^ (r >> 2)) & 3) * 16;
-        if constexpr (sizeof(T) == 2) column = (4 * (g >> 1) + (s >> 2)) * 64 + ((2 * (g & 1) + ((s & 3) >> 1)) ^ (g >> 1)) * 16 + (s & 1) * 8;
-        else column = (r >> 4) * Img::BLOCK + 4 * (lane >> 5) * 64 + ((s >> 2) ^ (lane >> 5)) * 16 + (s & 3) * 4;
+        column = (4 * (g >> 1) + (s >> 2)) * 64 + ((2 * (g & 1) + ((s & 3) >> 1)) ^ (g >> 1)) * 16 + (s & 1) * 8;
     }
     // rows row0 .. row0 + 31 of the tile at LDS address `tile` (row0 a multiple of 32), contraction slab `slab`
-    __device__ __forceinline__ Frag rows(uint32_t tile, int row0, int slab) const {
+    __device__ __forceinline__ bf16x8 rows(uint32_t tile, int row0, int slab) const {
         return *reinterpret_cast<FragPointer>(((tile + row) ^ (slab % 2 * 32)) + slab / 2 * Img::BLOCK + row0 * 64);
     }
-    // the TRANSPOSED tile: columns 32 t .. 32 t + 31 as rows, contraction over the tile rows that registers [SLAB_REGS * slab,
-    // SLAB_REGS * (slab + 1)) of an accumulator over rows row0 .. row0 + 31 stand for
+    // the TRANSPOSED tile: columns 32 t .. 32 t + 31 as rows, contraction over the tile rows that registers [8 slab, 8 (slab + 1)) of an
+    // accumulator over rows row0 .. row0 + 31 stand for
+    __device__ __forceinline__ bf16x8 columns(uint32_t tile, int row0, int slab, int t) const {
+        union { s16x4 h[2]; bf16x8 v; } u;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            u.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4*>(
+                ((tile + column) ^ (32 * i)) + t * Img::BLOCK + (row0 + 16 * slab + 8 * i) * 64));
+        return u.v;
+    }
+};
+
+template <int DP, int N>
+struct Reader<Split, DP, N> : Reader<__bf16, DP, N> {   // one image per part
+    typedef Reader<__bf16, DP, N> Base;
+    typedef typename Type<Split>::Frag Frag;
+    static constexpr int PART = Image<Split, DP, N>::PART;
+    using Base::Base;
+    __device__ __forceinline__ Frag rows(uint32_t tile, int row0, int slab) const {
+        return Frag{{Base::rows(tile, row0, slab), Base::rows(tile + PART, row0, slab), Base::rows(tile + 2 * PART, row0, slab)}};
+    }
     __device__ __forceinline__ Frag columns(uint32_t tile, int row0, int slab, int t) const {
-        if constexpr (sizeof(T) == 2) {
-            union { s16x4 h[2]; bf16x8 v; } u;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                u.h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4*>(
-                    ((tile + column) ^ (32 * i)) + t * Img::BLOCK + (row0 + 16 * slab + 8 * i) * 64));
-            return u.v;
-        } else {
-            f32x4 v;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                v[i] = *reinterpret_cast<__attribute__((address_space(3))) const float*>(((tile + column) ^ (slab % 2 * 32)) + 2 * t * Img::BLOCK +
-                                                                                        (row0 + 8 * slab + i) * 64);
-            return v;
-        }
+        return Frag{{Base::columns(tile, row0, slab, t), Base::columns(tile + PART, row0, slab, t), Base::columns(tile + 2 * PART, row0, slab, t)}};
     }
 };
 
@@ -210,6 +251,41 @@ struct Stage {
 #pragma unroll
         for (int i = 0; i < PER; ++i)
             if (ALL % THREADS == 0 || i + 1 < PER || to + i * 16 * THREADS < Img::BYTES) *reinterpret_cast<u32x4*>(tile + to + i * 16 * THREADS) = r[i];
+    }
+};
+
+// fp32 rows into the images of their parts: 8 values a chunk.
+template <int DP, int N>
+struct Stage<Split, DP, N> {
+    typedef Image<Split, DP, N> Img;
+    static constexpr int ALL = Img::PART / 16, PER = (ALL + THREADS - 1) / THREADS;
+    u32x4 r[PER][2];
+    uint32_t at[PER][2];
+    int to;
+    __device__ __forceinline__ Stage(int64_t token, int width, int tid) {
+        to = (tid * 16) ^ ((tid >> 4 & 3) * 16);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int n = tid + i * THREADS, row = n / 4 % N, chunk = n / 4 / N * 4 + n % 4;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                at[i][j] = chunk * 32 + j * 16 < width ? static_cast<uint32_t>(row * static_cast<int>(token) + chunk * 32 + j * 16) : NO_COLUMN;
+        }
+    }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rows) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) r[i][j] = __builtin_amdgcn_raw_buffer_load_b128(rows, at[i][j], 0, 0);
+    }
+    __device__ __forceinline__ void store(char* tile) const {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (ALL % THREADS != 0 && i + 1 == PER && to + i * 16 * THREADS >= Img::PART) continue;
+            const Type<Split>::Frag f = Type<Split>::from_memory(r[i][0], r[i][1]);
+#pragma unroll
+            for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x8*>(tile + p * Img::PART + to + i * 16 * THREADS) = f.part[p];
+        }
     }
 };
 
@@ -345,6 +421,24 @@ struct Held {
     }
 };
 
+template <int DP>
+struct Held<Split, DP> {
+    static constexpr int SLABS = DP / 16;
+    typename Type<Split>::Frag f[SLABS];
+    __device__ __forceinline__ void load(const Rows& rows, int row0, int lane) {
+        const __amdgpu_buffer_rsrc_t from = rows.from(row0);
+        auto piece = [&](int byte) {
+            return __builtin_amdgcn_raw_buffer_load_b128(
+                from, byte < rows.width ? static_cast<uint32_t>((lane & 31) * static_cast<int>(rows.token) + byte) : NO_COLUMN, 0, 0);
+        };
+#pragma unroll
+        for (int s = 0; s < SLABS; ++s) {
+            const int c = (2 * s + (lane >> 5)) * 32;
+            f[s] = Type<Split>::from_memory(piece(c), piece(c + 16));
+        }
+    }
+};
+
 // acc^T (lane = row, registers = columns d) times the lane's `factor` -> rows first .. first + 31 of memory, through LDS: a lane holds
 // four columns of a row at a time, and stores of 8 bytes per row cost as much as all the rest of a short sequence (256 x 128 x 12 x 64
 // bf16 forward: 43 us, 22 without the stores).  Every wave uses its own piece of `scratch`; the workgroup is done with its tiles.
@@ -390,16 +484,12 @@ __device__ __forceinline__ void zero_rows(T* base, int64_t token, int row0, int 
 }
 
 // A read of a matrix instruction's result needs wait states that the compiler inserts; where a branch stands between the two it has
-// left some out on one of the paths (fp32: the first read behind the branch saw row 15 of the tile before it was written).  Put between
-// the last matrix instruction and such a branch; tests/test_wait_states_cpu.py follows every path of the built code and says where.
-template <class T, bool TWO_BYTE_TYPES = false>
+// left some out on one of the paths (the first read behind the branch then sees the last row of the tile before it was written).  Put
+// between the last matrix instruction and such a branch; tests/test_wait_states_cpu.py follows every path of the built code and says where.
 __device__ __forceinline__ void settle() {
-    if constexpr (sizeof(T) == 4 || TWO_BYTE_TYPES) {
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (sizeof(T) == 4) asm volatile("s_nop 15\n\ts_nop 3");
-        else asm volatile("s_nop 11");
-        __builtin_amdgcn_sched_barrier(0);
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 11");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
@@ -407,7 +497,7 @@ template <class T, int DP, int BK, int WAVES>
 __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const Args a) {
     typedef Image<T, DP, BK> Img;
     typedef typename Type<T>::Frag Frag;
-    constexpr int TILE = Img::BYTES, SECOND = 16 / Type<T>::SLAB_REGS;
+    constexpr int TILE = Img::BYTES;
     extern __shared__ __align__(16) char lds[];   // [2][k tile, v tile]
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -454,7 +544,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
 #pragma unroll
                 for (int i = 0; i < Img::SLABS; ++i) s[b] = Type<T>::mma(read.rows(kt, 32 * b, i), q.f[i], s[b]);
             }
-            settle<T, true>();
+            settle();
             if (k0 + BK > w.length || (a.causal && k0 + BK - 1 > first)) {
                 const int visible = a.causal ? min(w.length, query + 1) : w.length;
 #pragma unroll
@@ -488,14 +578,13 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
                     sum += s[b][r];
                 }
 #pragma unroll
-                for (int i = 0; i < SECOND; ++i) {
+                for (int i = 0; i < 2; ++i) {
                     const Frag p = Type<T>::from_acc(s[b], i);
 #pragma unroll
                     for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mma(read.columns(vt, 32 * b, i, d), p, acc[d]);
                 }
             }
         }
-        settle<T>();
         if (t + 1 < tiles) {
             sk.store(lds + ((t + 1) & 1) * 2 * TILE);
             sv.store(lds + ((t + 1) & 1) * 2 * TILE + TILE);
@@ -513,7 +602,7 @@ template <class T, int DP, int BK, int WAVES>
 __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args a) {
     typedef Image<T, DP, BK> Img;
     typedef typename Type<T>::Frag Frag;
-    constexpr int TILE = Img::BYTES, SECOND = 16 / Type<T>::SLAB_REGS;
+    constexpr int TILE = Img::BYTES;
     extern __shared__ __align__(16) char lds[];   // [2][k tile, v tile]
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -574,21 +663,19 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
                 for (int i = 0; i < Img::SLABS; ++i) dp = Type<T>::mma(read.rows(vt, 32 * b, i), g.f[i], dp);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) * (dp[r] - delta);
-                settle<T>();
                 if (masked) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
                         if (k0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 >= visible) s[r] = 0.0f;
                 }
 #pragma unroll
-                for (int i = 0; i < SECOND; ++i) {
+                for (int i = 0; i < 2; ++i) {
                     const Frag ds = Type<T>::from_acc(s, i);
 #pragma unroll
                     for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mma(read.columns(kt, 32 * b, i, d), ds, acc[d]);
                 }
             }
         }
-        settle<T>();
         if (t + 1 < tiles) {
             sk.store(lds + ((t + 1) & 1) * 2 * TILE);
             sv.store(lds + ((t + 1) & 1) * 2 * TILE + TILE);
@@ -611,7 +698,7 @@ template <class T, int DP, int BQ, bool VL, int WAVES>
 __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Args a) {
     typedef Image<T, DP, BQ> Img;
     typedef typename Type<T>::Frag Frag;
-    constexpr int TILE = Img::BYTES, STAGE = 2 * TILE + 2 * BQ * 4, SECOND = 16 / Type<T>::SLAB_REGS;
+    constexpr int TILE = Img::BYTES, STAGE = 2 * TILE + 2 * BQ * 4;
     static_assert(STAGE % 64 == 0, "tiles start at multiples of 64 bytes");
     extern __shared__ __align__(16) char lds[];   // [2][q tile, g tile, L of its rows, D of its rows], with VL the workgroup's v rows
 
@@ -708,8 +795,8 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[4 * i + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * i + j], c, -l4[j]));
             }
-            settle<T>();
-            if ((a.causal && q0 + 32 * b < first + 31) || w.length == 1) {
+            // (Split: no branches inside the condition -- the compiler's count of wait states went wrong around one)
+            if (PARTS<T> == 3 ? ((a.causal & (q0 + 32 * b < first + 31)) | (w.length == 1)) : ((a.causal && q0 + 32 * b < first + 31) || w.length == 1)) {
                 const int hidden = a.causal ? key - q0 - 32 * b - 4 * half : -32;   // rows of the block in front of the key
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
@@ -718,7 +805,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
                 if (q0 + 32 * b + 4 * half == 0) dp[0] = rows_delta[0];
             }
 #pragma unroll
-            for (int i = 0; i < SECOND; ++i) {
+            for (int i = 0; i < 2; ++i) {
                 const Frag p = Type<T>::from_acc(s, i);
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) av[d] = Type<T>::mma(read.columns(gt, 32 * b, i, d), p, av[d]);
@@ -730,13 +817,12 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
                 for (int j = 0; j < 4; ++j) dp[4 * i + j] = s[4 * i + j] * (dp[4 * i + j] - d4[j]);
             }
 #pragma unroll
-            for (int i = 0; i < SECOND; ++i) {
+            for (int i = 0; i < 2; ++i) {
                 const Frag ds = Type<T>::from_acc(dp, i);
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) ak[d] = Type<T>::mma(read.columns(qt, 32 * b, i, d), ds, ak[d]);
             }
         }
-        settle<T>();
         if (n + 1 < steps) store(lds + ((n + 1) & 1) * STAGE);
     }
     __syncthreads();
@@ -788,10 +874,10 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(const Args a) {
 // Tile rows and waves per SIMD of each kernel.
 template <class T, int DP>
 struct Shape {
-    static constexpr bool TWO = sizeof(T) == 2, VL = TWO && (DP == 64 || DP > 96);
-    static constexpr int FORWARD_KEYS = TWO && DP <= 64 ? 64 : 32, DQ_KEYS = TWO && DP > 64 ? 64 : 32, QUERIES = TWO && DP <= 32 ? 64 : 32;
-    static constexpr int FORWARD_WAVES = !TWO ? 1 : DP <= 64 ? 4 : 3, DQ_WAVES = !TWO ? 1 : DP <= 64 ? 4 : 2;
-    static constexpr int DKV_WAVES = !TWO ? 1 : DP <= 64 ? 3 : 2;
+    static constexpr bool SPLIT = PARTS<T> == 3, VL = !SPLIT && (DP == 64 || DP > 96);
+    static constexpr int FORWARD_KEYS = !SPLIT && DP <= 64 ? 64 : 32, DQ_KEYS = !SPLIT && DP > 64 ? 64 : 32, QUERIES = !SPLIT && DP <= 32 ? 64 : 32;
+    static constexpr int FORWARD_WAVES = SPLIT ? (DP <= 64 ? 3 : 1) : DP <= 64 ? 4 : 3, DQ_WAVES = SPLIT ? (DP <= 64 ? 2 : 1) : DP <= 64 ? 4 : 2;
+    static constexpr int DKV_WAVES = SPLIT ? (DP <= 64 ? 2 : 1) : DP <= 64 ? 3 : 2;
     static constexpr int FORWARD_LDS = std::max(4 * Image<T, DP, FORWARD_KEYS>::BYTES, Pass<T, DP>::SCRATCH);
     static constexpr int DQ_LDS = std::max(4 * Image<T, DP, DQ_KEYS>::BYTES, Pass<T, DP>::SCRATCH);
     static constexpr int DKV_LDS =
@@ -815,8 +901,8 @@ int configure_kernels() {
     static std::once_flag flag;
     static int status = KF_OK;
     std::call_once(flag, [] {
-        if (!(configure<__bf16, 32>() && configure<__bf16, 64>() && configure<__bf16, 96>() && configure<__bf16, 128>() && configure<float, 32>() &&
-              configure<float, 64>() && configure<float, 96>() && configure<float, 128>()))
+        if (!(configure<__bf16, 32>() && configure<__bf16, 64>() && configure<__bf16, 96>() && configure<__bf16, 128>() && configure<Split, 32>() &&
+              configure<Split, 64>() && configure<Split, 96>() && configure<Split, 128>()))
             status = KF_ERR_LAUNCH_FAILED;
     });
     return status;
@@ -834,7 +920,7 @@ int launch_width(Args& a, bool backward, hipStream_t stream) {
         S::dkv<<<static_cast<unsigned>(slots * a.parts), THREADS, S::DKV_LDS, stream>>>(a);
         if (a.parts > 1) {
             const int64_t threads = a.rows * (a.heads / a.group) * (a.width / 4);
-            attention_join_kernel<T><<<static_cast<unsigned>((threads + THREADS - 1) / THREADS), THREADS, 0, stream>>>(a);
+            attention_join_kernel<typename Type<T>::Memory><<<static_cast<unsigned>((threads + THREADS - 1) / THREADS), THREADS, 0, stream>>>(a);
         }
     }
     return hipGetLastError() == hipSuccess ? KF_OK : KF_ERR_LAUNCH_FAILED;
@@ -939,7 +1025,7 @@ int kf_attention_forward(const kf_heads_view* out, float* lse, const kf_heads_vi
     a.q = tensor_of(q); a.k = tensor_of(k); a.v = tensor_of(v); a.o = tensor_of(out);
     a.lse = lse;
     const hipStream_t on = reinterpret_cast<hipStream_t>(stream);
-    return dtype == KF_BF16 ? launch_type<__bf16>(a, false, on) : launch_type<float>(a, false, on);
+    return dtype == KF_BF16 ? launch_type<__bf16>(a, false, on) : launch_type<Split>(a, false, on);
 }
 
 int64_t kf_attention_backward_workspace_bytes(int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width, int packed,
@@ -973,7 +1059,7 @@ int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, cons
     a.partial = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + delta_bytes(rows, heads));
     a.parts = static_cast<int>(dkv_parts(sequences, length, rows, heads, kv_heads, offsets != nullptr, causal));
     const hipStream_t on = reinterpret_cast<hipStream_t>(stream);
-    return dtype == KF_BF16 ? launch_type<__bf16>(a, true, on) : launch_type<float>(a, true, on);
+    return dtype == KF_BF16 ? launch_type<__bf16>(a, true, on) : launch_type<Split>(a, true, on);
 }
 
 }  // extern "C"
