@@ -334,10 +334,12 @@ __device__ __forceinline__ bool locate(const Args& a, int slot, bool last_first,
 // own: what reads the same k and v should go to one XCD, but no XCD may be left with the longest sequences.  Where (sequence, key /
 // value head) pairs of equal size are many, whole pairs are dealt to the XCDs (a.chunk = the tiles of a sequence), the heads of a
 // sequence one after the other (24 sequences of 29 to 233 tokens, 12 heads x 64 fp32: 210 us, 264 us with the sequences of a head one
-// after the other).  Otherwise single tiles are dealt, the heads of a tile one after
-// the other: with 1, 2, 4 or a multiple of 8 heads an XCD then sees the same heads in every tile.  The `members` query heads of a group
-// stay together.  False: nothing left (the grid is rounded up).
-constexpr int XCDS = 8;
+// after the other).  An XCD deals its workgroups to its compute units in turn, too, so the tiles of a pair -- of very different cost, if
+// causal -- are taken from another one on in every pair and every round of the compute units: without that a unit gets the same tile of
+// pair after pair (64 x 512 x 12 heads x 64 bf16 causal: dk / dv 121 us, 102 with it; dq 93 and 84; forward 70 and 63).
+// Otherwise single tiles are dealt, the heads of a tile one after the other: with 1, 2, 4 or a multiple of 8 heads an XCD then sees the
+// same heads in every tile.  The `members` query heads of a group stay together.  False: nothing left (the grid is rounded up).
+constexpr int XCDS = 8, CUS = 32;   // CUS: compute units of an XCD
 struct Item { int slot, kv_head, member; };
 __device__ __forceinline__ bool work_item(const Args& a, int members, Item& w) {
     const int kv_heads = a.heads / a.group;
@@ -345,7 +347,8 @@ __device__ __forceinline__ bool work_item(const Args& a, int members, Item& w) {
     const int64_t item = (n / chunk * XCDS + id % XCDS) * chunk + n % chunk, pair = item / members, unit = pair / a.chunk;
     w.member = static_cast<int>(item % members);
     w.kv_head = static_cast<int>(unit % kv_heads);
-    w.slot = static_cast<int>(unit / kv_heads * a.chunk + pair % a.chunk);
+    const int64_t round = n / chunk, turn = round + (chunk < CUS ? round * chunk / CUS : 0);
+    w.slot = static_cast<int>(unit / kv_heads * a.chunk + (pair + turn) % a.chunk);
     if (pair >= static_cast<int64_t>(a.slots) * kv_heads) return false;
     if (a.order) w.slot = a.order[w.slot];
     return true;
