@@ -130,7 +130,7 @@ MODEL_KERNELS = False
 def _key_mask(mask):
     """What :func:`_attend` takes for a [b, t] mask that is 1 at the real tokens of a row (the first ones): their counts for the package's
     kernel, a mask over the keys for torch's."""
-    return mask.sum(dim=1) if MODEL_KERNELS and mask.is_cuda else mask[:, None, None, :].to(torch.bool)
+    return mask.sum(dim=1, dtype=torch.int32) if MODEL_KERNELS and mask.is_cuda else mask[:, None, None, :].to(torch.bool)
 
 
 def _attend(q, k, v, causal: bool, key_mask=None):

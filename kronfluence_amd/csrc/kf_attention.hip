@@ -874,7 +874,14 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(const Args a) {
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
-// Tile rows and waves per SIMD of each kernel.
+// Tile rows and waves per SIMD of each kernel: as many waves as the registers allow (a wave's exponentials run beside another's matrix
+// instructions), and the tile height that leaves room for them.  Times in us, the other choice in brackets; A: 64 x 512 x 12 heads x 64,
+// B: 16 x 512 x 32/8 heads x 128, C: 64 x 512 x 12 heads x 32, all bf16 causal; D: fp32, 24 sequences of 29 to 233 tokens x 12 heads x 64.
+//   forward: 64 keys, four waves: A 62 (32 keys: 64), C 46 (32: 50); above width 64 32 keys, three waves: B 74 (64 keys, two waves: 78)
+//   dq: 32 keys, four waves: A 84 (64 keys, two waves: 85); above width 64 64 keys: B 110 (32 keys: 115)
+//   dk / dv: 32 queries, three waves: A 102 (64 queries, in registers for one wave: 231); width 32 64 queries: all of the backward C 135 (146)
+//   v from LDS (VL): A 102 (v in registers: 120), B 131 (213); width 96 has the registers
+//   fp32: three, two and two waves: D 27, 36, 44 (two, one and one: 28.5, 38, 62); above width 64 the parts' registers leave one
 template <class T, int DP>
 struct Shape {
     static constexpr bool SPLIT = PARTS<T> == 3, VL = !SPLIT && (DP == 64 || DP > 96);
@@ -899,16 +906,19 @@ bool configure() {
     return set(S::forward, S::FORWARD_LDS) && set(S::dq, S::DQ_LDS) && set(S::dkv, S::DKV_LDS);
 }
 
-// One-time kernel attribute set-up, thread-safe.
+// Kernel attribute set-up, once per device, thread-safe.
 int configure_kernels() {
-    static std::once_flag flag;
-    static int status = KF_OK;
-    std::call_once(flag, [] {
+    constexpr int DEVICES = 64;
+    static std::once_flag flags[DEVICES];
+    static int status[DEVICES] = {};
+    int device = 0;
+    if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= DEVICES) return KF_ERR_LAUNCH_FAILED;
+    std::call_once(flags[device], [device] {
         if (!(configure<__bf16, 32>() && configure<__bf16, 64>() && configure<__bf16, 96>() && configure<__bf16, 128>() && configure<Split, 32>() &&
               configure<Split, 64>() && configure<Split, 96>() && configure<Split, 128>()))
-            status = KF_ERR_LAUNCH_FAILED;
+            status[device] = KF_ERR_LAUNCH_FAILED;
     });
-    return status;
+    return status[device];
 }
 
 template <class T, int DP>

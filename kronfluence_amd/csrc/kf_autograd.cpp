@@ -157,18 +157,20 @@ Tensor work_order(const AttentionCall& c, const Tensor& starts) {
     return order;
 }
 
-Tensor attention_forward(const AttentionCall& c, Tensor q, Tensor k, Tensor v, const Tensor& lengths, const Tensor& offsets, Tensor* lse, Tensor* order_out) {
+// `lengths` and `offsets` come back as the kernels read them (a backward pass does not convert them again)
+Tensor attention_forward(const AttentionCall& c, Tensor q, Tensor k, Tensor v, Tensor& lengths, Tensor& offsets, Tensor* lse, Tensor* order_out) {
     Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
     if (lse) *lse = at::empty({c.heads, c.rows}, q.options().dtype(at::kFloat));
     if (c.empty()) return out.zero_();
     const c10::DeviceGuard guard(q.device());
     q = heads_operand(q); k = heads_operand(k); v = heads_operand(v);
-    const Tensor counts = row_counts(lengths, c.length), starts = row_counts(offsets, c.rows);
-    const Tensor order = work_order(c, starts);
+    lengths = row_counts(lengths, c.length);
+    offsets = row_counts(offsets, c.rows);
+    const Tensor order = work_order(c, offsets);
     if (order_out) *order_out = order;
     const kf_heads_view vo = view(out), vq = view(q), vk = view(k), vv = view(v);
     check(kf_attention_forward(&vo, lse ? lse->data_ptr<float>() : nullptr, &vq, &vk, &vv, c.dtype, c.sequences, c.length, c.rows, c.heads, c.kv_heads, c.width,
-                               static_cast<const int32_t*>(pointer(counts)), static_cast<const int32_t*>(pointer(starts)),
+                               static_cast<const int32_t*>(pointer(lengths)), static_cast<const int32_t*>(pointer(offsets)),
                                static_cast<const int32_t*>(pointer(order)), c.causal, c.scale, stream_of(q)),
           "kf_attention_forward");
     return out;
@@ -195,8 +197,7 @@ variable_list attention_backward(const AttentionCall& c, Tensor grad, Tensor out
 struct Attention : torch::autograd::Function<Attention> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& lengths_,
                           const std::optional<Tensor>& offsets_, bool causal, double scale) {
-        const Tensor lengths = given(lengths_), offsets = given(offsets_);
-        Tensor lse, order;
+        Tensor lengths = given(lengths_), offsets = given(offsets_), lse, order;
         const Tensor out = attention_forward(attention_call(q, k, v, lengths, offsets, causal, scale), q, k, v, lengths, offsets, &lse, &order);
         ctx->save_for_backward({q, k, v, out, lse, lengths, offsets, order});
         ctx->saved_data["causal"] = causal;
@@ -217,7 +218,7 @@ struct Attention : torch::autograd::Function<Attention> {
 
 Tensor attention(Tensor q, Tensor k, Tensor v, bool causal, const std::optional<double>& scale, const std::optional<Tensor>& lengths_,
                  const std::optional<Tensor>& offsets_) {
-    const Tensor lengths = given(lengths_), offsets = given(offsets_);
+    Tensor lengths = given(lengths_), offsets = given(offsets_);
     const int64_t width = q.dim() > 0 ? q.size(-1) : 0;
     const double by = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(width, 1)));
     const AttentionCall c = attention_call(q, k, v, lengths, offsets, causal, by);

@@ -11,8 +11,8 @@ transposed copy) and that grouped key / value heads, padded and packed batches n
 >>> h = functional.layer_norm(x, self.ln.weight, self.ln.bias, eps=self.ln.eps)
 
 Like the rest of the package they raise ``KfError`` for tensors that are not on an MI355X and for arguments the kernels do not take.
-First derivatives only (``create_graph=True`` is refused).  Under ``torch.autocast`` they cast as the torch operators do: attention runs in the autocast dtype, a norm
-returns float32 (reading its input as it is, with no cast in between).
+First derivatives only (``create_graph=True`` is refused).  Under ``torch.autocast`` they cast as the torch operators do: attention runs
+in the autocast dtype, a layer norm returns float32 (reading its input as it is, with no cast in between), an RMS norm its input's dtype.
 """
 
 from __future__ import annotations
@@ -52,7 +52,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
 def _norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float, centred: bool,
           out_dtype: Optional[torch.dtype]) -> torch.Tensor:
     if out_dtype is None:
-        out_dtype = torch.float32 if torch.is_autocast_enabled("cuda") and x.is_cuda else x.dtype
+        out_dtype = torch.float32 if centred and torch.is_autocast_enabled("cuda") and x.is_cuda else x.dtype
     return nat.autograd().norm(x, weight, bias, eps, centred, out_dtype)
 
 
@@ -69,8 +69,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, eps: Optional[float] = None,
              out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """``x / sqrt(mean(x^2) + eps) * weight`` over the last axis: :func:`layer_norm` without the mean.  ``eps`` defaults to the machine
-    epsilon of ``x.dtype``, as in ``torch.nn.RMSNorm``."""
+    """``x / sqrt(mean(x^2) + eps) * weight`` over the last axis: :func:`layer_norm` without the mean.  ``eps`` defaults to float32's machine
+    epsilon for inputs of every dtype, as ``torch.nn.RMSNorm`` takes it on the GPU; ``out_dtype`` to ``x.dtype``."""
     if eps is None:
-        eps = torch.finfo(x.dtype).eps if x.is_floating_point() else 0.0
+        eps = torch.finfo(torch.float32).eps
     return _norm(x, weight, None, eps, False, out_dtype)

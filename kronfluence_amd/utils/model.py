@@ -39,8 +39,7 @@ def apply_ddp(model: nn.Module, local_rank: int, rank: int, world_size: int) -> 
 def apply_fused_norms(model: nn.Module) -> nn.Module:
     """Replaces every ``nn.LayerNorm`` / ``nn.RMSNorm`` over one axis inside ``model`` by its counterpart on this package's kernels
     (``kronfluence_amd/module/norm.py``), in place, and returns ``model`` (the counterpart if ``model`` is such a norm itself).
-    Parameters, names and the state dict stay as they are; under autocast the norms return float32 as torch's do.  The norms then run on
-    an MI355X only.  Before or after ``prepare_model``; norms with hooks of their own are left alone."""
+    Parameters, names and the state dict stay as they are, and so do the dtypes the norms return.  The norms then run on an MI355X only.  Before or after ``prepare_model``; norms with hooks of their own are left alone."""
     from kronfluence_amd.module.norm import fused
 
     for parent in list(model.modules()):

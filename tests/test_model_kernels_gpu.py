@@ -115,3 +115,22 @@ def test_scores_through_every_stage_and_the_captured_train_pass(kind, tmp_path, 
     assert log["captures"] == 1 and log["replays"] == 7 and log["fallbacks"] == 0, log   # 8 whole batches, the ragged ninth eager
     assert rel(eager, want) <= 2 * 4 * 1.9e-3, rel(eager, want)
     assert rel(replayed, eager) <= 2e-6, rel(replayed, eager)   # the same kernels on the same inputs; only the score sums' order may differ
+
+
+@pytest.mark.parametrize("amp", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_fused_norms_return_what_the_torch_modules_return(dtype, amp):
+    """Types and default epsilon (rows so small that it is most of the denominator); values to the output type's rounding, one step apart
+    at most where both sides round once, plus the fp32 errors of 8 terms."""
+    from torch import nn
+
+    from kronfluence_amd.module.norm import fused
+
+    x = 3e-4 * torch.randn(5, 8, generator=torch.Generator().manual_seed(2)).cuda().to(dtype)
+    for module in (nn.LayerNorm(8), nn.RMSNorm(8), nn.RMSNorm(8, elementwise_affine=False), nn.LayerNorm(8, bias=False)):
+        module = module.cuda().to(dtype)
+        with torch.autocast("cuda", torch.bfloat16, enabled=amp):
+            want, got = module(x).detach(), fused(module)(x).detach()
+        assert got.dtype == want.dtype, (module, got.dtype, want.dtype)
+        step = 2 * 2.0 ** -8 if want.dtype == torch.bfloat16 else 32 * 2.0 ** -24
+        assert float((got.float() - want.float()).abs().max()) <= step * float(want.float().abs().max()), module
