@@ -335,8 +335,8 @@ __device__ __forceinline__ bool locate(const Args& a, int slot, bool last_first,
 // value head) pairs of equal size are many, whole pairs are dealt to the XCDs (a.chunk = the tiles of a sequence), the heads of a
 // sequence one after the other (24 sequences of 29 to 233 tokens, 12 heads x 64 fp32: 210 us, 264 us with the sequences of a head one
 // after the other).  An XCD deals its workgroups to its compute units in turn, too, so the tiles of a pair -- of very different cost, if
-// causal -- are taken from another one on in every pair and every round of the compute units: without that a unit gets the same tile of
-// pair after pair (64 x 512 x 12 heads x 64 bf16 causal: dk / dv 121 us, 102 with it; dq 93 and 84; forward 70 and 63).
+// causal -- are taken in reverse order in every other pair and every other round of the compute units: without that a unit gets the same
+// tile of pair after pair (64 x 512 x 12 heads x 64 bf16 causal: dk / dv 121 us, 102 with it; dq 93 and 82; forward 70 and 62).
 // Otherwise single tiles are dealt, the heads of a tile one after the other: with 1, 2, 4 or a multiple of 8 heads an XCD then sees the
 // same heads in every tile.  The `members` query heads of a group stay together.  False: nothing left (the grid is rounded up).
 constexpr int XCDS = 8, CUS = 32;   // CUS: compute units of an XCD
@@ -348,7 +348,8 @@ __device__ __forceinline__ bool work_item(const Args& a, int members, Item& w) {
     w.member = static_cast<int>(item % members);
     w.kv_head = static_cast<int>(unit % kv_heads);
     const int64_t round = n / chunk, turn = round + (chunk < CUS ? round * chunk / CUS : 0);
-    w.slot = static_cast<int>(unit / kv_heads * a.chunk + (pair + turn) % a.chunk);
+    const int64_t tile = pair % a.chunk;
+    w.slot = static_cast<int>(unit / kv_heads * a.chunk + (turn % 2 ? a.chunk - 1 - tile : tile));
     if (pair >= static_cast<int64_t>(a.slots) * kv_heads) return false;
     if (a.order) w.slot = a.order[w.slot];
     return true;
