@@ -334,23 +334,26 @@ __device__ __forceinline__ bool locate(const Args& a, int slot, bool last_first,
 // own: what reads the same k and v should go to one XCD, but no XCD may be left with the longest sequences.  Where (sequence, key /
 // value head) pairs of equal size are many, whole pairs are dealt to the XCDs (a.chunk = the tiles of a sequence), the heads of a
 // sequence one after the other (24 sequences of 29 to 233 tokens, 12 heads x 64 fp32: 210 us, 264 us with the sequences of a head one
-// after the other).  An XCD deals its workgroups to its compute units in turn, too, so the tiles of a pair -- of very different cost, if
-// causal -- are taken in reverse order in every other pair and every other round of the compute units: without that a unit gets the same
-// tile of pair after pair (64 x 512 x 12 heads x 64 bf16 causal: dk / dv 121 us, 102 with it; dq 93 and 82; forward 70 and 62).
+// after the other).  An XCD deals its workgroups to its compute units in turn, too, and the tiles of a pair are of very different cost, if
+// causal.  So the pairs of an XCD are worked on in blocks of about BLOCK_UNITS, the first (dearest) tiles of all pairs of a block first:
+// pair after pair, every unit would get the same tile each time, and the last dear tiles would start last (causal bf16: 64 x 512 x 12
+// heads x 64, dk / dv 121 us pair after pair, 98 in blocks; 4 x 2048 x 16 x 64, forward 77 and 53, backward 215 and 158).  In larger
+// blocks k and v leave the L2 (the first of these with 32 pairs a block: 102).
 // Otherwise single tiles are dealt, the heads of a tile one after the other: with 1, 2, 4 or a multiple of 8 heads an XCD then sees the
 // same heads in every tile.  The `members` query heads of a group stay together.  False: nothing left (the grid is rounded up).
-constexpr int XCDS = 8, CUS = 32;   // CUS: compute units of an XCD
+constexpr int XCDS = 8, BLOCK_UNITS = 16;
 struct Item { int slot, kv_head, member; };
 __device__ __forceinline__ bool work_item(const Args& a, int members, Item& w) {
-    const int kv_heads = a.heads / a.group;
-    const int64_t id = blockIdx.x, chunk = static_cast<int64_t>(a.chunk) * members, n = id / XCDS;
-    const int64_t item = (n / chunk * XCDS + id % XCDS) * chunk + n % chunk, pair = item / members, unit = pair / a.chunk;
-    w.member = static_cast<int>(item % members);
+    const int kv_heads = a.heads / a.group, id = static_cast<int>(blockIdx.x), n = id / XCDS;
+    const int items = a.chunk * members, units = static_cast<int>(gridDim.x) / (XCDS * items);   // (of an XCD; the grid is a multiple)
+    const int blocks = (units + BLOCK_UNITS - 1) / BLOCK_UNITS, most = (units + blocks - 1) / blocks;   // units of a block
+    const int block = n / (most * items) * most, here = min(most, units - block), in = n - block * items;
+    const int tile = in / (here * members), rest = in % (here * members);
+    const int64_t unit = static_cast<int64_t>(block + rest / members) * XCDS + id % XCDS;
+    w.member = rest % members;
     w.kv_head = static_cast<int>(unit % kv_heads);
-    const int64_t round = n / chunk, turn = round + (chunk < CUS ? round * chunk / CUS : 0);
-    const int64_t tile = pair % a.chunk;
-    w.slot = static_cast<int>(unit / kv_heads * a.chunk + (turn % 2 ? a.chunk - 1 - tile : tile));
-    if (pair >= static_cast<int64_t>(a.slots) * kv_heads) return false;
+    w.slot = static_cast<int>(unit / kv_heads * a.chunk + tile);
+    if (unit * a.chunk + tile >= static_cast<int64_t>(a.slots) * kv_heads) return false;
     if (a.order) w.slot = a.order[w.slot];
     return true;
 }
