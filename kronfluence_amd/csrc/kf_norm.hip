@@ -8,6 +8,9 @@
 // 16 384, beyond that the row is re-read from the cache.  The weight's gradient needs no atomics: a group adds up the columns of its
 // rows in registers, each workgroup writes one partial row, and a second kernel adds the partial rows in a fixed order.
 // All arithmetic is fp32; the outputs are rounded once.
+//
+// Measured (a copy reaches 5.2 TB/s): 131072 x 768 bf16 -> fp32 forward 138 us (4.4 TB/s), backward 138 + 6 (5.8 TB/s); 16384 x 768 fp32
+// forward 18 us, backward 27 + 6; RMS norm of 8192 x 4096 bf16 forward 26 us (5.1 TB/s), backward 41 + 4 (4.9 TB/s).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -53,13 +56,17 @@ __device__ __forceinline__ void widen(float (&x)[VEC], const Chunk<T, VEC>& c) {
 template <int VEC, class T>
 __device__ __forceinline__ void load(float (&x)[VEC], const T* p, int64_t column, int64_t width) { widen(x, load_chunk<VEC>(p, column, width)); }
 
-template <int VEC, class T>
+// PAST: past the caches, for results that the kernel does not read again (131072 x 768 bf16 -> fp32: forward 152 us, 138 with it; backward
+// 157 and 138; 16384 x 768 fp32: forward 21 and 18; what reads the result next is no slower: 2048 to 131072 rows, a product or a sum)
+template <bool PAST, int VEC, class T>
 __device__ __forceinline__ void store(T* p, int64_t column, int64_t width, const float (&x)[VEC]) {
     if (column + VEC <= width) {
-        Chunk<T, VEC> c;
+        typedef T Vector __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
+        Vector v;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) c.v[i] = static_cast<T>(x[i]);
-        *reinterpret_cast<Chunk<T, VEC>*>(p + column) = c;
+        for (int i = 0; i < VEC; ++i) v[i] = static_cast<T>(x[i]);
+        if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<Vector*>(p + column));
+        else *reinterpret_cast<Vector*>(p + column) = v;
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
@@ -174,7 +181,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : THREADS) void norm_forward_ker
 #pragma unroll
             for (int i = 0; i < VEC; ++i) out[i] = fmaf(v[j][i] * r, w[j][i], b[j][i]);
             const int64_t c = (lane + j * LANES) * VEC;
-            if (c < a.width) store(y, c, a.width, out);
+            if (c < a.width) store<true>(y, c, a.width, out);
         }
         if (a.stats && lane == 0) { a.stats[2 * row] = mu; a.stats[2 * row + 1] = r; }
     }
@@ -213,7 +220,7 @@ __global__ __launch_bounds__(WIDE_THREADS) void norm_forward_long_kernel(const F
             load(v, x, c, a.width);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) v[i] = fmaf((v[i] - mu) * r, w[i], b[i]);
-            store(y, c, a.width, v);
+            store<true>(y, c, a.width, v);
         }
         if (a.stats && threadIdx.x == 0) { a.stats[2 * row] = mu; a.stats[2 * row + 1] = r; }
     }
@@ -276,7 +283,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : THREADS) void norm_backward_ke
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) out[i] = r * (u[j][i] - mean_u - h[j][i] * mean_uh);
                 const int64_t c = (lane + j * LANES) * VEC;
-                if (c < a.width) store(dx, c, a.width, out);
+                if (c < a.width) store<true>(dx, c, a.width, out);
             }
         }
     }
@@ -304,7 +311,7 @@ __global__ __launch_bounds__(LANES > 64 ? LANES : THREADS) void norm_backward_ke
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int64_t c = (lane + j * LANES) * VEC;
-                if (c < a.width) store(out + part * a.width, c, a.width, part ? db[j] : dw[j]);
+                if (c < a.width) store<false>(out + part * a.width, c, a.width, part ? db[j] : dw[j]);
             }
         }
     }
@@ -356,7 +363,7 @@ __global__ __launch_bounds__(WIDE_THREADS) void norm_backward_long_kernel(const 
             if (a.weight) load_as(w, a.weight, a.w_dtype, c, a.width);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) h[i] = r * (u[i] * w[i] - mean_u - (h[i] - mu) * r * mean_uh);
-            store(dx, c, a.width, h);
+            store<true>(dx, c, a.width, h);
         }
     }
 }
