@@ -9,8 +9,8 @@
 // rows in registers, each workgroup writes one partial row, and a second kernel adds the partial rows in a fixed order.
 // All arithmetic is fp32; the outputs are rounded once.
 //
-// Measured (a copy reaches 5.2 TB/s): 131072 x 768 bf16 -> fp32 forward 138 us (4.4 TB/s), backward 138 + 6 (5.8 TB/s); 16384 x 768 fp32
-// forward 18 us, backward 27 + 6; RMS norm of 8192 x 4096 bf16 forward 26 us (5.1 TB/s), backward 41 + 4 (4.9 TB/s).
+// Measured (a copy reaches 5.2 TB/s): 131072 x 768 bf16 -> fp32 forward 105 us (5.8 TB/s), backward 138 + 6 (5.8 TB/s); 16384 x 768 fp32
+// forward 18 us, backward 27 + 6; RMS norm of 8192 x 4096 bf16 forward 25 us (5.4 TB/s), backward 41 + 4 (5.0 TB/s).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -398,10 +398,21 @@ __global__ __launch_bounds__(64 * STRANDS) void norm_reduce_kernel(const float* 
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
-// workgroups of a launch: enough to fill 256 compute units several times, each with several rows, so that the weights (and the
-// partial sums of a backward pass) are read (written) once per many rows
-int64_t forward_groups(int64_t rows, int64_t width) { return std::min<int64_t>(width <= WAVE_MAX ? cdiv(rows, 4) : rows, 2048); }
-int64_t backward_groups(int64_t rows, int64_t width) { return std::min<int64_t>(width <= WAVE_MAX ? cdiv(rows, 4) : rows, width <= WAVE_MAX ? 1024 : 512); }
+// Workgroups of a launch: as many as the card holds at once, each with several rows, so that the weights (and the partial sums of a
+// backward pass) are read (written) once per many rows and no second round is left half full (131072 x 768 bf16 -> fp32, 1536 at once:
+// forward 105 us, 143 with 2048; backward, 1024 at once: 140, 205 with 512).  A backward pass takes at most MAX_PARTIALS, which the
+// workspace has room for.
+constexpr int64_t CUS = 256, MAX_PARTIALS = 1024;
+template <auto KERNEL>
+int64_t resident(int threads) {
+    static const int64_t all = [threads] {
+        int blocks = 0;
+        return hipOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, KERNEL, threads, 0) == hipSuccess && blocks > 0 ? blocks * CUS : MAX_PARTIALS;
+    }();
+    return all;
+}
+int64_t row_groups(int64_t rows, int64_t width) { return width <= WAVE_MAX ? cdiv(rows, 4) : rows; }
+int64_t most_partials(int64_t rows, int64_t width) { return std::min(row_groups(rows, width), MAX_PARTIALS); }
 
 // f(LANES, NV) with the smallest group that holds a row of `width` columns in registers; LANES 0: none does
 template <int VEC, class F>
@@ -426,22 +437,35 @@ void with_group(int64_t width, F f) {
     f(one, integral_constant<int, 4>());
 }
 
+template <class X, class Y, int LANES, int NV>
+constexpr auto forward_kernel() {
+    if constexpr (LANES == 0) return &norm_forward_long_kernel<X, Y>;
+    else return &norm_forward_kernel<X, Y, LANES, NV>;
+}
+template <class X, class G, int LANES, int NV>
+constexpr auto backward_kernel() {
+    if constexpr (LANES == 0) return &norm_backward_long_kernel<X, G>;
+    else return &norm_backward_kernel<X, G, LANES, NV>;
+}
+
 template <class X, class Y>
 int forward_as(const ForwardArgs& a, hipStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(forward_groups(a.rows, a.width));
     with_group<vec_of<X, Y>()>(a.width, [&](auto lanes, auto nv) {
-        if constexpr (lanes == 0) norm_forward_long_kernel<X, Y><<<grid, WIDE_THREADS, 0, stream>>>(a);
-        else norm_forward_kernel<X, Y, lanes, nv><<<grid, lanes > 64 ? WIDE_THREADS : THREADS, 0, stream>>>(a);
+        constexpr int threads = lanes == 64 ? THREADS : WIDE_THREADS;
+        constexpr auto kernel = forward_kernel<X, Y, lanes, nv>();
+        kernel<<<static_cast<unsigned>(std::min(row_groups(a.rows, a.width), resident<kernel>(threads))), threads, 0, stream>>>(a);
     });
     return launch_status();
 }
 
+// `groups`: the partial rows it writes
 template <class X, class G>
-int backward_as(const BackwardArgs& a, hipStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(backward_groups(a.rows, a.width));
+int backward_as(const BackwardArgs& a, hipStream_t stream, int64_t& groups) {
     with_group<vec_of<X, G>()>(a.width, [&](auto lanes, auto nv) {
-        if constexpr (lanes == 0) norm_backward_long_kernel<X, G><<<grid, WIDE_THREADS, 0, stream>>>(a);
-        else norm_backward_kernel<X, G, lanes, nv><<<grid, lanes > 64 ? WIDE_THREADS : THREADS, 0, stream>>>(a);
+        constexpr int threads = lanes == 64 ? THREADS : WIDE_THREADS;
+        constexpr auto kernel = backward_kernel<X, G, lanes, nv>();
+        groups = std::min(most_partials(a.rows, a.width), resident<kernel>(threads));
+        kernel<<<static_cast<unsigned>(groups), threads, 0, stream>>>(a);
     });
     return launch_status();
 }
@@ -478,7 +502,7 @@ int kf_norm_forward(void* y, int y_dtype, float* stats, const void* x, int x_dty
 }
 
 int64_t kf_norm_backward_workspace_bytes(int64_t rows, int64_t width) {
-    return rows > 0 && width > 0 ? backward_groups(rows, width) * 2 * width * 4 : 0;
+    return rows > 0 && width > 0 ? most_partials(rows, width) * 2 * width * 4 : 0;
 }
 
 int kf_norm_backward(void* dx, void* dweight, void* dbias, const void* grad, int grad_dtype, const void* x, int x_dtype, const float* stats, int64_t rows,
@@ -493,11 +517,12 @@ int kf_norm_backward(void* dx, void* dweight, void* dbias, const void* grad, int
     const BackwardArgs a = {dx, sums ? reinterpret_cast<float*>(workspace) : nullptr, stats, grad, x, weight, rows, width, row_stride, w_dtype,
                             centred != 0, with_bias};
     const hipStream_t on = reinterpret_cast<hipStream_t>(stream);
-    if (int s = with_types(x_dtype, grad_dtype, [&](auto t, auto g) { return backward_as<decltype(t), decltype(g)>(a, on); })) return s;
+    int64_t groups = 0;
+    if (int s = with_types(x_dtype, grad_dtype, [&](auto t, auto g) { return backward_as<decltype(t), decltype(g)>(a, on, groups); })) return s;
     if (!sums) return KF_OK;
     if (cdiv(width, 64) > 0x7fffffff) return KF_ERR_INVALID_ARGUMENT;
     norm_reduce_kernel<<<dim3(static_cast<unsigned>(cdiv(width, 64)), with_bias + 1), 64 * STRANDS, 0, on>>>(
-        a.partial, backward_groups(rows, width), width, with_bias + 1, dweight, dbias, w_dtype);
+        a.partial, groups, width, with_bias + 1, dweight, dbias, w_dtype);
     return launch_status();
 }
 
