@@ -639,7 +639,8 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
     }
     const int64_t stat = head * a.rows + w.stat;
     const float lse = real ? a.lse[stat + query] : INFINITY;
-    if (half == 0 && real) a.delta[stat + query] = delta;
+    const bool alone = first < w.length && (a.causal ? min(w.length, first + 32) : w.length) <= 32;   // (wave-uniform)
+    if (half == 0 && real && !alone) a.delta[stat + query] = delta;
 
     f32x16 acc[DP / 32] = {};
     const float c = a.scale * LOG2E;
@@ -650,6 +651,27 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
     sv.load(v.from(0));
     sk.store(lds);
     sv.store(lds + TILE);
+    // Rows whose keys all stand in one block: D as the sum of p dp there, in fp32.  out, which D comes from otherwise, is rounded, and where
+    // a row sees few keys its gradients are small beside do . out (two keys, bf16: dq and dk off by 1.4 % of their norm, 0.2 % with it).
+    if (w.row0 == 0 && (a.causal || w.length <= 32)) {
+        __syncthreads();
+        if (alone) {
+            const uint32_t kt = lds_address(lds), vt = kt + TILE;
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int i = 0; i < Img::SLABS; ++i) s = Type<T>::mma(read.rows(kt, 0, i), q.f[i], s);
+#pragma unroll
+            for (int i = 0; i < Img::SLABS; ++i) dp = Type<T>::mma(read.rows(vt, 0, i), g.f[i], dp);
+            settle();
+            const int visible = a.causal ? min(w.length, query + 1) : w.length;
+            delta = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                delta = fmaf(8 * (r / 4) + 4 * half + r % 4 < visible ? __builtin_amdgcn_exp2f(fmaf(s[r], c, -lse)) : 0.0f, dp[r], delta);
+            delta += other_half(delta);
+            if (half == 0 && real) a.delta[stat + query] = delta;
+        }
+    }
     for (int t = 0; t < tiles; ++t) {
         const uint32_t kt = lds_address(lds) + (t & 1) * 2 * TILE, vt = kt + TILE;
         const int k0 = t * BK;

@@ -6,7 +6,8 @@ Tolerances are elementwise bounds on the rounding errors the kernels may make, e
 attention   p carries the fp32 errors of a width-long product, of exp2 and of the sum over n keys -- relative
             ep = (width + 8) E max(scale |q| |k|) + (n + 16) E -- and, with bf16 inputs, one rounding U to its operand type.
             out:  (ep + Up) (p |v|) + U |out|
-            D:    sum |do| err(out) + (width + 2) E |do| |out|
+            D:    sum |do| err(out) + (width + 2) E |do| |out|;   (ep + (n + 4) E) sum p |dp| + (width + 2) E sum p |do| |v| for rows that see
+                  32 keys at most
             ds:   (ep + Up) |ds| + p (err(D) + (width + 2) E |do| |v|) + E p (|dp| + |D|);    rounded once more (U) for dq, dk
             dq:   scale err(ds) |k| + (n + 2) E scale |ds| |k| + U |dq|;   dk, dv likewise
             (Up = U for bf16, 0 for fp32: fp32 operands are not rounded)
@@ -47,7 +48,7 @@ def close(got, want, bound, what):
 # ------------------------------------------------------------------------------------------------
 # attention
 # ------------------------------------------------------------------------------------------------
-def expected_sequence(q, k, v, g, causal, scale):
+def expected_sequence(q, k, v, g, causal, scale, few=False):
     """Values and error bounds for one sequence and one kv head: ``q``, ``g`` [n, group, width], ``k``, ``v`` [n, width]."""
     dtype = q.dtype
     U, Up = HALF[dtype], HALF[dtype] if dtype == BF16 else 0.0
@@ -65,6 +66,8 @@ def expected_sequence(q, k, v, g, causal, scale):
     ds = p * (dp - delta)
     dq, dk, dv = scale * ds @ k, scale * ds.transpose(1, 2) @ q, p.transpose(1, 2) @ g
     err_delta = (g.abs() * err_out).sum(-1, keepdim=True) + (width + 2) * E * (g.abs() * out.abs()).sum(-1, keepdim=True)
+    if few:
+        err_delta = (p * ((ep + (n + 4) * E) * dp.abs() + (width + 2) * E * (g.abs() @ v.abs().transpose(1, 2)))).sum(-1, keepdim=True)
     err_ds = ((ep + 2 * E) * ds.abs() + p * (err_delta + (width + 2) * E * (g.abs() @ v.abs().transpose(1, 2)))
               + E * p * (dp.abs() + delta.abs()) + Up * ds.abs() + (n + 2) * E * ds.abs())
     err_dq = scale * err_ds @ k.abs() + U * dq.abs()
@@ -76,7 +79,7 @@ def expected_sequence(q, k, v, g, causal, scale):
     return ((heads_last(out), heads_last(err_out)), (heads_last(dq), heads_last(err_dq)), (dk_sum, err_dk), (dv_sum, err_dv))
 
 
-def check_attention(functional, q, k, v, g, causal, spans, scale=None, lengths=None, cu_seqlens=None):
+def check_attention(functional, q, k, v, g, causal, spans, scale=None, lengths=None, cu_seqlens=None, few=False):
     """``spans``: (index of the sequence's rows) for every sequence that has tokens; rows outside every span must come back 0."""
     q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
     out = functional.attention(q, k, v, causal=causal, scale=scale, lengths=lengths, cu_seqlens=cu_seqlens)
@@ -93,7 +96,7 @@ def check_attention(functional, q, k, v, g, causal, spans, scale=None, lengths=N
         for h in range(kv_heads):
             of = slice(h * group, (h + 1) * group)
             parts = expected_sequence(q.detach()[span][:, of], k.detach()[span][:, h], v.detach()[span][:, h], g[span][:, of], causal,
-                                      1.0 / math.sqrt(width) if scale is None else scale)
+                                      1.0 / math.sqrt(width) if scale is None else scale, few)
             for i, (value, error) in enumerate(parts):
                 place = of if i < 2 else h
                 want[i][span][:, place] = value
@@ -134,6 +137,21 @@ def test_attention_padded_rows_hold_anything(functional, dtype, causal, width):
     spans = [(i, slice(0, n)) for i, n in enumerate(lengths) if n]
     for kind in (torch.int32, torch.int64):
         check_attention(functional, q, k, v, g, causal, spans, lengths=torch.tensor(lengths, dtype=kind, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv_heads,width", [(4, 1, 32), (2, 2, 64), (2, 1, 128)])
+def test_attention_gradients_of_rows_with_few_keys(functional, dtype, causal, heads, kv_heads, width):
+    """Peaked rows with 2 to 32 keys: do . out there is far greater than the gradients it is taken off, so a rounded out must not enter."""
+    lengths = [2, 2, 2, 2, 3, 5, 8, 17, 31, 32]
+    q, k, v, g = (make((sum(lengths), n, width), dtype, seed, scale)
+                  for n, seed, scale in ((heads, 1, 3.0), (kv_heads, 2, 1.0), (kv_heads, 3, 1.0), (heads, 4, 0.05)))
+    offsets = [0]
+    for n in lengths:
+        offsets.append(offsets[-1] + n)
+    spans = [slice(a, b) for a, b in zip(offsets, offsets[1:])]
+    check_attention(functional, q, k, v, g, causal, spans, cu_seqlens=torch.tensor(offsets, dtype=torch.int32, device="cuda"), few=True)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
