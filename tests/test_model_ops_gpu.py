@@ -518,3 +518,54 @@ def test_norm_under_autocast_and_on_empty_rows(functional):
     weight = w.clone().requires_grad_()
     functional.layer_norm(empty, weight).sum().backward()
     assert empty.grad.shape == (0, 96) and not weight.grad.any()
+
+
+# ------------------------------------------------------------------------------------------------
+# tensors of more than 2^32 elements
+# ------------------------------------------------------------------------------------------------
+@pytest.fixture
+def room():
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 120 << 30:
+        pytest.skip("needs 120 GB of free device memory")
+    yield
+    torch.cuda.empty_cache()
+
+
+def test_attention_offsets_past_32_bits(functional, room):
+    """The last sequences of a packed batch of 2^32 elements and more are those of a small batch, bit for bit."""
+    heads, width, each, n = 8, 16, 64, (1 << 25) // 64 + 1
+    q, k, v, g = (torch.empty(n * each + 5, heads, width, dtype=BF16, device="cuda") for _ in range(4))
+    last = slice((n - 3) * each, n * each)
+    for i, t in enumerate((q, k, v, g)):
+        t.zero_()
+        t[last] = make((3 * each, heads, width), BF16, i + 1)
+    assert q.numel() > 1 << 32
+    offsets = torch.arange(0, (n + 1) * each, each, dtype=torch.int32, device="cuda")
+
+    def both(q, k, v, g, offsets):
+        q, k, v = (t.requires_grad_() for t in (q, k, v))
+        out = functional.attention(q, k, v, cu_seqlens=offsets)
+        return (out.detach(),) + torch.autograd.grad(out, (q, k, v), g)
+
+    want = both(*(t[last].clone() for t in (q, k, v, g)), offsets[:4].clone())
+    got = both(q, k, v, g, offsets)
+    for name, a, b in zip(("out", "dq", "dk", "dv"), got, want):
+        assert torch.equal(a[last], b) and not bool(a[n * each:].any()) and not bool(a[:each].any()), name
+
+
+@pytest.mark.parametrize("width", [4096, 20000])
+def test_norm_offsets_past_32_bits(functional, room, width):
+    rows = (1 << 32) // width + 7
+    x, g = (torch.zeros(rows, width, dtype=BF16, device="cuda") for _ in range(2))
+    x[-3:], g[-3:] = make((3, width), BF16, 1), make((3, width), BF16, 2)
+    w = make((width,), F32, 3)
+
+    def both(x, g):
+        x = x.requires_grad_()
+        y = functional.layer_norm(x, w)
+        return y.detach(), torch.autograd.grad(y, x, g)[0]
+
+    want = both(x[-3:].clone(), g[-3:].clone())
+    for a, b in zip(both(x, g), want):
+        assert torch.equal(a[-3:], b) and not bool(a[:-3].any())
