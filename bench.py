@@ -514,7 +514,8 @@ def _event_summary(events, peak_tflops: float, kernel: str, elapsed_s: Optional[
 
 
 def kernel_source_hash() -> str:
-    """sha256 over the sources of the kernels a kept PMC profile reports (every HIP source and header but the eigensolver's):
+    """sha256 over the sources of the kernels a kept PMC profile reports (every HIP source and header but the eigensolver's
+    and the model passes'):
     identifies the code the profile was taken on."""
     import glob
     import hashlib
@@ -523,8 +524,8 @@ def kernel_source_hash() -> str:
     paths = sorted(glob.glob(os.path.join(ROOT, "kronfluence_amd", "csrc", "*.hip")) + glob.glob(os.path.join(ROOT, "kronfluence_amd", "csrc", "*.h"))
                    + glob.glob(os.path.join(ROOT, "include", "*.h")))
     for path in paths:
-        if os.path.basename(path) == "kf_eigh.hip":
-            continue   # the eigensolver: none of its kernels is in the PMC summary (its evidence is the eigh logs under profiles/)
+        if os.path.basename(path) in ("kf_eigh.hip", "kf_attention.hip", "kf_norm.hip"):
+            continue   # none of their kernels is in the PMC summary (evidence: the eigh logs and model_ops_kernel_stats.csv under profiles/)
         with open(path, "rb") as handle:
             digest.update(os.path.basename(path).encode() + b"\0" + handle.read())
     return digest.hexdigest()

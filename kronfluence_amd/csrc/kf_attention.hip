@@ -20,6 +20,11 @@
 // kernels: 64 x 256 x 12 heads x 64, forward 131 to 84 us, backward 470 to 325; 2 x 2048 x 16 x 128 causal, 334 to 223 and 1129 to 817.
 // Finite values from 3.39e38 on (their first part rounds to infinity) act as infinities, parts below 2^-126 as 0.
 //
+// Measured (us; causal but for the first; forward, dq, dk / dv): bf16 256 x 128 x 12 heads x 64, padded: 37, 45, 48 (bound by prologue and
+// epilogue of one-tile sequences); 64 x 512 x 12 x 64: 61, 81, 97 and 16 x 512 x 32/8 x 128: 72, 106, 125 (vector instructions of the
+// softmax, few rounds of tiles); 1 x 8192 x 32/8 x 128: 572 (960 TFLOP/s), 777, 1087 + 28 (matrix instructions); fp32 24 x 29..233 x 12 x 64:
+// 27, 36, 43 (few, uneven workgroups).
+//
 // Roundings to fewer bits than 32: P and dS are rounded to bf16 as operands of their second product when the inputs are bf16 (one
 // rounding of half a step, 2^-9 relative, per term of a sum whose inputs carry the same rounding), and the outputs once at the end.
 // Maxima, sums, L, D and all accumulators are fp32.
@@ -333,8 +338,8 @@ __device__ __forceinline__ bool locate(const Args& a, int slot, bool last_first,
 // Workgroup -> (slot, kv_head, member of its group).  Consecutive workgroup ids go to the eight XCDs in turn, and each has an L2 of its
 // own: what reads the same k and v should go to one XCD, but no XCD may be left with the longest sequences.  Where (sequence, key /
 // value head) pairs of equal size are many, whole pairs are dealt to the XCDs (a.chunk = the tiles of a sequence), the heads of a
-// sequence one after the other (24 sequences of 29 to 233 tokens, 12 heads x 64 fp32: 210 us, 264 us with the sequences of a head one
-// after the other).  An XCD deals its workgroups to its compute units in turn, too, and the tiles of a pair are of very different cost, if
+// sequence one after the other (24 sequences of 29 to 233 tokens, 12 heads x 64, in fp32 products: 210 us, 264 with the sequences of a
+// head one after the other).  An XCD deals its workgroups to its compute units in turn, too, and the tiles of a pair are of very different cost, if
 // causal.  So the pairs of an XCD are worked on in blocks of about BLOCK_UNITS, the first (dearest) tiles of all pairs of a block first:
 // pair after pair, every unit would get the same tile each time, and the last dear tiles would start last (causal bf16: 64 x 512 x 12
 // heads x 64, dk / dv 121 us pair after pair, 98 in blocks; 4 x 2048 x 16 x 64, forward 77 and 53, backward 215 and 158).  In larger
@@ -359,8 +364,9 @@ __device__ __forceinline__ bool work_item(const Args& a, int members, Item& w) {
 }
 
 // The slots of a packed batch by falling cost: documents come in any order, and a long one whose tiles start last leaves the card
-// waiting for it (24 documents of 12011 tokens, 16/4 heads x 128 bf16: forward 101 to 85 us, dq 131 to 123, dk / dv 183 to 152).  The cost of a slot is that of its tile in the
-// kernels over queries (last tiles first) and in the one over keys (first tiles first) alike: the tiles of its sequence it meets.
+// waiting for it (24 documents of 12011 tokens, 16/4 heads x 128 bf16: forward 101 us in the
+// order they come, 85 in this one; dq 131 and 123, dk / dv 183 and 152).  The cost of a slot is that of its tile in the kernels over
+// queries (last tiles first) and in the one over keys (first tiles first) alike: the tiles of its sequence it meets.
 // One workgroup: a histogram of costs, places from the highest down; the order inside a cost is of no consequence.
 constexpr int COSTS = 2048, MAX_ORDERED = 16384;
 __global__ __launch_bounds__(1024) void attention_order_kernel(const Args a, int32_t* order) {
@@ -983,9 +989,9 @@ int64_t delta_bytes(int64_t rows, int64_t heads) { return (rows * heads * 4 + 15
 
 // How many workgroups share the queries of one key tile in the dk / dv kernel.  512 workgroups of it fit the card at a time, and
 // the first tile of a causal sequence has twice the mean work: with all of them resident at once the kernel takes as long as its
-// largest item.  Measured (32/8 heads x 128): one document of 8192 tokens, 512 items: 2064 us whole, 1233 + 27 us (join) in two parts,
-// 1218 + 58 in four; 24 documents of 12011 tokens in all, 16/4 heads, 472 items: 467 us whole, 294 + 21 in two, 218 + 36 in four;
-// 16 x 512 tokens, 512 items of equal cost at four steps a head: 173 us whole, 182 + 29 in two.
+// largest item.  Measured (bf16, causal, width 128): one document of 8192 tokens, 32/8 heads, 512 items: 1867 us whole, 1138 + 28 us
+// (join) in two parts, 1135 + 58 in four; 24 documents of 12011 tokens in all, 16/4 heads, 472 items: 425 us whole, 235 + 21 in two,
+// 159 + 36 in four; 16 x 512 tokens, 32/8 heads, 512 items of at most 64 steps: 128 us whole, 108 + 30 in two.
 int64_t dkv_parts(int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, bool packed, bool causal) {
     const int64_t items = tile_slots(sequences, length, rows, packed) * kv_heads, steps = ((packed ? rows : length) + 31) / 32 * (heads / kv_heads);
     const int64_t wanted = ((packed ? 2048 : causal ? 1024 : 512) + items - 1) / items;

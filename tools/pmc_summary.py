@@ -33,14 +33,14 @@ SCORE_KERNELS = SCORE_GEMM + PSG + ("conv_pad_phases_kernel", "pad_grid_kernel",
 
 
 def kernel_source_hash() -> str:
-    """sha256 over the sources of the kernels the summary reports -- every HIP source and header but the eigensolver's (same
+    """sha256 over the sources of the kernels the summary reports -- every HIP source and header but the eigensolver's and the model passes' (same
     function as bench.py's): identifies the code a profile was taken on."""
     digest = hashlib.sha256()
     paths = sorted(glob.glob(os.path.join(ROOT, "kronfluence_amd", "csrc", "*.hip")) + glob.glob(os.path.join(ROOT, "kronfluence_amd", "csrc", "*.h"))
                    + glob.glob(os.path.join(ROOT, "include", "*.h")))
     for path in paths:
-        if os.path.basename(path) == "kf_eigh.hip":
-            continue   # the eigensolver: none of its kernels is in the PMC summary (its evidence is the eigh logs under profiles/)
+        if os.path.basename(path) in ("kf_eigh.hip", "kf_attention.hip", "kf_norm.hip"):
+            continue   # none of their kernels is in the PMC summary (evidence: the eigh logs and model_ops_kernel_stats.csv under profiles/)
         with open(path, "rb") as handle:
             digest.update(os.path.basename(path).encode() + b"\0" + handle.read())
     return digest.hexdigest()
