@@ -20,8 +20,8 @@
 // kernels: 64 x 256 x 12 heads x 64, forward 131 to 84 us, backward 470 to 325; 2 x 2048 x 16 x 128 causal, 334 to 223 and 1129 to 817.
 // Finite values from 3.39e38 on (their first part rounds to infinity) act as infinities, parts below 2^-126 as 0.
 //
-// Measured (us; causal but for the first; forward, dq, dk / dv): bf16 256 x 128 x 12 heads x 64, padded: 37, 45, 48 (bound by prologue and
-// epilogue of one-tile sequences); 64 x 512 x 12 x 64: 61, 81, 97 and 16 x 512 x 32/8 x 128: 72, 106, 125 (vector instructions of the
+// Measured (us; causal but for the first; forward, dq, dk / dv): bf16 256 x <= 128 x 12 heads x 64, padded: 37, all of the backward 87 (latency
+// of one-tile sequences); 64 x 512 x 12 x 64: 61, 81, 97 and 16 x 512 x 32/8 x 128: 72, 106, 125 (vector instructions of the
 // softmax, few rounds of tiles); 1 x 8192 x 32/8 x 128: 572 (960 TFLOP/s), 777, 1087 + 28 (matrix instructions); fp32 24 x 29..233 x 12 x 64:
 // 27, 36, 43 (few, uneven workgroups).
 //
@@ -876,6 +876,190 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
     store_rows<T, DP>(av, lds, dv, a.dv.token, first, w.written, a.width, 1.0f, wave, lane);
 }
 
+// ---- backward of batches of 33 to ROWS tokens a row: all three gradients at once --------------------------------------------
+// One workgroup per (sequence, key / value head).  A wave owns 32 keys and meets all queries, as in the dk / dv kernel, and leaves ds in
+// LDS as [key][query]; then it owns 32 queries, and dq is the product of two transposed reads.  s, dp and the exponentials are computed
+// once instead of twice, the inputs read once.  Measured against the two kernels (bf16, 12 heads x 64): 256 x 128 tokens 118 us (144),
+// 512 x 64 tokens 124 (133), 1024 x 32 tokens 207 (189: those stay with the two kernels); 256 x 128 x 12 x 32 59 (93).  Bound by latency:
+// LDS and registers leave room for two workgroups, and each is load, products, store one after the other.
+template <int DP>
+struct Short {
+    typedef Image<__bf16, DP, ROWS> Img;       // q, do, k
+    typedef Image<__bf16, ROWS, ROWS> Grad;    // ds
+    static constexpr int G = Pass<__bf16, DP>::SCRATCH, STATS = Img::BYTES;   // results go out over q and the statistics
+    static constexpr int DS = G + Img::BYTES, LDS = DS + Grad::BYTES;   // (k and v pass through the place of ds first)
+    static_assert(2 * Img::BYTES <= Grad::BYTES, "k and v fit there");
+    static_assert(STATS + 2 * ROWS * 4 <= G && G % 64 == 0, "q and the statistics fit under the results' scratch");
+};
+template <int DP>
+__global__ __launch_bounds__(THREADS, DP <= 32 ? 3 : 2) void attention_short_backward_kernel(const Args a) {
+    typedef __bf16 T;
+    typedef Short<DP> S;
+    typedef typename S::Img Img;
+    extern __shared__ __align__(16) char lds[];   // [q, L, D][do, then k][ds]
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    Item item;
+    Place w;
+    if (!work_item(a, 1, item) || !locate(a, item.slot, false, w)) return;
+    const int kv_head = item.kv_head, first = 32 * wave, own = first + (lane & 31), blocks = (w.length + 31) / 32;
+    T* dk = rows_out<T>(a.dk, w, kv_head);
+    T* dv = rows_out<T>(a.dv, w, kv_head);
+    if (w.length == 0) {
+        zero_rows<T, DP>(dk, a.dk.token, 0, w.written, a.width, tid);
+        zero_rows<T, DP>(dv, a.dv.token, 0, w.written, a.width, tid);
+        for (int n = 0; n < a.group; ++n) zero_rows<T, DP>(rows_out<T>(a.dq, w, kv_head * a.group + n), a.dq.token, 0, w.written, a.width, tid);
+        return;
+    }
+    const Reader<T, DP, ROWS> read(lane);
+    const Reader<T, ROWS, ROWS> read_ds(lane);
+    const uint32_t qt = lds_address(lds), gt = qt + S::G, dt = qt + S::DS;
+    float* stats = reinterpret_cast<float*>(lds + S::STATS);   // [L, D][ROWS]
+    Held<T, DP> k, v;
+    f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
+    const float c = a.scale * LOG2E;
+    const Rows k_rows = input_rows<T>(a, a.k, w, kv_head), v_rows = input_rows<T>(a, a.v, w, kv_head);
+    Stage<T, DP, ROWS> sk(k_rows.token, k_rows.width, tid);
+    sk.load(k_rows.from(0));
+
+    for (int head = kv_head * a.group; head < (kv_head + 1) * a.group; ++head) {
+        {
+            const Rows q = input_rows<T>(a, a.q, w, head), g = input_rows<T>(a, a.g, w, head);
+            Stage<T, DP, ROWS> sq(q.token, q.width, tid), sg(g.token, g.width, tid);
+            sq.load(q.from(0));
+            sg.load(g.from(0));
+            const Rows o = input_rows<T>(a, a.o, w, head);
+            Stage<T, DP, ROWS> so(o.token, o.width, tid), sv(v_rows.token, v_rows.width, tid);
+            so.load(o.from(0));
+            if (head == kv_head * a.group) sv.load(v_rows.from(0));
+            float l = INFINITY;   // (p = 0 for rows that hold no token)
+            if (tid < ROWS && tid < w.length) l = a.lse[head * a.rows + w.stat + tid];
+            __syncthreads();   // (the head before: its dq is out, its ds read)
+            sq.store(lds);
+            sg.store(lds + S::G);
+            if (tid < ROWS) stats[tid] = l;
+            // D: four threads have a row's chunks, chunk i those of row tid / 4 + 64 (i % 2)
+            float delta[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < Stage<T, DP, ROWS>::PER; ++i) {
+                union { u32x4 u; bf16x8 f; } x, y;
+                x.u = so.r[i];
+                y.u = sg.r[i];
+                delta[i % 2] = Type<T>::dot(x.f, y.f, delta[i % 2]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                delta[i] += __shfl_xor(delta[i], 1);
+                delta[i] += __shfl_xor(delta[i], 2);
+                if (tid % 4 == 0) stats[ROWS + tid / 4 + 64 * i] = delta[i];
+            }
+            if (head == kv_head * a.group) {   // the wave's k and v, by way of the place of ds
+                sk.store(lds + S::DS);
+                sv.store(lds + S::DS + Img::BYTES);
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < Img::SLABS; ++i) {
+                    k.f[i] = read.rows(dt, first, i);
+                    v.f[i] = read.rows(dt + Img::BYTES, first, i);
+                }
+            }
+        }
+        __syncthreads();
+        if (a.causal || w.length <= 32) {   // rows that see 32 keys at most: D from p and dp (see the dq kernel)
+            if (wave == 0) {
+                f32x16 s = {}, dp = {};
+#pragma unroll
+                for (int i = 0; i < Img::SLABS; ++i) s = Type<T>::mma(k.f[i], read.rows(qt, 0, i), s);
+#pragma unroll
+                for (int i = 0; i < Img::SLABS; ++i) dp = Type<T>::mma(v.f[i], read.rows(gt, 0, i), dp);
+                settle();
+                const int visible = a.causal ? min(w.length, own + 1) : w.length;
+                const float l = stats[own];
+                float delta = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    delta = fmaf(8 * (r / 4) + 4 * half + r % 4 < visible ? __builtin_amdgcn_exp2f(fmaf(s[r], c, -l)) : 0.0f, dp[r], delta);
+                delta += other_half(delta);
+                if (half == 0) stats[ROWS + own] = own < w.length ? delta : 0.0f;
+            }
+            __syncthreads();
+        }
+        if (first < w.length) {
+            for (int b = a.causal ? wave : 0; b < blocks; ++b) {
+                f32x16 s = {}, dp = {};
+#pragma unroll
+                for (int i = 0; i < Img::SLABS; ++i) s = Type<T>::mma(read.rows(qt, 32 * b, i), k.f[i], s);
+#pragma unroll
+                for (int i = 0; i < Img::SLABS; ++i) dp = Type<T>::mma(read.rows(gt, 32 * b, i), v.f[i], dp);
+                const float* rows_lse = stats + 32 * b + 4 * half;
+                const float* rows_delta = rows_lse + ROWS;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(rows_lse + 8 * i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) s[4 * i + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * i + j], c, -l4[j]));
+                }
+                settle();
+                if ((a.causal & (b == wave)) | (first + 32 > w.length) | (w.length == 1)) {
+                    // rows of the block that do not see the key: those in front of it, or all
+                    const int hidden = own >= w.length ? 32 : a.causal ? own - 32 * b - 4 * half : -32;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (8 * (r / 4) + r % 4 < hidden) s[r] = 0.0f;
+                    // the first row of a causal sequence, or the only one, sees one key: ds is exactly 0
+                    if (32 * b + 4 * half == 0 && (a.causal || w.length == 1)) dp[0] = rows_delta[0];
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const bf16x8 p = Type<T>::from_acc(s, i);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) av[d] = Type<T>::mma(read.columns(gt, 32 * b, i, d), p, av[d]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(rows_delta + 8 * i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) dp[4 * i + j] = s[4 * i + j] * (dp[4 * i + j] - d4[j]);
+                    Type<T>::store4(lds + S::DS + b * S::Grad::BLOCK + own * 64 + ((i ^ (own >> 2)) & 3) * 16 + 8 * half, dp[4 * i], dp[4 * i + 1],
+                                    dp[4 * i + 2], dp[4 * i + 3]);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const bf16x8 ds = Type<T>::from_acc(dp, i);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) ak[d] = Type<T>::mma(read.columns(qt, 32 * b, i, d), ds, ak[d]);
+                }
+            }
+        }
+        __syncthreads();   // q and do are done with
+        sk.store(lds + S::G);
+        __syncthreads();
+        f32x16 aq[DP / 32] = {};
+        if (first < w.length) {
+            const int end = a.causal ? wave + 1 : blocks;
+            for (int b = 0; b < end; ++b)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const bf16x8 ds = read_ds.columns(dt, 32 * b, i, wave);
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) aq[d] = Type<T>::mma(read.columns(gt, 32 * b, i, d), ds, aq[d]);
+                }
+        }
+        settle();
+        if (own >= w.length) {
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) aq[d] = f32x16{};
+        }
+        store_rows<T, DP>(aq, lds, rows_out<T>(a.dq, w, head), a.dq.token, first, w.written, a.width, a.scale, wave, lane);
+    }
+    if (own >= w.length) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) { ak[d] = f32x16{}; av[d] = f32x16{}; }
+    }
+    store_rows<T, DP>(ak, lds, dk, a.dk.token, first, w.written, a.width, a.scale, wave, lane);
+    store_rows<T, DP>(av, lds, dv, a.dv.token, first, w.written, a.width, 1.0f, wave, lane);
+}
+
 // dk and dv as the sums of the parts in order; zero in rows of no sequence.  One thread per four columns.
 template <class T>
 __global__ __launch_bounds__(THREADS) void attention_join_kernel(const Args a) {
@@ -916,6 +1100,7 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(const Args a) {
 //   fp32: three, two and two waves: D 27, 36, 44 (two, one and one: 28.5, 38, 62); above width 64 the parts' registers leave one
 template <class T, int DP>
 struct Shape {
+    static constexpr bool SHORT = PARTS<T> == 1 && DP <= 64;   // wider heads and split values leave the LDS no room for two workgroups
     static constexpr bool SPLIT = PARTS<T> == 3, VL = !SPLIT && (DP == 64 || DP > 96);
     static constexpr int FORWARD_KEYS = !SPLIT && DP <= 64 ? 64 : 32, DQ_KEYS = !SPLIT && DP > 64 ? 64 : 32, QUERIES = !SPLIT && DP <= 32 ? 64 : 32;
     static constexpr int FORWARD_WAVES = SPLIT ? (DP <= 64 ? 3 : 1) : DP <= 64 ? 4 : 3, DQ_WAVES = SPLIT ? (DP <= 64 ? 2 : 1) : DP <= 64 ? 4 : 2;
@@ -935,6 +1120,8 @@ bool configure() {
     auto set = [](auto f, int bytes) {
         return hipFuncSetAttribute(reinterpret_cast<const void*>(f), hipFuncAttributeMaxDynamicSharedMemorySize, bytes) == hipSuccess;
     };
+    if constexpr (S::SHORT)
+        if (!set(&attention_short_backward_kernel<DP>, Short<DP>::LDS)) return false;
     return set(S::forward, S::FORWARD_LDS) && set(S::dq, S::DQ_LDS) && set(S::dkv, S::DKV_LDS);
 }
 
@@ -961,6 +1148,11 @@ int launch_width(Args& a, bool backward, hipStream_t stream) {
     if (!backward) {
         S::forward<<<items, THREADS, S::FORWARD_LDS, stream>>>(a);
     } else {
+        if constexpr (S::SHORT)
+            if (a.offsets == nullptr && a.length > 32 && a.length <= ROWS) {
+                attention_short_backward_kernel<DP><<<static_cast<unsigned>(slots), THREADS, Short<DP>::LDS, stream>>>(a);
+                return hipGetLastError() == hipSuccess ? KF_OK : KF_ERR_LAUNCH_FAILED;
+            }
         S::dq<<<items, THREADS, S::DQ_LDS, stream>>>(a);
         S::dkv<<<static_cast<unsigned>(slots * a.parts), THREADS, S::DKV_LDS, stream>>>(a);
         if (a.parts > 1) {

@@ -139,6 +139,20 @@ def test_attention_padded_rows_hold_anything(functional, dtype, causal, width):
         check_attention(functional, q, k, v, g, causal, spans, lengths=torch.tensor(lengths, dtype=kind, device="cuda"))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("length,heads,kv_heads,width", [(128, 4, 2, 64), (128, 3, 3, 32), (100, 4, 1, 48), (33, 2, 2, 64), (32, 2, 1, 8), (31, 6, 2, 40),
+                                                         (1, 2, 1, 64)])
+def test_attention_short_padded_batches(functional, causal, length, heads, kv_heads, width):
+    """Batches of at most 128 tokens a row (with more than 32 the backward pass is one kernel): every length around its blocks of 32, NaN behind the tokens."""
+    lengths = sorted({n for n in (0, 1, 2, 31, 32, 33, 63, 64, 65, 95, 96, 97, 127, 128, length) if n <= length})
+    q, k, v, g = (make((len(lengths), length, n, width), BF16, seed, scale)
+                  for n, seed, scale in ((heads, 1, 2.0), (kv_heads, 2, 1.0), (kv_heads, 3, 1.0), (heads, 4, 0.1)))
+    for i, n in enumerate(lengths):
+        q[i, n:], k[i, n:], v[i, n:], g[i, n:] = math.nan, math.inf, math.nan, -math.inf
+    spans = [(i, slice(0, n)) for i, n in enumerate(lengths) if n]
+    check_attention(functional, q, k, v, g, causal, spans, lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("heads,kv_heads,width", [(4, 1, 32), (2, 2, 64), (2, 1, 128)])
