@@ -40,7 +40,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
 
     Rows of no sequence (padding; packed rows behind the last offset) are 0 in the output and in every gradient, whatever the inputs
     hold there.  An infinity or NaN at a REAL token may reach every row of its sequence, as it does in the plain formula (0 * inf); float32
-    values from 3.39e38 on count as infinite.
+    values from 3.39e38 on count as infinite, and below 1e-33 their last bits may be lost.
     ``scale`` is positive and ``1 / sqrt(width)`` by default.
     """
     if torch.is_autocast_enabled("cuda") and q.is_cuda:

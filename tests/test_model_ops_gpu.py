@@ -351,6 +351,39 @@ def test_attention_and_norm_in_two_captured_graphs(functional):
                 assert torch.equal(a, e), turn
 
 
+@pytest.mark.parametrize("dtype,lengths,packed", [(BF16, [100, 64, 1, 0], False), (F32, [100, 64, 1, 0], False), (BF16, [300] * 30 + [0, 1, 77], True),
+                                                  (F32, [300] * 30 + [0, 1, 77], True)])
+def test_every_form_of_attention_captured(functional, dtype, lengths, packed):
+    """As above: short rows in one backward kernel, fp32, packed documents in order of cost with new offsets at every replay."""
+    heads, width, most = 4, 64, max(lengths)
+    shape = (sum(lengths) + 5, heads, width) if packed else (len(lengths), most, heads, width)
+    q, k, v = (make(shape, dtype, i + 1).requires_grad_() for i in range(3))
+    g = make(shape, dtype, 4, 0.1)
+
+    def rows(turn):
+        if not packed:
+            return torch.tensor([max(0, n - turn) for n in lengths], dtype=torch.int32, device="cuda")
+        turned = lengths[turn:] + lengths[:turn]
+        return torch.tensor([sum(turned[:i]) for i in range(len(turned) + 1)], dtype=torch.int32, device="cuda")
+
+    counts = rows(0)
+
+    def step():
+        out = functional.attention(q, k, v, **({"cu_seqlens": counts} if packed else {"lengths": counts}))
+        return (out.detach(),) + torch.autograd.grad(out, (q, k, v), g)
+
+    graph, got = capture(step)
+    for turn in range(3):
+        with torch.no_grad():
+            counts.copy_(rows(32 * turn if packed else turn))
+            q.copy_(make(shape, dtype, 60 + turn))
+        eager = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        for a, e in zip(got, eager):
+            assert torch.equal(a, e), turn
+
+
 def test_second_derivatives_are_refused(functional):
     """A graph of the gradients would silently lack these operators."""
     from kronfluence_amd._native import KfError
