@@ -8,8 +8,10 @@
 // Errors become KfError.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <cmath>
@@ -67,6 +69,21 @@ bool wants_graph(std::initializer_list<const Tensor*> tensors) {
 // The kernels' backward passes are not differentiable themselves: a graph of the gradients would silently lack these operators.
 void first_derivatives_only() {
     if (at::GradMode::is_enabled()) throw KfFailure("invalid argument: kronfluence_amd.functional has first derivatives only (create_graph=True)");
+}
+
+// The kernels read memory and write into fresh tensors: a forward-mode tangent, a node of a trace, or what a wrapper (torch.func's
+// transforms, a subclass with a dispatch of its own) stands for would be lost without a word.
+void plain_tensors(std::initializer_list<const Tensor*> tensors) {
+    constexpr c10::DispatchKeySet wrappers({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                            c10::DispatchKey::Functionalize, c10::DispatchKey::ZeroTensor});
+    for (const Tensor* t : tensors) {
+        if (!t->defined()) continue;
+        KF_REQUIRE(!t->key_set().has_any(wrappers),
+                   "kronfluence_amd.functional takes plain tensors (no torch.func transform, no subclass with a dispatch of its own)");
+        KF_REQUIRE(!t->_fw_grad(0).defined(), "kronfluence_amd.functional has no forward-mode derivatives (the tangent would be lost)");
+    }
+    KF_REQUIRE(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+               "kronfluence_amd.functional cannot be recorded in a trace");
 }
 
 Tensor given(const std::optional<Tensor>& t) { return t.has_value() ? *t : Tensor(); }
@@ -209,6 +226,7 @@ struct Attention : torch::autograd::Function<Attention> {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &lengths = saved[5], &offsets = saved[6];
         if (!grads[0].defined()) return variable_list(7);
+        plain_tensors({&grads[0]});
         const AttentionCall c = attention_call(q, k, v, lengths, offsets, ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
         variable_list d = attention_backward(c, grads[0], saved[3], saved[4], q, k, v, lengths, offsets, saved[7]);
         d.resize(7);
@@ -219,6 +237,7 @@ struct Attention : torch::autograd::Function<Attention> {
 Tensor attention(Tensor q, Tensor k, Tensor v, bool causal, const std::optional<double>& scale, const std::optional<Tensor>& lengths_,
                  const std::optional<Tensor>& offsets_) {
     Tensor lengths = given(lengths_), offsets = given(offsets_);
+    plain_tensors({&q, &k, &v, &lengths, &offsets});
     const int64_t width = q.dim() > 0 ? q.size(-1) : 0;
     const double by = scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(std::max<int64_t>(width, 1)));
     const AttentionCall c = attention_call(q, k, v, lengths, offsets, causal, by);
@@ -296,6 +315,7 @@ struct Norm : torch::autograd::Function<Norm> {
         Tensor weight = saved[1], grad = grads[0];
         variable_list d(6);
         if (!grad.defined()) return d;
+        plain_tensors({&grad});
         const int64_t bias = ctx->saved_data["bias"].toInt();
         NormCall c = norm_call(x, weight, Tensor());
         const auto plain = x.options().memory_format(at::MemoryFormat::Contiguous);
@@ -328,6 +348,7 @@ struct Norm : torch::autograd::Function<Norm> {
 
 Tensor norm(const Tensor& x, const std::optional<Tensor>& weight_, const std::optional<Tensor>& bias_, double eps, bool centred, at::ScalarType out_type) {
     const Tensor weight = given(weight_), bias = given(bias_);
+    plain_tensors({&x, &weight, &bias});
     KF_REQUIRE(out_type == at::kFloat || out_type == at::kBFloat16 || out_type == at::kHalf,
                std::string("norms return float32, bfloat16 or float16 tensors, not ") + c10::toString(out_type));
     KF_REQUIRE(std::isfinite(eps) && eps >= 0, "eps is finite and not negative");

@@ -11,7 +11,8 @@ transposed copy) and that grouped key / value heads, padded and packed batches n
 >>> h = functional.layer_norm(x, self.ln.weight, self.ln.bias, eps=self.ln.eps)
 
 Like the rest of the package they raise ``KfError`` for tensors that are not on an MI355X and for arguments the kernels do not take.
-First derivatives only (``create_graph=True`` is refused).  Under ``torch.autocast`` they cast as the torch operators do: attention runs
+First derivatives in reverse mode only: ``create_graph=True``, forward-mode tangents, ``torch.func`` transforms, traces and tensor subclasses
+with a dispatch of their own are refused.  Under ``torch.autocast`` they cast as the torch operators do: attention runs
 in the autocast dtype, a layer norm returns float32 (reading its input as it is, with no cast in between), an RMS norm its input's dtype.
 """
 
