@@ -478,6 +478,11 @@ __global__ __launch_bounds__(256) void eigh_update_kernel(double* __restrict__ W
                     acc[b] = __builtin_amdgcn_mfma_f64_16x16x4f64(a, bv, acc[b], 0, 0, 0);
                 }
             }
+            // The stores below stand behind branches.  A store of an fp64 matrix result needs 18 wait states after the instruction, and the
+            // compiler counted them along the path that takes the first store only: 12 where it is skipped and a later one is not.
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("s_nop 15\n\ts_nop 1");
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 const int64_t i = i0 + b * 16 + (lane & 15);
