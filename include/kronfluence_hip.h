@@ -440,7 +440,7 @@ int kf_mul_bcast(float* out, const void* X, int x_dtype, const float* M, int64_t
 int kf_cast(void* dst, int dst_dtype, const void* src, int src_dtype, int64_t numel, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
- * Model passes (ABI 15) -- the untracked parts of a transformer that every stage runs forward and
+ * Model passes (ABI 16) -- the untracked parts of a transformer that every stage runs forward and
  * backward between the tracked layers.  All of them: fp32 statistics, sums and accumulators, one
  * rounding of each output; no atomics (a result does not depend on the order of workgroups).
  * ------------------------------------------------------------------------------------------- */
@@ -463,17 +463,19 @@ typedef struct kf_heads_view {
  * Query head h reads key / value head h / (heads / kv_heads).
  *
  * Rows that hold no real token (padding; packed rows behind the last sequence) get out = 0 and, in the backward pass, gradients of
- * 0; what the inputs hold there is never used.  lse (fp32 [heads][rows], nullable in the forward call): log2 of the sum of
- * 2^(scale log2(e) q.k), +inf for rows without a token; the backward call needs it.
+ * 0; what the inputs hold there is never used.  stats (kf_attention_stats_bytes, 16-byte aligned, nullable in the forward call) is what
+ * the backward call of the same sizes reads: [heads][rows] log2 of the sum of 2^(scale log2(e) q.k) in fp32, +inf for rows without a
+ * token; then, for KF_BF16 where the backward call needs them, the eight bits of every element of out below its rounding.
  * width <= 128, a multiple of 8 (bf16) or 4 (fp32); scale > 0.
  */
-int kf_attention_forward(const kf_heads_view* out, float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v,
+int64_t kf_attention_stats_bytes(int dtype, int64_t length, int64_t rows, int64_t heads, int64_t width, int packed);
+int kf_attention_forward(const kf_heads_view* out, float* stats, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v,
                          int dtype, int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width,
                          const int32_t* lengths, const int32_t* offsets, const int32_t* order, int causal, float scale, void* stream);
 int64_t kf_attention_backward_workspace_bytes(int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width,
                                               int packed, int causal);
 int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, const kf_heads_view* dv, const kf_heads_view* grad,
-                          const kf_heads_view* out, const float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v,
+                          const kf_heads_view* out, const float* stats, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v,
                           int dtype, int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width,
                           const int32_t* lengths, const int32_t* offsets, const int32_t* order, int causal, float scale, void* workspace,
                           int64_t workspace_bytes, void* stream);

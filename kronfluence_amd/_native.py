@@ -15,7 +15,7 @@ from typing import Optional
 import torch  # noqa: F401  (must precede the dlopen below)
 
 LIB_NAME = "libkronfluence_hip.so"
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 KF_F32, KF_BF16, KF_F16, KF_F64, KF_I64, KF_I32, KF_U8 = range(7)
 
@@ -93,6 +93,7 @@ SIGNATURES = {
     "kf_cast": (_i, [_p, _i, _p, _i, _i64, _p]),
     "kf_attention_order_bytes": (_i64, [_i64, _i64, _i64]),
     "kf_attention_order": (_i, [_p, _p, _i64, _i64, _i, _p]),
+    "kf_attention_stats_bytes": (_i64, [_i] + [_i64] * 4 + [_i]),
     "kf_attention_forward": (_i, [_h, _p, _h, _h, _h, _i] + [_i64] * 6 + [_p, _p, _p, _i, _f, _p]),
     "kf_attention_backward_workspace_bytes": (_i64, [_i64] * 6 + [_i, _i]),
     "kf_attention_backward": (_i, [_h] * 5 + [_p] + [_h] * 3 + [_i] + [_i64] * 6 + [_p, _p, _p, _i, _f, _p, _i64, _p]),

@@ -20,14 +20,18 @@
 // kernels: 64 x 256 x 12 heads x 64, forward 131 to 84 us, backward 470 to 325; 2 x 2048 x 16 x 128 causal, 334 to 223 and 1129 to 817.
 // Finite values from 3.39e38 on (their first part rounds to infinity) act as infinities, parts below 2^-126 as 0.
 //
-// Measured (us; causal but for the first; forward, dq, dk / dv): bf16 256 x <= 128 x 12 heads x 64, padded: 37, all of the backward 87 (latency
-// of one-tile sequences); 64 x 512 x 12 x 64: 61, 81, 97 and 16 x 512 x 32/8 x 128: 72, 106, 125 (vector instructions of the
-// softmax, few rounds of tiles); 1 x 8192 x 32/8 x 128: 572 (960 TFLOP/s), 777, 1087 + 28 (matrix instructions); fp32 24 x 29..233 x 12 x 64:
-// 27, 36, 43 (few, uneven workgroups).
+// Measured (us; causal but for the first; forward, dq, dk / dv): bf16 256 x <= 128 x 12 heads x 64, padded: 38, all of the backward 83 (latency
+// of one-tile sequences); 64 x 512 x 12 x 64: 68, 86, 97 and 16 x 512 x 32/8 x 128: 80, 114, 126 (vector instructions of the
+// softmax, few rounds of tiles); 1 x 8192 x 32/8 x 128: 575 (956 TFLOP/s), 757, 1070 + 28; fp32 24 x 29..233 x 12 x 64: 27, 36, 44 (few, uneven
+// workgroups).  The low bytes of o cost the forward pass 7 and dq 6 us of the second of these.
 //
-// Roundings to fewer bits than 32: P and dS are rounded to bf16 as operands of their second product when the inputs are bf16 (one
-// rounding of half a step, 2^-9 relative, per term of a sum whose inputs carry the same rounding), and the outputs once at the end.
-// Maxima, sums, L, D and all accumulators are fp32.
+// Roundings to fewer bits than 32, all with bf16 inputs: P and dS as operands of their second product (half a step, at most 2^-8 of a term
+// of a sum whose inputs carry the same rounding), and the outputs once at the end.  Maxima, sums, L, D and all accumulators are fp32.
+// Neither rounding may enter D, which a peaked row's gradients are far below (a key that outweighs all others: p -> 1, ds -> 0).  So o is
+// divided by the sum of the ROUNDED p, and the forward pass keeps the next eight bits of o (at most 2^-15 of it is left): with e_j the
+// relative error of p_j, do_i . o_i is then off by sum_j p_j (e_j - sum_k p_k e_k) do_i . v_j = sum_j e_j ds_j, no more than dS's own rounding.
+// Measured against 64 bits, dq of 128 keys with scores of a standard deviation of 12: 0.30 % of its norm (0.28 % with the exact D, 0.71 %
+// from the rounded o over the sum of p alone); with one key 20 above the others nothing of the gradient was right.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -46,6 +50,7 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int THREADS = 256;      // 4 waves
 constexpr int ROWS = 128;         // rows (queries; keys in the dK / dV kernel) of a workgroup: 32 per wave
@@ -60,6 +65,7 @@ struct Tensor {   // [batch][token][head][width], the width contiguous; strides 
 struct Args {
     Tensor q, k, v, o, g;          // g: the gradient of o
     Tensor dq, dk, dv;
+    Tensor rest;                   // [heads][rows][rest_width(width)]: the low byte of o (see Low); or null
     float* lse;                    // [heads][rows]: L
     float* delta;                  // [heads][rows]: D
     float* partial;                // [parts][dk, dv][kv_heads][rows][width], if the dk / dv kernel's work is split (parts > 1)
@@ -104,6 +110,13 @@ struct Type<__bf16> {
         for (int i = 0; i < 8; ++i) acc = fmaf(static_cast<float>(a[i]), static_cast<float>(b[i]), acc);
         return acc;
     }
+    static __device__ __forceinline__ float total(Frag a, float acc) {   // two elements an instruction
+        typedef __bf16 Pair __attribute__((ext_vector_type(2)));
+        const Pair one = {static_cast<__bf16>(1.0f), static_cast<__bf16>(1.0f)};
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) acc = __builtin_amdgcn_fdot2_f32_bf16(Pair{a[i], a[i + 1]}, one, acc, false);
+        return acc;
+    }
 };
 
 template <>
@@ -111,6 +124,27 @@ struct Type<float> {                           // (the partial sums of the dk / 
     static __device__ __forceinline__ void store4(void* p, float a, float b, float c, float d) {
         f32x4 v = {a, b, c, d};
         *reinterpret_cast<f32x4*>(p) = v;
+    }
+};
+
+// The eight bits of a float below its rounding to bf16, signed: the two together are a float of 16 significant bits.  (Bit patterns of floats
+// ascend with their magnitude, so that the difference needs no look at the exponent.)
+struct Low {
+    int8_t byte;
+    static __device__ __forceinline__ uint32_t of(float x) {
+        const int below = static_cast<int>(__float_as_uint(x) - (static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<__bf16>(x))) << 16));
+        return static_cast<uint32_t>(min(below + 0x80, 0x7fff) >> 8) & 0xff;
+    }
+    static __device__ __forceinline__ float join(__bf16 high, uint32_t low, int byte) {   // byte `byte` of `low`
+        return __uint_as_float((static_cast<uint32_t>(__builtin_bit_cast(uint16_t, high)) << 16) + ((static_cast<int32_t>(low << (24 - 8 * byte)) >> 24) << 8));
+    }
+};
+__host__ __device__ constexpr int64_t rest_width(int64_t width) { return (width + 15) / 16 * 16; }   // (stored 16 bytes at a time)
+
+template <>
+struct Type<Low> {
+    static __device__ __forceinline__ void store4(void* p, float a, float b, float c, float d) {
+        *reinterpret_cast<uint32_t*>(p) = Low::of(a) | Low::of(b) << 8 | Low::of(c) << 16 | Low::of(d) << 24;
     }
 };
 
@@ -533,6 +567,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
     f32x16 acc[DP / 32] = {};
     const float c = a.scale * LOG2E;
     float top = -INFINITY, sum = 0.0f;   // a running reference near the maximum of c s; this half's part of the running sum
+    float weight = 0.0f;                 // (bf16: the sum of p as the second product's operand has it)
 
     const int end = a.causal ? min(w.length, w.row0 + ROWS) : w.length, tiles = (end + BK - 1) / BK;
     Stage<T, DP, BK> sk(k.token, k.width, tid), sv(v.token, v.width, tid);
@@ -577,6 +612,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
                 const float now = fmaxf(top, m), shrink = __builtin_amdgcn_exp2f(top - now);   // (m is finite where it is greater)
                 if (m > top + SLACK) {
                     sum *= shrink;
+                    weight *= shrink;
 #pragma unroll
                     for (int d = 0; d < DP / 32; ++d) acc[d] *= shrink;
                     top = now;
@@ -593,6 +629,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const Frag p = Type<T>::from_acc(s[b], i);
+                    if constexpr (PARTS<T> == 1) weight = Type<T>::total(p, weight);
 #pragma unroll
                     for (int d = 0; d < DP / 32; ++d) acc[d] = Type<T>::mma(read.columns(vt, 32 * b, i, d), p, acc[d]);
                 }
@@ -604,9 +641,18 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
         }
     }
     sum += other_half(sum);
+    weight = PARTS<T> == 1 ? weight + other_half(weight) : sum;
     const bool real = query < w.length;
+    const float by = real ? 1.0f / weight : 0.0f;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) acc[d] *= by;
     __syncthreads();
-    store_rows<T, DP>(acc, lds, o, a.o.token, first, w.written, a.width, real ? 1.0f / sum : 0.0f, wave, lane);
+    store_rows<T, DP>(acc, lds, o, a.o.token, first, w.written, a.width, 1.0f, wave, lane);
+    if constexpr (PARTS<T> == 1) {
+        static_assert(Pass<Low, DP>::STRIDE <= Pass<T, DP>::STRIDE, "in the same piece of the scratch as the wave's rows before");
+        if (a.rest.p)
+            store_rows<Low, DP>(acc, lds + wave * 32 * (Pass<T, DP>::STRIDE - Pass<Low, DP>::STRIDE), rows_out<Low>(a.rest, w, head), a.rest.token, first, w.length, static_cast<int>(rest_width(a.width)), 1.0f, wave, lane);
+    }
     if (lse && half == 0 && query < w.written) lse[query] = real ? top + __builtin_amdgcn_logf(sum) : INFINITY;
 }
 
@@ -639,8 +685,24 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dq_kernel(const Args
     {
         Held<T, DP> o;
         o.load(input_rows<T>(a, a.o, w, head), first, lane);
+        if constexpr (PARTS<T> == 1) {   // (no low bytes: rows of no length, zeros without touching memory)
+            const Rows rest{reinterpret_cast<const char*>(rows_of<Low>(a.rest, w, head)), a.rest.token, a.rest.p ? w.length : 0, a.width};
+            const __amdgpu_buffer_rsrc_t from = rest.from(first);
+            u32x2 low[Img::SLABS];
 #pragma unroll
-        for (int s = 0; s < Img::SLABS; ++s) delta = Type<T>::dot(o.f[s], g.f[s], delta);
+            for (int s = 0; s < Img::SLABS; ++s) {
+                const int column = 16 * s + 8 * half;
+                low[s] = __builtin_amdgcn_raw_buffer_load_b64(from, column < a.width ? static_cast<uint32_t>((lane & 31) * static_cast<int>(rest.token) + column)
+                                                                                     : NO_COLUMN, 0, 0);
+            }
+#pragma unroll
+            for (int s = 0; s < Img::SLABS; ++s)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) delta = fmaf(Low::join(o.f[s][i], low[s][i / 4], i % 4), static_cast<float>(g.f[s][i]), delta);
+        } else {
+#pragma unroll
+            for (int s = 0; s < Img::SLABS; ++s) delta = Type<T>::dot(o.f[s], g.f[s], delta);
+        }
         delta += other_half(delta);
     }
     const int64_t stat = head * a.rows + w.stat;
@@ -877,11 +939,11 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
 }
 
 // ---- backward of batches of 33 to ROWS tokens a row: all three gradients at once --------------------------------------------
-// One workgroup per (sequence, key / value head).  A wave owns 32 keys and meets all queries, as in the dk / dv kernel, and leaves ds in
-// LDS as [key][query]; then it owns 32 queries, and dq is the product of two transposed reads.  s, dp and the exponentials are computed
-// once instead of twice, the inputs read once.  Measured against the two kernels (bf16, 12 heads x 64): 256 x 128 tokens 118 us (144),
-// 512 x 64 tokens 124 (133), 1024 x 32 tokens 207 (189: those stay with the two kernels); 256 x 128 x 12 x 32 59 (93).  Bound by latency:
-// LDS and registers leave room for two workgroups, and each is load, products, store one after the other.
+// One workgroup per (sequence, key / value head).  A wave first owns 32 queries and takes their D from p and dp over all keys; then 32 keys,
+// and meets all queries, as in the dk / dv kernel, leaving ds in LDS as [key][query]; then 32 queries again, and dq is the product of two
+// transposed reads.  Seven products as in the two kernels, but the inputs are read once and o not at all.  Measured (backward, bf16, causal, 12 heads
+// x 64; the two kernels in brackets): 256 x 128 tokens 96 us (132), 512 x 64 112 (140), 1024 x 33 198 (224); 256 x 128 x 12 x 32 58 (93).
+// Bound by latency: LDS and registers leave room for two workgroups, and each is load, products, store one after the other.
 template <int DP>
 struct Short {
     typedef Image<__bf16, DP, ROWS> Img;       // q, do, k
@@ -929,61 +991,51 @@ __global__ __launch_bounds__(THREADS, DP <= 32 ? 3 : 2) void attention_short_bac
             sq.load(q.from(0));
             sg.load(g.from(0));
             const Rows o = input_rows<T>(a, a.o, w, head);
-            Stage<T, DP, ROWS> so(o.token, o.width, tid), sv(v_rows.token, v_rows.width, tid);
-            so.load(o.from(0));
-            if (head == kv_head * a.group) sv.load(v_rows.from(0));
+            Stage<T, DP, ROWS> sv(v_rows.token, v_rows.width, tid);
+            sv.load(v_rows.from(0));
             float l = INFINITY;   // (p = 0 for rows that hold no token)
             if (tid < ROWS && tid < w.length) l = a.lse[head * a.rows + w.stat + tid];
             __syncthreads();   // (the head before: its dq is out, its ds read)
             sq.store(lds);
             sg.store(lds + S::G);
+            sk.store(lds + S::DS);   // k and v pass through the place of ds
+            sv.store(lds + S::DS + Img::BYTES);
             if (tid < ROWS) stats[tid] = l;
-            // D: four threads have a row's chunks, chunk i those of row tid / 4 + 64 (i % 2)
-            float delta[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < Stage<T, DP, ROWS>::PER; ++i) {
-                union { u32x4 u; bf16x8 f; } x, y;
-                x.u = so.r[i];
-                y.u = sg.r[i];
-                delta[i % 2] = Type<T>::dot(x.f, y.f, delta[i % 2]);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                delta[i] += __shfl_xor(delta[i], 1);
-                delta[i] += __shfl_xor(delta[i], 2);
-                if (tid % 4 == 0) stats[ROWS + tid / 4 + 64 * i] = delta[i];
-            }
-            if (head == kv_head * a.group) {   // the wave's k and v, by way of the place of ds
-                sk.store(lds + S::DS);
-                sv.store(lds + S::DS + Img::BYTES);
-                __syncthreads();
-#pragma unroll
-                for (int i = 0; i < Img::SLABS; ++i) {
-                    k.f[i] = read.rows(dt, first, i);
-                    v.f[i] = read.rows(dt + Img::BYTES, first, i);
-                }
-            }
         }
         __syncthreads();
-        if (a.causal || w.length <= 32) {   // rows that see 32 keys at most: D from p and dp (see the dq kernel)
-            if (wave == 0) {
+        if (head == kv_head * a.group) {
+#pragma unroll
+            for (int i = 0; i < Img::SLABS; ++i) {
+                k.f[i] = read.rows(dt, first, i);
+                v.f[i] = read.rows(dt + Img::BYTES, first, i);
+            }
+        }
+        // D of the wave's 32 queries as the sum of p dp over their keys, in fp32: nothing of it is rounded, and o is not read
+        if (first < w.length) {
+            typename Type<T>::Frag q[Img::SLABS], g[Img::SLABS];
+#pragma unroll
+            for (int i = 0; i < Img::SLABS; ++i) {
+                q[i] = read.rows(qt, first, i);
+                g[i] = read.rows(gt, first, i);
+            }
+            const int visible = a.causal ? min(w.length, own + 1) : w.length, end = a.causal ? wave + 1 : blocks;
+            const float l = stats[own];
+            float delta = 0.0f;
+            for (int b = 0; b < end; ++b) {
                 f32x16 s = {}, dp = {};
 #pragma unroll
-                for (int i = 0; i < Img::SLABS; ++i) s = Type<T>::mma(k.f[i], read.rows(qt, 0, i), s);
+                for (int i = 0; i < Img::SLABS; ++i) s = Type<T>::mma(read.rows(dt, 32 * b, i), q[i], s);
 #pragma unroll
-                for (int i = 0; i < Img::SLABS; ++i) dp = Type<T>::mma(v.f[i], read.rows(gt, 0, i), dp);
+                for (int i = 0; i < Img::SLABS; ++i) dp = Type<T>::mma(read.rows(dt + Img::BYTES, 32 * b, i), g[i], dp);
                 settle();
-                const int visible = a.causal ? min(w.length, own + 1) : w.length;
-                const float l = stats[own];
-                float delta = 0.0f;
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    delta = fmaf(8 * (r / 4) + 4 * half + r % 4 < visible ? __builtin_amdgcn_exp2f(fmaf(s[r], c, -l)) : 0.0f, dp[r], delta);
-                delta += other_half(delta);
-                if (half == 0) stats[ROWS + own] = own < w.length ? delta : 0.0f;
+                    delta = fmaf(32 * b + 8 * (r / 4) + 4 * half + r % 4 < visible ? __builtin_amdgcn_exp2f(fmaf(s[r], c, -l)) : 0.0f, dp[r], delta);
             }
-            __syncthreads();
+            delta += other_half(delta);
+            if (half == 0) stats[ROWS + own] = own < w.length ? delta : 0.0f;
         }
+        __syncthreads();
         if (first < w.length) {
             for (int b = a.causal ? wave : 0; b < blocks; ++b) {
                 f32x16 s = {}, dp = {};
@@ -1140,6 +1192,12 @@ int configure_kernels() {
     return status[device];
 }
 
+// The rows that attention_short_backward_kernel takes: it and rows that see 32 keys at most have D from p and dp, and need no remainder.
+bool short_rows(int dtype, int64_t length, int64_t width, bool packed) { return dtype == KF_BF16 && !packed && length > 32 && length <= ROWS && width <= 64; }
+bool keeps_rest(int dtype, int64_t length, int64_t width, bool packed) {
+    return dtype == KF_BF16 && (packed || length > 32) && !short_rows(dtype, length, width, packed);
+}
+
 template <class T, int DP>
 int launch_width(Args& a, bool backward, hipStream_t stream) {
     typedef Shape<T, DP> S;
@@ -1149,7 +1207,7 @@ int launch_width(Args& a, bool backward, hipStream_t stream) {
         S::forward<<<items, THREADS, S::FORWARD_LDS, stream>>>(a);
     } else {
         if constexpr (S::SHORT)
-            if (a.offsets == nullptr && a.length > 32 && a.length <= ROWS) {
+            if (short_rows(KF_BF16, a.length, a.width, a.offsets != nullptr)) {
                 attention_short_backward_kernel<DP><<<static_cast<unsigned>(slots), THREADS, Short<DP>::LDS, stream>>>(a);
                 return hipGetLastError() == hipSuccess ? KF_OK : KF_ERR_LAUNCH_FAILED;
             }
@@ -1188,6 +1246,14 @@ int64_t dkv_parts(int64_t sequences, int64_t length, int64_t rows, int64_t heads
     const int64_t items = tile_slots(sequences, length, rows, packed) * kv_heads, steps = ((packed ? rows : length) + 31) / 32 * (heads / kv_heads);
     const int64_t wanted = ((packed ? 2048 : causal ? 1024 : 512) + items - 1) / items;
     return std::max<int64_t>(1, std::min(std::min(wanted, MAX_PARTS), steps / 128));
+}
+
+// the statistics that the forward call leaves for the backward one: L, and where it is kept the remainder
+void place_stats(Args& a, float* stats, int dtype, bool packed) {
+    a.lse = stats;
+    if (stats == nullptr || !keeps_rest(dtype, a.length, a.width, packed)) return;
+    const int64_t token = rest_width(a.width);
+    a.rest = Tensor{reinterpret_cast<const char*>(stats) + delta_bytes(a.rows, a.heads), packed ? 0 : a.length * token, token, a.rows * token};
 }
 
 Tensor tensor_of(const kf_heads_view* v) { return Tensor{v->p, v->batch_stride, v->token_stride, v->head_stride}; }
@@ -1249,18 +1315,25 @@ int kf_attention_order(int32_t* order, const int32_t* offsets, int64_t sequences
     return hipGetLastError() == hipSuccess ? KF_OK : KF_ERR_LAUNCH_FAILED;
 }
 
-int kf_attention_forward(const kf_heads_view* out, float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v, int dtype,
+int64_t kf_attention_stats_bytes(int dtype, int64_t length, int64_t rows, int64_t heads, int64_t width, int packed) {
+    if (rows <= 0 || heads <= 0 || width <= 0 || (!packed && length <= 0)) return 0;
+    return delta_bytes(rows, heads) + (keeps_rest(dtype, length, width, packed) ? rows * heads * rest_width(width) : 0);
+}
+
+int kf_attention_forward(const kf_heads_view* out, float* stats, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v, int dtype,
                          int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width, const int32_t* lengths,
                          const int32_t* offsets, const int32_t* order, int causal, float scale, void* stream) {
     Args a = {};
     if (int s = fill(a, dtype, sequences, length, rows, heads, kv_heads, width, lengths, offsets, causal, scale)) return s;
     const int64_t per = dtype == KF_BF16 ? 8 : 4;
-    if (!usable(out, per, width) || !usable(q, per, width) || !usable(k, per, width) || !usable(v, per, width)) return KF_ERR_INVALID_ARGUMENT;
+    if (!usable(out, per, width) || !usable(q, per, width) || !usable(k, per, width) || !usable(v, per, width) ||
+        reinterpret_cast<uintptr_t>(stats) % 16 != 0)
+        return KF_ERR_INVALID_ARGUMENT;
     if (order != nullptr && offsets == nullptr) return KF_ERR_INVALID_ARGUMENT;
     a.order = order;
     if (int s = configure_kernels()) return s;
     a.q = tensor_of(q); a.k = tensor_of(k); a.v = tensor_of(v); a.o = tensor_of(out);
-    a.lse = lse;
+    place_stats(a, stats, dtype, offsets != nullptr);
     const hipStream_t on = reinterpret_cast<hipStream_t>(stream);
     return dtype == KF_BF16 ? launch_type<__bf16>(a, false, on) : launch_type<Split>(a, false, on);
 }
@@ -1273,7 +1346,7 @@ int64_t kf_attention_backward_workspace_bytes(int64_t sequences, int64_t length,
 }
 
 int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, const kf_heads_view* dv, const kf_heads_view* grad, const kf_heads_view* out,
-                          const float* lse, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v, int dtype, int64_t sequences,
+                          const float* stats, const kf_heads_view* q, const kf_heads_view* k, const kf_heads_view* v, int dtype, int64_t sequences,
                           int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width, const int32_t* lengths, const int32_t* offsets,
                           const int32_t* order, int causal, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
     Args a = {};
@@ -1282,7 +1355,7 @@ int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, cons
     const kf_heads_view* all[] = {dq, dk, dv, grad, out, q, k, v};
     for (const kf_heads_view* t : all)
         if (!usable(t, per, width)) return KF_ERR_INVALID_ARGUMENT;
-    if (lse == nullptr) return KF_ERR_INVALID_ARGUMENT;
+    if (stats == nullptr || reinterpret_cast<uintptr_t>(stats) % 16 != 0) return KF_ERR_INVALID_ARGUMENT;
     if (workspace == nullptr ||
         workspace_bytes < kf_attention_backward_workspace_bytes(sequences, length, rows, heads, kv_heads, width, offsets != nullptr, causal))
         return KF_ERR_WORKSPACE_TOO_SMALL;
@@ -1291,7 +1364,7 @@ int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, cons
     if (int s = configure_kernels()) return s;
     a.q = tensor_of(q); a.k = tensor_of(k); a.v = tensor_of(v); a.o = tensor_of(out); a.g = tensor_of(grad);
     a.dq = tensor_of(dq); a.dk = tensor_of(dk); a.dv = tensor_of(dv);
-    a.lse = const_cast<float*>(lse);
+    place_stats(a, const_cast<float*>(stats), dtype, offsets != nullptr);
     a.delta = reinterpret_cast<float*>(workspace);
     a.partial = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + delta_bytes(rows, heads));
     a.parts = static_cast<int>(dkv_parts(sequences, length, rows, heads, kv_heads, offsets != nullptr, causal));

@@ -175,9 +175,10 @@ Tensor work_order(const AttentionCall& c, const Tensor& starts) {
 }
 
 // `lengths` and `offsets` come back as the kernels read them (a backward pass does not convert them again)
-Tensor attention_forward(const AttentionCall& c, Tensor q, Tensor k, Tensor v, Tensor& lengths, Tensor& offsets, Tensor* lse, Tensor* order_out) {
+Tensor attention_forward(const AttentionCall& c, Tensor q, Tensor k, Tensor v, Tensor& lengths, Tensor& offsets, Tensor* stats, Tensor* order_out) {
     Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
-    if (lse) *lse = at::empty({c.heads, c.rows}, q.options().dtype(at::kFloat));
+    if (stats)
+        *stats = at::empty({kf_attention_stats_bytes(c.dtype, c.length, c.rows, c.heads, c.width, offsets.defined()) / 4}, q.options().dtype(at::kFloat));
     if (c.empty()) return out.zero_();
     const c10::DeviceGuard guard(q.device());
     q = heads_operand(q); k = heads_operand(k); v = heads_operand(v);
@@ -186,14 +187,14 @@ Tensor attention_forward(const AttentionCall& c, Tensor q, Tensor k, Tensor v, T
     const Tensor order = work_order(c, offsets);
     if (order_out) *order_out = order;
     const kf_heads_view vo = view(out), vq = view(q), vk = view(k), vv = view(v);
-    check(kf_attention_forward(&vo, lse ? lse->data_ptr<float>() : nullptr, &vq, &vk, &vv, c.dtype, c.sequences, c.length, c.rows, c.heads, c.kv_heads, c.width,
+    check(kf_attention_forward(&vo, stats ? stats->data_ptr<float>() : nullptr, &vq, &vk, &vv, c.dtype, c.sequences, c.length, c.rows, c.heads, c.kv_heads, c.width,
                                static_cast<const int32_t*>(pointer(lengths)), static_cast<const int32_t*>(pointer(offsets)),
                                static_cast<const int32_t*>(pointer(order)), c.causal, c.scale, stream_of(q)),
           "kf_attention_forward");
     return out;
 }
 
-variable_list attention_backward(const AttentionCall& c, Tensor grad, Tensor out, const Tensor& lse, Tensor q, Tensor k, Tensor v, const Tensor& lengths,
+variable_list attention_backward(const AttentionCall& c, Tensor grad, Tensor out, const Tensor& stats, Tensor q, Tensor k, Tensor v, const Tensor& lengths,
                                  const Tensor& offsets, const Tensor& order) {
     const auto plain = q.options().memory_format(at::MemoryFormat::Contiguous);
     Tensor dq = at::empty(q.sizes(), plain), dk = at::empty(k.sizes(), plain), dv = at::empty(v.sizes(), plain);
@@ -204,7 +205,7 @@ variable_list attention_backward(const AttentionCall& c, Tensor grad, Tensor out
     const int64_t bytes = kf_attention_backward_workspace_bytes(c.sequences, c.length, c.rows, c.heads, c.kv_heads, c.width, offsets.defined(), c.causal);
     const Tensor workspace = at::empty({bytes}, q.options().dtype(at::kByte));
     const kf_heads_view vdq = view(dq), vdk = view(dk), vdv = view(dv), vg = view(grad), vo = view(out), vq = view(q), vk = view(k), vv = view(v);
-    check(kf_attention_backward(&vdq, &vdk, &vdv, &vg, &vo, lse.data_ptr<float>(), &vq, &vk, &vv, c.dtype, c.sequences, c.length, c.rows, c.heads, c.kv_heads,
+    check(kf_attention_backward(&vdq, &vdk, &vdv, &vg, &vo, stats.data_ptr<float>(), &vq, &vk, &vv, c.dtype, c.sequences, c.length, c.rows, c.heads, c.kv_heads,
                                 c.width, static_cast<const int32_t*>(pointer(counts)), static_cast<const int32_t*>(pointer(starts)),
                                 static_cast<const int32_t*>(pointer(order)), c.causal, c.scale, workspace.data_ptr(), bytes, stream_of(q)),
           "kf_attention_backward");
@@ -214,9 +215,9 @@ variable_list attention_backward(const AttentionCall& c, Tensor grad, Tensor out
 struct Attention : torch::autograd::Function<Attention> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& lengths_,
                           const std::optional<Tensor>& offsets_, bool causal, double scale) {
-        Tensor lengths = given(lengths_), offsets = given(offsets_), lse, order;
-        const Tensor out = attention_forward(attention_call(q, k, v, lengths, offsets, causal, scale), q, k, v, lengths, offsets, &lse, &order);
-        ctx->save_for_backward({q, k, v, out, lse, lengths, offsets, order});
+        Tensor lengths = given(lengths_), offsets = given(offsets_), stats, order;
+        const Tensor out = attention_forward(attention_call(q, k, v, lengths, offsets, causal, scale), q, k, v, lengths, offsets, &stats, &order);
+        ctx->save_for_backward({q, k, v, out, stats, lengths, offsets, order});
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["scale"] = scale;
         return out;

@@ -1,0 +1,118 @@
+"""Attention (kronfluence_amd/functional.py) where it is most easily wrong: rows of no sequence, rows whose softmax is peaked, batches that
+take the split or the dealt-out paths.  Bounds are those of tests/test_model_ops_gpu.py with a tighter one for D in bf16:
+
+D is the product of do with an output that carries its rounding remainder (an error of U^2 |out|) and that the ROUNDED p sum to one in:
+out = sum_j p_j (1 + e_j) v_j / (1 + sum_k p_k e_k), |e_j| <= U, so that to first order
+    D - D_exact = sum_j p_j (e_j - sum_k p_k e_k) dp_j = sum_j e_j p_j (dp_j - D_exact) = sum_j e_j ds_j
+-- at most U sum |ds_j| (and ep sum |ds_j| from p's own fp32 errors), however far do . out is above the gradients.  Beside it stand the fp32
+sums: (n + 16) E sum |do| (p |v|) and (2 width + 4) E sum |do| |out|."""
+
+import math
+
+import pytest
+import torch
+from test_model_ops_gpu import BF16, E, F32, HALF, close, make
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def functional():
+    from kronfluence_amd import functional
+
+    return functional
+
+
+def expected(q, k, v, g, causal, exact_rows=0):
+    """Values and bounds of one sequence and one kv head (``q``, ``g`` [n, group, width]; ``k``, ``v`` [n, width]): out, dq, dk, dv.  The first
+    ``exact_rows`` rows take D from p and dp in fp32."""
+    dtype = q.dtype
+    U, Up = HALF[dtype], HALF[dtype] if dtype == BF16 else 0.0
+    q, k, v, g = (t.double().transpose(0, 1) if t.dim() == 3 else t.double()[None] for t in (q, k, v, g))
+    group, n, width = q.shape
+    scale = 1.0 / math.sqrt(width)
+    s = scale * q @ k.transpose(1, 2)
+    if causal:
+        s = s.masked_fill(~torch.ones(n, n, dtype=torch.bool, device=s.device).tril(), -math.inf)
+    p = torch.softmax(s, dim=-1)
+    ep = (width + 8) * E * float((scale * q.abs() @ k.abs().transpose(1, 2)).max()) + (n + 16) * E
+    out, dp = p @ v, g @ v.transpose(1, 2)
+    delta = (p * dp).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    gv = g.abs() @ v.abs().transpose(1, 2)
+    if dtype == BF16:    # p_j (e_j - mean e) v_j = e_j p_j (v_j - out)
+        err_out = (ep + Up) * ((p @ v.abs()) + out.abs()) + n * E * (p @ v.abs()) + U * out.abs()
+        err_delta = ((ep + U) * (1 + 2 * U) * ds.abs().sum(-1, keepdim=True) + (n + 16) * E * (p * gv).sum(-1, keepdim=True)
+                     + (U * U + (2 * width + 4) * E) * (g.abs() * out.abs()).sum(-1, keepdim=True))
+    else:
+        err_out = (ep + n * E) * (p @ v.abs()) + U * out.abs()
+        err_delta = (g.abs() * err_out).sum(-1, keepdim=True) + (width + 2) * E * (g.abs() * out.abs()).sum(-1, keepdim=True)
+    if exact_rows:
+        few = (p * ((ep + (n + 4) * E) * dp.abs() + (width + 2) * E * gv)).sum(-1, keepdim=True)
+        err_delta = torch.where(torch.arange(n, device=s.device)[:, None] < exact_rows, few, err_delta)
+    err_ds = (ep + 2 * E + Up + (n + 2) * E) * ds.abs() + p * (err_delta + (width + 2) * E * gv) + E * p * (dp.abs() + delta.abs())
+    dq, dk, dv = scale * ds @ k, (scale * ds.transpose(1, 2) @ q).sum(0), (p.transpose(1, 2) @ g).sum(0)
+    err_dq = scale * err_ds @ k.abs() + U * dq.abs()
+    err_dk = (scale * err_ds.transpose(1, 2) @ q.abs()).sum(0) + group * n * E * (scale * ds.abs().transpose(1, 2) @ q.abs()).sum(0) + U * dk.abs()
+    err_dv = ((ep + Up + (group * n + 2) * E) * (p.transpose(1, 2) @ g.abs())).sum(0) + U * dv.abs()
+    last = lambda t: t.transpose(0, 1)
+    return (last(out), last(err_out)), (last(dq), last(err_dq)), (dk, err_dk), (dv, err_dv)
+
+
+def passes(functional, q, k, v, g, causal, **batch):
+    q, k, v = (t.detach().requires_grad_() for t in (q, k, v))
+    out = functional.attention(q, k, v, causal=causal, **batch)
+    return (out.detach(),) + torch.autograd.grad(out, (q, k, v), g)
+
+
+def check(functional, q, k, v, g, causal, spans, exact_rows=0, **batch):
+    """Every sequence against 64 bits; rows outside all of ``spans`` are 0."""
+    got = passes(functional, q, k, v, g, causal, **batch)
+    group = q.shape[-2] // k.shape[-2]
+    want = [torch.zeros(t.shape, dtype=torch.float64, device=t.device) for t in (q, q, k, v)]
+    bound = [torch.zeros_like(w) for w in want]
+    for span in spans:
+        for h in range(k.shape[-2]):
+            of = slice(h * group, (h + 1) * group)
+            for i, (value, error) in enumerate(expected(q[span][:, of], k[span][:, h], v[span][:, h], g[span][:, of], causal, exact_rows)):
+                want[i][span][:, of if i < 2 else h] = value
+                bound[i][span][:, of if i < 2 else h] = error
+    for name, a, w, b in zip(("out", "dq", "dk", "dv"), got, want, bound):
+        close(a, w, b, name)
+    return got
+
+
+# ------------------------------------------------------------------------------------------------
+# peaked rows: gradients far below do . out
+# ------------------------------------------------------------------------------------------------
+def peaked(shape, kv_shape, kind):
+    """bf16 q, k, v, g.  "sharp": random scores ten times the usual; "sink": the first key outweighs all the others together."""
+    q, k, v, g = make(shape, BF16, 1), make(kv_shape, BF16, 2), make(kv_shape, BF16, 3), make(shape, BF16, 4, 0.05)
+    if kind == "sharp":
+        return q * 10, k, v, g
+    q = (q.float() + 1.0).to(BF16)
+    k[..., 0, :, :] = {"sink": 1.25, "strong sink": 2.5}[kind]      # scores of 10 and 20 above the others
+    return q, k, v, g
+
+
+@pytest.mark.parametrize("kind", ["sharp", "sink", "strong sink"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("batch,length,heads,kv_heads,width", [
+    (2, 33, 2, 1, 64), (2, 64, 4, 2, 32), (2, 100, 2, 2, 64), (1, 128, 4, 1, 64),       # rows of the one-kernel backward
+    (2, 64, 2, 1, 128), (1, 129, 2, 1, 64), (1, 130, 2, 2, 96), (1, 513, 4, 1, 64), (1, 700, 2, 1, 128)])
+def test_gradients_of_peaked_rows(functional, kind, causal, batch, length, heads, kv_heads, width):
+    q, k, v, g = peaked((batch, length, heads, width), (batch, length, kv_heads, width), kind)
+    check(functional, q, k, v, g, causal, [(i, slice(0, length)) for i in range(batch)], exact_rows=32 if causal else 0)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv_heads,width,length", [(4, 1, 32, 33), (2, 2, 64, 40), (4, 2, 64, 128), (3, 3, 32, 100), (2, 1, 96, 64)])
+def test_few_keys_in_padded_rows(functional, causal, heads, kv_heads, width, length):
+    """Sequences of 2 to 32 tokens in longer rows (33 to 128 and width <= 64: the one-kernel backward): D to fp32's accuracy."""
+    lengths = [2, 2, 3, 5, 8, 17, 31, 32]
+    q, k, v, g = (make((len(lengths), length, n, width), BF16, seed, scale)
+                  for n, seed, scale in ((heads, 1, 3.0), (kv_heads, 2, 1.0), (kv_heads, 3, 1.0), (heads, 4, 0.05)))
+    for i, n in enumerate(lengths):
+        q[i, n:], k[i, n:], v[i, n:], g[i, n:] = math.nan, math.inf, math.nan, -math.inf
+    check(functional, q, k, v, g, causal, [(i, slice(0, n)) for i, n in enumerate(lengths)], exact_rows=32,
+          lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"))
