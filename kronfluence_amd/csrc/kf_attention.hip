@@ -643,9 +643,9 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
     sum += other_half(sum);
     weight = PARTS<T> == 1 ? weight + other_half(weight) : sum;
     const bool real = query < w.length;
-    const float by = real ? 1.0f / weight : 0.0f;
+    const float by = 1.0f / weight;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) acc[d] *= by;
+    for (int d = 0; d < DP / 32; ++d) acc[d] = real ? acc[d] * by : f32x16{};   // (a real token's infinity stays out of the rows of none)
     __syncthreads();
     store_rows<T, DP>(acc, lds, o, a.o.token, first, w.written, a.width, 1.0f, wave, lane);
     if constexpr (PARTS<T> == 1) {

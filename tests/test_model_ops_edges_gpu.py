@@ -1,7 +1,8 @@
 """Attention (kronfluence_amd/functional.py) where it is most easily wrong: rows of no sequence, rows whose softmax is peaked, batches that
 take the split or the dealt-out paths.  Bounds are those of tests/test_model_ops_gpu.py with a tighter one for D in bf16:
 
-D is the product of do with an output that carries its rounding remainder (an error of U^2 |out|) and that the ROUNDED p sum to one in:
+D is the product of do with an output that carries the next eight bits (a unit of them is 2^-8 of a bf16 step, 2^-15 |out| at most; rounded
+to half a unit, or to a whole one beside the tie that the signed byte does not reach: 2 U^2 |out|) and that the ROUNDED p sum to one in:
 out = sum_j p_j (1 + e_j) v_j / (1 + sum_k p_k e_k), |e_j| <= U, so that to first order
     D - D_exact = sum_j p_j (e_j - sum_k p_k e_k) dp_j = sum_j e_j p_j (dp_j - D_exact) = sum_j e_j ds_j
 -- at most U sum |ds_j| (and ep sum |ds_j| from p's own fp32 errors), however far do . out is above the gradients.  Beside it stand the fp32
@@ -43,7 +44,7 @@ def expected(q, k, v, g, causal, exact_rows=0):
     if dtype == BF16:    # p_j (e_j - mean e) v_j = e_j p_j (v_j - out)
         err_out = (ep + Up) * ((p @ v.abs()) + out.abs()) + n * E * (p @ v.abs()) + U * out.abs()
         err_delta = ((ep + U) * (1 + 2 * U) * ds.abs().sum(-1, keepdim=True) + (n + 16) * E * (p * gv).sum(-1, keepdim=True)
-                     + (U * U + (2 * width + 4) * E) * (g.abs() * out.abs()).sum(-1, keepdim=True))
+                     + (2 * U * U + (2 * width + 4) * E) * (g.abs() * out.abs()).sum(-1, keepdim=True))
     else:
         err_out = (ep + n * E) * (p @ v.abs()) + U * out.abs()
         err_delta = (g.abs() * err_out).sum(-1, keepdim=True) + (width + 2) * E * (g.abs() * out.abs()).sum(-1, keepdim=True)
@@ -80,6 +81,29 @@ def check(functional, q, k, v, g, causal, spans, exact_rows=0, **batch):
     for name, a, w, b in zip(("out", "dq", "dk", "dv"), got, want, bound):
         close(a, w, b, name)
     return got
+
+
+def offsets_of(lengths, kind=torch.int32):
+    return torch.tensor([sum(lengths[:i]) for i in range(len(lengths) + 1)], dtype=kind, device="cuda")
+
+
+# ------------------------------------------------------------------------------------------------
+# rows of no sequence
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("width", [64, 128])
+def test_padding_beside_an_infinite_value(functional, dtype, causal, width):
+    """Padding rows that share a block of 32 with real ones stay 0 although a real token's v is infinite (its own rows may be anything)."""
+    lengths = [3, 33, 64, 100, 1]
+    q, k, v, g = (make((len(lengths), 150, 2, width), dtype, i, 1.0 if i < 4 else 0.1) for i in (1, 2, 3, 4))
+    v[:, 0, :, 5], v[:, 0, :, 6] = math.inf, math.nan
+    got = passes(functional, q, k, v, g, causal, lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+    packed = [torch.cat([t[i, :n] for i, n in enumerate(lengths)] + [t[0, :20]]) for t in (q, k, v, g)]
+    rows = passes(functional, *packed, causal, cu_seqlens=offsets_of(lengths))
+    for name, a, b in zip(("out", "dq", "dk", "dv"), got, rows):
+        assert all(not a[i, n:].any() for i, n in enumerate(lengths)), name
+        assert not b[sum(lengths):].any(), name
 
 
 # ------------------------------------------------------------------------------------------------
