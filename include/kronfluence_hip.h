@@ -458,11 +458,11 @@ typedef struct kf_heads_view {
  *
  * Padded batch (offsets == NULL): `sequences` rows of `length` tokens, rows = sequences * length; lengths (device int32
  * [sequences], nullable) gives the real tokens of each row, the first ones.  Packed batch: sequence s is token rows
- * offsets[s] .. offsets[s + 1] (device int32 [sequences + 1]) of `rows` in all; lengths == NULL, `length` ignored.  Values are
- * clamped to the rows that exist.  causal: token i sees tokens 0 .. i of its sequence, otherwise every real token of it.
+ * offsets[s] .. offsets[s + 1] (device int32 [sequences + 1], ASCENDING: kf_attention_starts makes them so) of `rows` in all; lengths ==
+ * NULL, `length` ignored.  Values are clamped to the rows that exist.  causal: token i sees tokens 0 .. i of its sequence, otherwise every real token of it.
  * Query head h reads key / value head h / (heads / kv_heads).
  *
- * Rows that hold no real token (padding; packed rows behind the last sequence) get out = 0 and, in the backward pass, gradients of
+ * Rows that hold no real token (padding; packed rows in front of the first or behind the last sequence) get out = 0 and, in the backward pass, gradients of
  * 0; what the inputs hold there is never used.  stats (kf_attention_stats_bytes, 16-byte aligned, nullable in the forward call) is what
  * the backward call of the same sizes reads: [heads][rows] log2 of the sum of 2^(scale log2(e) q.k) in fp32, +inf for rows without a
  * token; then, for KF_BF16 where the backward call needs them, the eight bits of every element of out below its rounding.
@@ -479,6 +479,9 @@ int kf_attention_backward(const kf_heads_view* dq, const kf_heads_view* dk, cons
                           int dtype, int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, int64_t width,
                           const int32_t* lengths, const int32_t* offsets, const int32_t* order, int causal, float scale, void* workspace,
                           int64_t workspace_bytes, void* stream);
+/* Packed batches: kf_attention_starts writes the offsets (KF_I32 or KF_I64 [sequences + 1]) clamped to [0, rows], each at least the one before
+ * it, as int32: rows that fall in no sequence are then those in front of the first and behind the last, whatever the offsets hold. */
+int kf_attention_starts(int32_t* starts, const void* offsets, int offsets_dtype, int64_t sequences, int64_t rows, void* stream);
 /* Packed batches: kf_attention_order writes the order in which the tiles of the batch are best worked on (the longest documents first),
  * to be handed to the forward and the backward call of the same offsets (nullable there; it changes no result).
  * kf_attention_order_bytes is 0 where an order gains nothing. */

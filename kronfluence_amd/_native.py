@@ -92,6 +92,7 @@ SIGNATURES = {
     "kf_mul_bcast": (_i, [_p, _p, _i, _p, _i64, _i64, _f, _p]),
     "kf_cast": (_i, [_p, _i, _p, _i, _i64, _p]),
     "kf_attention_order_bytes": (_i64, [_i64, _i64, _i64]),
+    "kf_attention_starts": (_i, [_p, _p, _i, _i64, _i64, _p]),
     "kf_attention_order": (_i, [_p, _p, _i64, _i64, _i, _p]),
     "kf_attention_stats_bytes": (_i64, [_i] + [_i64] * 4 + [_i]),
     "kf_attention_forward": (_i, [_h, _p, _h, _h, _h, _i] + [_i64] * 6 + [_p, _p, _p, _i, _f, _p]),

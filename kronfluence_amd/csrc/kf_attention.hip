@@ -338,7 +338,8 @@ struct Place {
 
 // Tile slots.  Padded batch: ceil(length / ROWS) per sequence.  Packed batch: sequence s takes slots [c_s / ROWS + s,
 // c_{s+1} / ROWS + s + 1) with c the offsets -- at least ceil(len / ROWS) of them, found by a binary search without a table or a
-// host copy of the offsets; the rows behind the last sequence are one more sequence of no visible tokens.  Offsets outside
+// host copy of the offsets; the rows behind the last sequence are one more sequence of no visible tokens.  So are the rows in front of
+// the first one: they take the slots below c_0 / ROWS, and their last, partial tile the slot behind all others.  Offsets outside
 // [0, rows] are clamped, so that no content of the offsets can send an access out of bounds.
 __device__ __forceinline__ bool locate(const Args& a, int slot, bool last_first, Place& w) {
     if (a.offsets == nullptr) {
@@ -352,6 +353,14 @@ __device__ __forceinline__ bool locate(const Args& a, int slot, bool last_first,
     const int total = static_cast<int>(a.rows);
     auto offset = [&](int s) { return s > a.sequences ? total : min(max(a.offsets[s], 0), total); };
     auto first_slot = [&](int s) { return offset(s) / ROWS + s; };
+    const int front = offset(0);
+    if (slot < front / ROWS || slot == total / ROWS + a.sequences + 1) {
+        w.sequence = 0; w.start = 0; w.stat = 0;
+        w.written = front;
+        w.length = 0;
+        w.row0 = min(slot, front / ROWS) * ROWS;
+        return w.row0 < front;
+    }
     int lo = 0, hi = a.sequences;   // first_slot(lo) <= slot; the last such
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -393,7 +402,7 @@ __device__ __forceinline__ bool work_item(const Args& a, int members, Item& w) {
     w.kv_head = static_cast<int>(unit % kv_heads);
     w.slot = static_cast<int>(unit / kv_heads * a.chunk + tile);
     if (unit * a.chunk + tile >= static_cast<int64_t>(a.slots) * kv_heads) return false;
-    if (a.order) w.slot = a.order[w.slot];
+    if (a.order && w.slot < a.slots - 1) w.slot = a.order[w.slot];   // (the last slot, of the rows in front, is not among those ordered)
     return true;
 }
 
@@ -430,6 +439,34 @@ __global__ __launch_bounds__(1024) void attention_order_kernel(const Args a, int
     place[high - 1] = before + n0;
     __syncthreads();
     for (int s = threadIdx.x; s < a.slots; s += 1024) order[atomicAdd(&place[cost_of(s)], 1)] = s;
+}
+
+// Offsets as the kernels above take them: clamped to the rows, and none below one before it.  One workgroup, a running maximum.
+__global__ __launch_bounds__(1024) void attention_starts_kernel(int32_t* starts, const void* offsets, bool wide, int64_t count, int64_t rows) {
+    __shared__ int top[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int before = 0;   // the maximum of all earlier offsets
+    for (int64_t base = 0; base < count; base += 1024) {
+        const int64_t i = base + threadIdx.x;
+        int x = 0;
+        if (i < count) {
+            const int64_t given = wide ? reinterpret_cast<const int64_t*>(offsets)[i] : reinterpret_cast<const int32_t*>(offsets)[i];
+            x = static_cast<int>(min(max(given, int64_t{0}), rows));
+        }
+#pragma unroll
+        for (int step = 1; step < 64; step *= 2) {
+            const int other = __shfl_up(x, step);
+            if (lane >= step) x = max(x, other);
+        }
+        if (lane == 63) top[wave] = x;
+        __syncthreads();
+        for (int n = 0; n < 16; ++n) {
+            if (n == wave) x = max(x, before);
+            before = max(before, top[n]);   // (for every wave that of the whole block in the end)
+        }
+        if (i < count) starts[i] = x;
+        __syncthreads();
+    }
 }
 
 template <class T>
@@ -919,6 +956,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
 #pragma unroll
                 for (int d = 0; d < DP / 32; ++d) ak[d] = Type<T>::mma(read.columns(qt, 32 * b, i, d), ds, ak[d]);
             }
+            if constexpr (PARTS<T> == 3 && DP > 64) settle();   // (the accumulators leave their registers where the loop ends)
         }
         if (n + 1 < steps) store(lds + ((n + 1) & 1) * STAGE);
     }
@@ -1123,7 +1161,7 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(const Args a) {
     int64_t sequence = 0, token = row;
     bool real;
     if (a.offsets) {
-        real = row < a.offsets[a.sequences];
+        real = row >= a.offsets[0] && row < a.offsets[a.sequences];
     } else {
         sequence = row / a.length;
         token = row % a.length;
@@ -1229,6 +1267,7 @@ int launch_type(Args& a, bool backward, hipStream_t stream) {
     return launch_width<T, 128>(a, backward, stream);
 }
 
+// (packed: without the last slot, which holds a tile of the rows in front of the first sequence at most)
 int64_t tile_slots(int64_t sequences, int64_t length, int64_t rows, bool packed) {
     return packed ? rows / ROWS + sequences + 1 : sequences * ((length + ROWS - 1) / ROWS);
 }
@@ -1273,7 +1312,7 @@ int fill(Args& a, int dtype, int64_t sequences, int64_t length, int64_t rows, in
         width % per != 0 || !(scale > 0.0f) || !isfinite(scale))
         return KF_ERR_INVALID_ARGUMENT;
     if (offsets ? lengths != nullptr : (length <= 0 || sequences > limit / length || rows != sequences * length)) return KF_ERR_INVALID_ARGUMENT;
-    const int64_t slots = tile_slots(sequences, length, rows, offsets != nullptr);
+    const int64_t slots = tile_slots(sequences, length, rows, offsets != nullptr) + (offsets != nullptr);
     const int64_t tiles = offsets ? 0 : slots / sequences, groups = offsets ? 0 : sequences * kv_heads;
     const int64_t chunk = groups >= 64 ? tiles : 1;
     if (sequences >= limit || slots > (limit / MAX_PARTS - XCDS * chunk * heads) / heads) return KF_ERR_INVALID_ARGUMENT;
@@ -1300,6 +1339,13 @@ int64_t kf_attention_order_bytes(int64_t sequences, int64_t rows, int64_t heads)
     if (sequences <= 0 || rows <= 0 || heads <= 0) return 0;
     const int64_t slots = tile_slots(sequences, 0, rows, true);
     return slots <= MAX_ORDERED && slots * heads > RESIDENT ? slots * 4 : 0;
+}
+
+int kf_attention_starts(int32_t* starts, const void* offsets, int offsets_dtype, int64_t sequences, int64_t rows, void* stream) {
+    if (offsets_dtype != KF_I32 && offsets_dtype != KF_I64) return KF_ERR_UNSUPPORTED_DTYPE;
+    if (starts == nullptr || offsets == nullptr || sequences < 0 || rows < 0 || rows > 0x7fffffff) return KF_ERR_INVALID_ARGUMENT;
+    attention_starts_kernel<<<1, 1024, 0, reinterpret_cast<hipStream_t>(stream)>>>(starts, offsets, offsets_dtype == KF_I64, sequences + 1, rows);
+    return hipGetLastError() == hipSuccess ? KF_OK : KF_ERR_LAUNCH_FAILED;
 }
 
 int kf_attention_order(int32_t* order, const int32_t* offsets, int64_t sequences, int64_t rows, int causal, void* stream) {

@@ -159,10 +159,20 @@ kf_heads_view view(const Tensor& t) {   // (an axis of one element may carry any
                          t.size(dims - 2) > 1 ? t.stride(dims - 2) : 0};
 }
 
-// lengths / offsets as the kernels read them: contiguous int32, which they clamp to the rows that exist
+// lengths as the kernels read them: contiguous int32, which they clamp to the rows that exist
 Tensor row_counts(const Tensor& t, int64_t most) {
     if (!t.defined()) return t;
     return (t.scalar_type() == at::kInt ? t : t.clamp(0, most).to(at::kInt)).contiguous();
+}
+
+// offsets as the kernels read them: int32, within the rows and ascending, whatever the caller's say
+Tensor row_starts(const AttentionCall& c, const Tensor& offsets) {
+    if (!offsets.defined()) return offsets;
+    const Tensor given = offsets.contiguous(), starts = at::empty({c.sequences + 1}, offsets.options().dtype(at::kInt));
+    check(kf_attention_starts(starts.data_ptr<int32_t>(), given.data_ptr(), given.scalar_type() == at::kLong ? KF_I64 : KF_I32, c.sequences, c.rows,
+                              stream_of(given)),
+          "kf_attention_starts");
+    return starts;
 }
 
 // the order a packed batch is best worked on in, or an undefined tensor
@@ -174,7 +184,7 @@ Tensor work_order(const AttentionCall& c, const Tensor& starts) {
     return order;
 }
 
-// `lengths` and `offsets` come back as the kernels read them (a backward pass does not convert them again)
+// `lengths` and `offsets` come back as the kernels read them, for the backward pass
 Tensor attention_forward(const AttentionCall& c, Tensor q, Tensor k, Tensor v, Tensor& lengths, Tensor& offsets, Tensor* stats, Tensor* order_out) {
     Tensor out = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
     if (stats)
@@ -183,7 +193,7 @@ Tensor attention_forward(const AttentionCall& c, Tensor q, Tensor k, Tensor v, T
     const c10::DeviceGuard guard(q.device());
     q = heads_operand(q); k = heads_operand(k); v = heads_operand(v);
     lengths = row_counts(lengths, c.length);
-    offsets = row_counts(offsets, c.rows);
+    offsets = row_starts(c, offsets);
     const Tensor order = work_order(c, offsets);
     if (order_out) *order_out = order;
     const kf_heads_view vo = view(out), vq = view(q), vk = view(k), vv = view(v);
@@ -201,12 +211,11 @@ variable_list attention_backward(const AttentionCall& c, Tensor grad, Tensor out
     if (c.empty()) return {dq.zero_(), dk.zero_(), dv.zero_()};
     const c10::DeviceGuard guard(q.device());
     grad = heads_operand(grad); out = heads_operand(out); q = heads_operand(q); k = heads_operand(k); v = heads_operand(v);
-    const Tensor counts = row_counts(lengths, c.length), starts = row_counts(offsets, c.rows);
     const int64_t bytes = kf_attention_backward_workspace_bytes(c.sequences, c.length, c.rows, c.heads, c.kv_heads, c.width, offsets.defined(), c.causal);
     const Tensor workspace = at::empty({bytes}, q.options().dtype(at::kByte));
     const kf_heads_view vdq = view(dq), vdk = view(dk), vdv = view(dv), vg = view(grad), vo = view(out), vq = view(q), vk = view(k), vv = view(v);
     check(kf_attention_backward(&vdq, &vdk, &vdv, &vg, &vo, stats.data_ptr<float>(), &vq, &vk, &vv, c.dtype, c.sequences, c.length, c.rows, c.heads, c.kv_heads,
-                                c.width, static_cast<const int32_t*>(pointer(counts)), static_cast<const int32_t*>(pointer(starts)),
+                                c.width, static_cast<const int32_t*>(pointer(lengths)), static_cast<const int32_t*>(pointer(offsets)),
                                 static_cast<const int32_t*>(pointer(order)), c.causal, c.scale, workspace.data_ptr(), bytes, stream_of(q)),
           "kf_attention_backward");
     return {dq, dk, dv};

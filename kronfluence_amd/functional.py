@@ -36,10 +36,10 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     ``width <= 128``; any strides (a contiguous last axis and 16-byte aligned rows are read in place, others are copied).
 
     ``lengths`` (``[batch]``, int32 / int64 on the device) counts the real tokens of each row, the first ones; ``cu_seqlens``
-    (``[sequences + 1]``, the first row of every sequence, ascending from 0) cuts a packed batch.  Entries are clamped to the rows
-    that exist; neither is read by the host.  A token sees the tokens of its own sequence, with ``causal`` those up to itself.
+    (``[sequences + 1]``, the first row of every sequence and the last one's end, ascending) cuts a packed batch.  Entries are clamped to
+    the rows that exist, and an offset below one before it counts as that one (its sequence is empty); neither is read by the host.  A token sees the tokens of its own sequence, with ``causal`` those up to itself.
 
-    Rows of no sequence (padding; packed rows behind the last offset) are 0 in the output and in every gradient, whatever the inputs
+    Rows of no sequence (padding; packed rows in front of the first offset or behind the last) are 0 in the output and in every gradient, whatever the inputs
     hold there.  An infinity or NaN at a REAL token may reach every row of its sequence, as it does in the plain formula (0 * inf); float32
     values from 3.39e38 on count as infinite, and below 1e-33 their last bits may be lost.
     ``scale`` is positive and ``1 / sqrt(width)`` by default.  A bfloat16 call with a graph keeps, beside q, k, v and the output, 8 bits per

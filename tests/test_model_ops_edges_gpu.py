@@ -83,6 +83,13 @@ def check(functional, q, k, v, g, causal, spans, exact_rows=0, **batch):
     return got
 
 
+def poison(*shapes):
+    """Blocks of the sizes that the call will allocate, filled with NaN and given back to the allocator."""
+    blocks = [torch.full(shape, math.nan, dtype=dtype, device="cuda") for shape, dtype in shapes for _ in range(8)]
+    torch.cuda.synchronize()
+    del blocks
+
+
 def offsets_of(lengths, kind=torch.int32):
     return torch.tensor([sum(lengths[:i]) for i in range(len(lengths) + 1)], dtype=kind, device="cuda")
 
@@ -104,6 +111,65 @@ def test_padding_beside_an_infinite_value(functional, dtype, causal, width):
     for name, a, b in zip(("out", "dq", "dk", "dv"), got, rows):
         assert all(not a[i, n:].any() for i, n in enumerate(lengths)), name
         assert not b[sum(lengths):].any(), name
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+@pytest.mark.parametrize("front,lengths,tail", [(1, [5], 0), (127, [1, 130], 3), (128, [64], 0), (300, [0, 129, 7], 200), (129, [], 5), (257, [0], 0),
+                                                (140, [30] * 40, 1)])
+def test_packed_rows_in_front_of_the_first_sequence(functional, dtype, causal, kind, front, lengths, tail):
+    """cu_seqlens that starts above 0: the rows in front belong to no sequence, whatever they and the allocator's memory hold."""
+    total = front + sum(lengths) + tail
+    q, g = make((total, 4, 64), dtype, 1), make((total, 4, 64), dtype, 4, 0.1)
+    k, v = make((total, 2, 64), dtype, 2), make((total, 2, 64), dtype, 3)
+    for t in (q, k, v, g):
+        t[:front], t[total - tail:] = math.nan, math.nan
+    offsets = offsets_of(lengths, kind) + front
+    spans = [(slice(a, b),) for a, b in zip(offsets.tolist(), offsets.tolist()[1:]) if b > a]
+    poison((q.shape, dtype), (k.shape, dtype))
+    check(functional, q, k, v, g, causal, spans, cu_seqlens=offsets)
+
+
+@pytest.mark.parametrize("front,lengths,heads,kv_heads,dtype", [(200, [900, 3, 0, 500], 32, 1, BF16), (77, [1100], 32, 1, F32), (1, [1200, 40], 64, 2, BF16)])
+def test_packed_rows_in_front_where_tiles_are_ordered_and_split(functional, front, lengths, heads, kv_heads, dtype):
+    from kronfluence_amd import _native
+
+    total = front + sum(lengths) + 9
+    call = (len(lengths), 0, total, heads, kv_heads, 32, 1, 1)
+    assert _native.lib().kf_attention_backward_workspace_bytes(*call) > 8 * total * heads     # dk and dv in parts
+    q, g = make((total, heads, 32), dtype, 1), make((total, heads, 32), dtype, 4, 0.1)
+    k, v = make((total, kv_heads, 32), dtype, 2), make((total, kv_heads, 32), dtype, 3)
+    for t in (q, k, v, g):
+        t[:front], t[total - 9:] = math.nan, math.nan
+    offsets = offsets_of(lengths) + front
+    spans = [(slice(a, b),) for a, b in zip(offsets.tolist(), offsets.tolist()[1:]) if b > a]
+    poison((q.shape, dtype), (k.shape, dtype), ((total * heads * 40,), F32))
+    check(functional, q, k, v, g, True, spans, cu_seqlens=offsets)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+@pytest.mark.parametrize("offsets,total", [([0, 100, 60, 200], 210), ([50, 20, 180, 170, 260], 300), ([0, 500, 100], 300), ([-7, 40, 1 << 30], 130),
+                                           ([90, 0], 140), ([200] + list(range(0, 1400)) + [1300], 1500)])
+def test_offsets_that_do_not_ascend(functional, dtype, kind, offsets, total):
+    """Offsets outside the rows are clamped, and one below the one before it counts as that one: every row is written once."""
+    if kind == torch.int64:
+        offsets = [n if n < 1 << 30 else 1 << 40 for n in offsets]
+    q, g = make((total, 2, 64), dtype, 1), make((total, 2, 64), dtype, 4, 0.1)
+    k, v = make((total, 1, 64), dtype, 2), make((total, 1, 64), dtype, 3)
+    ascending, most = [], 0
+    for n in offsets:
+        most = max(most, min(max(n, 0), total))
+        ascending.append(most)
+    poison((q.shape, dtype), (k.shape, dtype))
+    got = passes(functional, q, k, v, g, True, cu_seqlens=torch.tensor(offsets, dtype=kind, device="cuda"))
+    want = passes(functional, q, k, v, g, True, cu_seqlens=torch.tensor(ascending, dtype=kind, device="cuda"))
+    for name, a, b in zip(("out", "dq", "dk", "dv"), got, want):
+        assert torch.equal(a, b), name
+        assert not a[:ascending[0]].any() and not a[ascending[-1]:].any(), name
+    spans = [(slice(a, b),) for a, b in zip(ascending, ascending[1:]) if b > a]
+    check(functional, q, k, v, g, True, spans, cu_seqlens=torch.tensor(offsets, dtype=kind, device="cuda"))
 
 
 # ------------------------------------------------------------------------------------------------
