@@ -206,3 +206,42 @@ def test_few_keys_in_padded_rows(functional, causal, heads, kv_heads, width, len
         q[i, n:], k[i, n:], v[i, n:], g[i, n:] = math.nan, math.inf, math.nan, -math.inf
     check(functional, q, k, v, g, causal, [(i, slice(0, n)) for i, n in enumerate(lengths)], exact_rows=32,
           lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+
+
+# ------------------------------------------------------------------------------------------------
+# dk and dv in parts; whole (sequence, head) pairs dealt to the XCDs
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("causal,lengths,heads,kv_heads,width", [
+    (True, [1030], 32, 1, 72), (False, [1030], 32, 1, 96), (True, [1030], 64, 2, 128), (False, [1030, 1, 517], 32, 1, 128),
+    (True, [1030, 0, 129, 1029], 32, 1, 64), (False, [0, 700], 32, 1, 32)])
+def test_dk_dv_in_parts(functional, dtype, causal, lengths, heads, kv_heads, width):
+    """Dense and padded batches whose dk and dv are summed from parts, NaN behind the tokens."""
+    from kronfluence_amd import _native
+
+    batch, length = len(lengths), 1030
+    call = (batch, length, batch * length, heads, kv_heads, width, 0, int(causal))
+    delta = (batch * length * heads * 4 + 15) // 16 * 16
+    whole = 2 * kv_heads * batch * length * width * 4
+    parts, rest = divmod(_native.lib().kf_attention_backward_workspace_bytes(*call) - delta, whole)
+    assert rest == 0 and parts >= 2
+    q, k, v, g = (make((batch, length, n, width), dtype, seed, scale)
+                  for n, seed, scale in ((heads, 1, 1.5), (kv_heads, 2, 1.0), (kv_heads, 3, 1.0), (heads, 4, 0.1)))
+    for i, n in enumerate(lengths):
+        q[i, n:], k[i, n:], v[i, n:], g[i, n:] = math.nan, math.inf, math.nan, -math.inf
+    padded = {} if lengths == [length] else {"lengths": torch.tensor(lengths, dtype=torch.int32, device="cuda")}
+    check(functional, q, k, v, g, causal, [(i, slice(0, n)) for i, n in enumerate(lengths) if n], **padded)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("causal,batch,length,heads,kv_heads,width", [(True, 33, 300, 4, 2, 64), (False, 16, 129, 4, 4, 128), (True, 70, 200, 2, 1, 32),
+                                                                      (False, 66, 257, 1, 1, 72), (True, 9, 520, 16, 8, 64)])
+def test_pairs_dealt_to_the_xcds(functional, dtype, causal, batch, length, heads, kv_heads, width):
+    """At least 64 (sequence, key / value head) pairs: blocks of pairs of one XCD, more and fewer than a multiple of eight."""
+    lengths = [max(0, length - 37 * (i % 8)) if i % 5 else length for i in range(batch)]
+    q, k, v, g = (make((batch, length, n, width), dtype, seed, scale)
+                  for n, seed, scale in ((heads, 1, 1.5), (kv_heads, 2, 1.0), (kv_heads, 3, 1.0), (heads, 4, 0.1)))
+    for i, n in enumerate(lengths):
+        q[i, n:], k[i, n:], v[i, n:], g[i, n:] = math.nan, math.inf, math.nan, -math.inf
+    check(functional, q, k, v, g, causal, [(i, slice(0, n)) for i, n in enumerate(lengths) if n],
+          lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"))
