@@ -26,6 +26,8 @@ from kronfluence_amd import _native as nat
 
 __all__ = ["attention", "layer_norm", "rms_norm"]
 
+_AUTOCAST = (torch.float32, torch.bfloat16, torch.float16)   # what autocast casts: float64 and integers stay, and are refused as outside of it
+
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = True, scale: Optional[float] = None,
               lengths: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -47,7 +49,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     """
     if torch.is_autocast_enabled("cuda") and q.is_cuda:
         dtype = torch.get_autocast_dtype("cuda")
-        q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+        q, k, v = (t.to(dtype) if t.dtype in _AUTOCAST else t for t in (q, k, v))
     return nat.autograd().attention(q, k, v, bool(causal), scale, lengths, cu_seqlens)
 
 

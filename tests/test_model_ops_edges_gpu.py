@@ -245,3 +245,14 @@ def test_pairs_dealt_to_the_xcds(functional, dtype, causal, batch, length, heads
         q[i, n:], k[i, n:], v[i, n:], g[i, n:] = math.nan, math.inf, math.nan, -math.inf
     check(functional, q, k, v, g, causal, [(i, slice(0, n)) for i, n in enumerate(lengths) if n],
           lengths=torch.tensor(lengths, dtype=torch.int32, device="cuda"))
+
+
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float64, torch.int64])
+def test_autocast_casts_no_other_types(functional, dtype):
+    """As torch's operators under autocast: float64 is not rounded to bf16 on the way in, an integer is no head."""
+    from kronfluence_amd._native import KfError
+
+    q = torch.ones(1, 5, 1, 8, dtype=dtype, device="cuda")
+    with torch.autocast("cuda", torch.bfloat16), pytest.raises(KfError, match="bfloat16 or float32"):
+        functional.attention(q, q, q)
