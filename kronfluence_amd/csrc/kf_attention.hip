@@ -18,7 +18,8 @@
 // fp32 runs on the same bf16 instructions: every value is split into three bf16 parts, exactly, and a product is six products of parts
 // (struct Split) -- 6/16 of the time of v_mfma_f32_32x32x2_f32 at fp32's accuracy.  Measured against that instruction in the same
 // kernels: 64 x 256 x 12 heads x 64, forward 131 to 84 us, backward 470 to 325; 2 x 2048 x 16 x 128 causal, 334 to 223 and 1129 to 817.
-// Finite values from 3.39e38 on (their first part rounds to infinity) act as infinities, parts below 2^-126 as 0.
+// Infinities, and finite values from 3.39e38 on (their first part rounds to infinity), give NaN (inf - inf in the split); parts below 2^-126
+// count as 0.
 //
 // Measured (us; causal but for the first; forward, dq, dk / dv): bf16 256 x <= 128 x 12 heads x 64, padded: 38, all of the backward 83 (latency
 // of one-tile sequences); 64 x 512 x 12 x 64: 68, 86, 97 and 16 x 512 x 32/8 x 128: 80, 114, 126 (vector instructions of the
@@ -83,7 +84,8 @@ struct Args {
 
 // ---- element types ---------------------------------------------------------------------------------------------------------
 // fp32 whose products are sums of bf16 products: every value is exactly the sum of three bf16 parts (8 + 8 + 8 bits), and of the nine
-// products of parts the six greater ones are taken -- the three left out are below 2^-26 of the whole, a quarter of fp32's half step.
+// products of parts the six greater ones are taken.  Part 1 is at most 2^-8 of the value's power of two and part 2 2^-17, so that the three left
+// out come to 2^-24 of the product at most, as one more rounding of it would (below 2^-26 for 97 % of random pairs).
 struct Split { float value; };
 
 template <class T>

@@ -43,7 +43,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
 
     Rows of no sequence (padding; packed rows in front of the first offset or behind the last) are 0 in the output and in every gradient, whatever the inputs
     hold there.  An infinity or NaN at a REAL token may reach every row of its sequence, as it does in the plain formula (0 * inf); float32
-    values from 3.39e38 on count as infinite, and below 1e-33 their last bits may be lost.
+    infinities and values from 3.39e38 on give NaN there, and below 1e-33 the last bits may be lost.
     ``scale`` is positive and ``1 / sqrt(width)`` by default.  A bfloat16 call with a graph keeps, beside q, k, v and the output, 8 bits per
     output element for its backward pass.
     """
