@@ -1190,6 +1190,8 @@ __global__ __launch_bounds__(THREADS) void attention_join_kernel(const Args a) {
 //   dk / dv: 32 queries, three waves: A 102 (64 queries, in registers for one wave: 231); width 32 64 queries: all of the backward C 135 (146)
 //   v from LDS (VL): A 102 (v in registers: 120), B 131 (213); width 96 has the registers
 //   fp32: three, two and two waves: D 27, 36, 44 (two, one and one: 28.5, 38, 62); above width 64 the parts' registers leave one
+// What these choices spill: dk / dv bf16 at width 128 10 vector registers (24 bytes of scratch a lane), fp32 at width 64 5 (24 bytes) and at
+// width 128 36 (148 bytes); the one-kernel backward 25 to 28 scalar registers, into vector ones.
 template <class T, int DP>
 struct Shape {
     static constexpr bool SHORT = PARTS<T> == 1 && DP <= 64;   // wider heads and split values leave the LDS no room for two workgroups
@@ -1283,6 +1285,10 @@ int64_t delta_bytes(int64_t rows, int64_t heads) { return (rows * heads * 4 + 15
 // largest item.  Measured (bf16, causal, width 128): one document of 8192 tokens, 32/8 heads, 512 items: 1867 us whole, 1138 + 28 us
 // (join) in two parts, 1135 + 58 in four; 24 documents of 12011 tokens in all, 16/4 heads, 472 items: 425 us whole, 235 + 21 in two,
 // 159 + 36 in four; 16 x 512 tokens, 32/8 heads, 512 items of at most 64 steps: 128 us whole, 108 + 30 in two.
+// A part of at least 128 steps (all of the backward, us; at least 64, at least 256): 1 x 2048 x 8/2 x 128 274 (180, 459), 1 x 2048 x 32/4 x 64 175
+// (175, 281), 1 x 8192 x 8 x 64 360 (360, 419), 2 x 2048 x 16 x 64 136 (137, 137).  The lengths of packed documents are not known here,
+// and their steps are counted as if all rows were one: right for 41 of 100 to 2000 tokens, 16/4 heads x 128 (198 us, whole 461), a loss for short ones
+// (64 of 128 tokens, 16/4 x 128: 118 us, whole 81; 96 of 64, 12/4 x 64: 51 and 32).
 int64_t dkv_parts(int64_t sequences, int64_t length, int64_t rows, int64_t heads, int64_t kv_heads, bool packed, bool causal) {
     const int64_t items = tile_slots(sequences, length, rows, packed) * kv_heads, steps = ((packed ? rows : length) + 31) / 32 * (heads / kv_heads);
     const int64_t wanted = ((packed ? 2048 : causal ? 1024 : 512) + items - 1) / items;
@@ -1316,6 +1322,9 @@ int fill(Args& a, int dtype, int64_t sequences, int64_t length, int64_t rows, in
     if (offsets ? lengths != nullptr : (length <= 0 || sequences > limit / length || rows != sequences * length)) return KF_ERR_INVALID_ARGUMENT;
     const int64_t slots = tile_slots(sequences, length, rows, offsets != nullptr) + (offsets != nullptr);
     const int64_t tiles = offsets ? 0 : slots / sequences, groups = offsets ? 0 : sequences * kv_heads;
+    // Whole pairs from 64 on (all of the backward, us, causal bf16; single tiles in brackets): 8 x 2048 x 8 x 64 158 (211), 16 x 512 x 8 x 64 44
+    // (49), 64 x 512 x 2/1 x 64 55 (57); fewer pairs of few tiles are even: 4 x 512 x 8/4 x 128 80 (79), 2 x 2048 x 8 x 64 113 (113), and at
+    // 32 pairs of many tiles whole ones would gain: 4 x 2048 x 8 x 64 122 (138).
     const int64_t chunk = groups >= 64 ? tiles : 1;
     if (sequences >= limit || slots > (limit / MAX_PARTS - XCDS * chunk * heads) / heads) return KF_ERR_INVALID_ARGUMENT;
     a.chunk = static_cast<int>(chunk);
