@@ -50,6 +50,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
@@ -133,9 +134,12 @@ struct Type<float> {                           // (the partial sums of the dk / 
 // ascend with their magnitude, so that the difference needs no look at the exponent.)
 struct Low {
     int8_t byte;
-    static __device__ __forceinline__ uint32_t of(float x) {
-        const int below = static_cast<int>(__float_as_uint(x) - (static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<__bf16>(x))) << 16));
-        return static_cast<uint32_t>(min(below + 0x80, 0x7fff) >> 8) & 0xff;
+    // The low halves of two floats as signed numbers are what their roundings leave off, but for the tie 0x8000 that rounds down (to an even
+    // high half): one less there, and anywhere the high half is even, is 0x7fff.  Rounded to a byte with saturation, in the byte's place.
+    static __device__ __forceinline__ uint32_t two(float x, float y) {
+        const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+        const uint32_t low = __builtin_amdgcn_perm(b, a, 0x05040100), even = ~__builtin_amdgcn_perm(b, a, 0x07060302) & 0x00010001;
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_add_sat(__builtin_bit_cast(s16x2, low) - __builtin_bit_cast(s16x2, even), s16x2{0x80, 0x80}));
     }
     static __device__ __forceinline__ float join(__bf16 high, uint32_t low, int byte) {   // byte `byte` of `low`
         return __uint_as_float((static_cast<uint32_t>(__builtin_bit_cast(uint16_t, high)) << 16) + ((static_cast<int32_t>(low << (24 - 8 * byte)) >> 24) << 8));
@@ -146,7 +150,7 @@ __host__ __device__ constexpr int64_t rest_width(int64_t width) { return (width 
 template <>
 struct Type<Low> {
     static __device__ __forceinline__ void store4(void* p, float a, float b, float c, float d) {
-        *reinterpret_cast<uint32_t*>(p) = Low::of(a) | Low::of(b) << 8 | Low::of(c) << 16 | Low::of(d) << 24;
+        *reinterpret_cast<uint32_t*>(p) = __builtin_amdgcn_perm(Low::two(c, d), Low::two(a, b), 0x07050301);
     }
 };
 
