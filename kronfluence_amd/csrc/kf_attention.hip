@@ -31,8 +31,8 @@
 // Neither rounding may enter D, which a peaked row's gradients are far below (a key that outweighs all others: p -> 1, ds -> 0).  So o is
 // divided by the sum of the ROUNDED p, and the forward pass keeps the next eight bits of o (at most 2^-15 of it is left): with e_j the
 // relative error of p_j, do_i . o_i is then off by sum_j p_j (e_j - sum_k p_k e_k) do_i . v_j = sum_j e_j ds_j, no more than dS's own rounding.
-// Measured against 64 bits, dq of 128 keys with scores of a standard deviation of 12: 0.30 % of its norm (0.28 % with the exact D, 0.71 %
-// from the rounded o over the sum of p alone); with one key 20 above the others nothing of the gradient was right.
+// Measured against 64 bits, dq as a part of its norm (with the rounded o over the sum of p in brackets): 128 keys, scores with a standard deviation of
+// 12, 0.24 % (0.64); one key 10 above 511 others 0.24 % (1.6), 20 above 1.7 % (57; what is left is fp32's); usual scores 0.24 % (0.24).
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
