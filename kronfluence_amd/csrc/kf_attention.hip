@@ -694,7 +694,8 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_forward_kernel(const
     if constexpr (PARTS<T> == 1) {
         static_assert(Pass<Low, DP>::STRIDE <= Pass<T, DP>::STRIDE, "in the same piece of the scratch as the wave's rows before");
         if (a.rest.p)
-            store_rows<Low, DP>(acc, lds + wave * 32 * (Pass<T, DP>::STRIDE - Pass<Low, DP>::STRIDE), rows_out<Low>(a.rest, w, head), a.rest.token, first, w.length, static_cast<int>(rest_width(a.width)), 1.0f, wave, lane);
+            store_rows<Low, DP>(acc, lds + wave * 32 * (Pass<T, DP>::STRIDE - Pass<Low, DP>::STRIDE), rows_out<Low>(a.rest, w, head), a.rest.token, first,
+                                w.length, static_cast<int>(rest_width(a.width)), 1.0f, wave, lane);
     }
     if (lse && half == 0 && query < w.written) lse[query] = real ? top + __builtin_amdgcn_logf(sum) : INFINITY;
 }
@@ -987,7 +988,7 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
 // and meets all queries, as in the dk / dv kernel, leaving ds in LDS as [key][query]; then 32 queries again, and dq is the product of two
 // transposed reads.  Seven products as in the two kernels, but the inputs are read once and o not at all.  Measured (backward, bf16, causal, 12 heads
 // x 64; the two kernels in brackets): 256 x 128 tokens 96 us (132), 512 x 64 112 (140), 1024 x 33 198 (224); 256 x 128 x 12 x 32 58 (93).
-// Bound by latency: LDS and registers leave room for two workgroups, and each is load, products, store one after the other.
+// Rows of 32 and fewer (1024 x 32: 193) stay with the two kernels, which need no low bytes there.  Bound by latency: LDS and registers leave room for two workgroups, and each is load, products, store one after the other.
 template <int DP>
 struct Short {
     typedef Image<__bf16, DP, ROWS> Img;       // q, do, k
