@@ -988,7 +988,8 @@ __global__ __launch_bounds__(THREADS, WAVES) void attention_dkv_kernel(const Arg
 // and meets all queries, as in the dk / dv kernel, leaving ds in LDS as [key][query]; then 32 queries again, and dq is the product of two
 // transposed reads.  Seven products as in the two kernels, but the inputs are read once and o not at all.  Measured (backward, bf16, causal, 12 heads
 // x 64; the two kernels in brackets): 256 x 128 tokens 96 us (132), 512 x 64 112 (140), 1024 x 33 198 (224); 256 x 128 x 12 x 32 58 (93).
-// Rows of 32 and fewer (1024 x 32: 193) stay with the two kernels, which need no low bytes there.  Bound by latency: LDS and registers leave room for two workgroups, and each is load, products, store one after the other.
+// Rows of 32 and fewer (1024 x 32: 193) stay with the two kernels, which need no low bytes there.  Bound by latency: LDS and registers
+// leave room for two workgroups, and each is load, products, store one after the other.
 template <int DP>
 struct Short {
     typedef Image<__bf16, DP, ROWS> Img;       // q, do, k

@@ -39,10 +39,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
 
     ``lengths`` (``[batch]``, int32 / int64 on the device) counts the real tokens of each row, the first ones; ``cu_seqlens``
     (``[sequences + 1]``, the first row of every sequence and the last one's end, ascending) cuts a packed batch.  Entries are clamped to
-    the rows that exist, and an offset below one before it counts as that one (its sequence is empty); neither is read by the host.  A token sees the tokens of its own sequence, with ``causal`` those up to itself.
+    the rows that exist, and an offset below one before it counts as that one (its sequence is empty); neither is read by the host.  A
+    token sees the tokens of its own sequence, with ``causal`` those up to itself.
 
-    Rows of no sequence (padding; packed rows in front of the first offset or behind the last) are 0 in the output and in every gradient, whatever the inputs
-    hold there.  An infinity or NaN at a REAL token may reach every row of its sequence, as it does in the plain formula (0 * inf); float32
+    Rows of no sequence (padding; packed rows in front of the first offset or behind the last) are 0 in the output and in every gradient,
+    whatever the inputs hold there.  An infinity or NaN at a REAL token may reach every row of its sequence, as it does in the plain formula (0 * inf); float32
     infinities and values from 3.39e38 on give NaN there, and below 1e-33 the last bits may be lost.
     ``scale`` is positive and ``1 / sqrt(width)`` by default.  A bfloat16 call with a graph keeps, beside q, k, v and the output, 8 bits per
     output element for its backward pass.
